@@ -647,6 +647,102 @@ mf_status mf_moe_unpermute(mf_moe* h, mf_stream stream, const float* route_parti
                            const float* route_weights, const uint32_t* idx, const uint16_t* residual,
                            uint32_t t, uint16_t* y);
 
+/* ------------------------------------------- low-rank adapters, block norms */
+
+/* A server that runs one set of quantized weights for many requests gives every request a small correction of its own: the
+ * projection W x of a row becomes W x + c_a B_a (A_a x), a = the row's adapter, A_a [rank, n] and B_a [m, rank] bf16.  The calls
+ * below add those corrections, for all rows of a batch at once, to results that mf_gemv, mf_qmm or mf_shared_expert left.
+ * No counterpart in the reference, which runs one model for one user. */
+#define MF_MAX_ADAPTERS 1024
+#define MF_MAX_ADAPTER_RANK 256
+#define MF_MAX_ADAPTER_TARGETS 4
+
+/* The adapters a device holds.  Adapter a has ranks[a] live rows in every A_a and columns in every B_a (at most `rank`, what it
+ * has room for); what lies beyond them is never used, whatever it holds.  The values may be changed between calls: an adapter is
+ * swapped by writing its part of the pool, its rank and its scale. */
+typedef struct {
+  uint32_t num_adapters;  /* 1 .. MF_MAX_ADAPTERS */
+  uint32_t rank;          /* a multiple of 8, 8 .. MF_MAX_ADAPTER_RANK */
+  uint32_t n;             /* length of a row of x, a multiple of 64 */
+  const uint32_t* ranks;  /* device [num_adapters], values 0 .. rank (larger ones count as rank); NULL: all `rank` */
+  const float* scales;    /* device [num_adapters], c_a; NULL: all 1 */
+} mf_adapter_pool;
+
+/* One of the projections that read the same x (gate and up; or one alone). */
+typedef struct {
+  const uint16_t* a;  /* bf16 [num_adapters, rank, n], 16-byte aligned */
+  const uint16_t* b;  /* bf16 [num_adapters, m, rank], 16-byte aligned */
+  void* y;            /* the projection's result, row i at element i * y_stride: updated in place */
+  uint32_t m;         /* any, from 1 on */
+  uint32_t y_stride;  /* >= m */
+} mf_adapter_target;
+
+/* The rows of a batch in the order of their adapters, found on the device with no host readback (as mf_moe_group does for
+ * routes; no counterpart in the reference).  adapter_of_row int32 [t]; a row whose value is not in [0, num_adapters) has no
+ * adapter.  plan: mf_adapter_plan_bytes(t, num_adapters) bytes, 16-byte aligned, which afterwards hold as uint32
+ *   [0, t)                          row numbers, stably sorted by adapter, rows without one last
+ *   [t, t + num_adapters + 1)       where each adapter's rows start in that list; the last entry: where the rows without one do
+ * and behind that what mf_adapter_apply reads.  One plan serves every mf_adapter_apply of the same rows, whatever the
+ * projection: a step makes it once.  t = 0 is a batch without rows; t <= MF_MAX_ROWS.  The sizes are 0 for arguments that the
+ * call refuses. */
+size_t mf_adapter_plan_bytes(uint32_t t, uint32_t num_adapters);
+mf_status mf_adapter_group(mf_ctx* ctx, mf_stream stream, const int32_t* adapter_of_row, uint32_t t, uint32_t num_adapters,
+                           uint32_t* plan, size_t plan_bytes);
+
+/* y_s[i, :] = narrow(y_s[i, :] + c_a * B_s,a (A_s,a x[i, :])) for every row i of the batch that has an adapter a, and every
+ * target s; rows without one keep their bits.  No counterpart in the reference.  x bf16, row i at element i * x_stride
+ * (x_stride >= n); y bf16, or fp32 when y_f32 != 0.  The sums and A x are held in fp32; for the second product A x is cut into
+ * bf16 terms, two for bf16 results (2^-16 of the correction), three for fp32 ones (all of its bits).
+ * plan: NULL, or what mf_adapter_group left for the same adapter_of_row, t and num_adapters.  Without one the rows are taken as
+ * they lie: right for rows whose neighbours share an adapter (prompts, one request, few rows); a batch that mixes many adapters
+ * is faster with one.  A row's result may differ in its last bits between batches of other sizes and between the two ways (the
+ * sum over n is cut differently), never between two equal calls.
+ * workspace: mf_adapter_workspace_bytes bytes, 16-byte aligned (they serve every smaller t too).  x and the ys are faster when
+ * 16-byte aligned with strides that are multiples of 8.  No y may share memory with x or with another y, column ranges of one
+ * buffer excepted (MF_ERR_INVALID_ARGUMENT).  t = 0 does nothing; t <= MF_MAX_ROWS.  An infinity or a NaN of x stays with its
+ * row; one in an adapter's live weights makes the results it meets infinite or NaN.  Forward only: the library has no gradients. */
+size_t mf_adapter_workspace_bytes(const mf_adapter_pool* pool, uint32_t num_targets, uint32_t t);
+mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool* pool, const mf_adapter_target* targets,
+                           uint32_t num_targets, const uint16_t* x, uint32_t x_stride, const int32_t* adapter_of_row, uint32_t t,
+                           int y_f32, const uint32_t* plan, void* workspace, size_t workspace_bytes);
+
+/* What multiplies a block's output on its way into the stream. */
+typedef enum {
+  MF_GATE_NONE = 0,
+  MF_GATE_ROW = 1,     /* sigmoid of one bf16 logit a row: gate [t], entry i at i * gate_stride (0: 1) -- mf_sigmoid_scalar_mul's gate */
+  MF_GATE_ELEMENT = 2, /* sigmoid of one bf16 logit an element: gate [t, d] */
+  MF_GATE_CHANNEL = 3  /* one bf16 factor a channel, as it is: gate [d] */
+} mf_gate_kind;
+
+typedef struct {
+  uint16_t* hidden;             /* bf16 [t, d]: the stream, updated in place */
+  const void* delta;            /* [t, d]: the block's output, bf16, or fp32 when delta_f32 != 0; NULL: none, the stream is only read */
+  const uint16_t* gate;         /* as gate_kind says, else NULL */
+  const uint16_t* post_weight;  /* bf16 [d]: the norm behind the block; NULL: none */
+  const uint16_t* pre_weight;   /* bf16 [d]: the norm in front of the next one; NULL: none (out is NULL too) */
+  uint16_t* out;                /* bf16 [t, d] */
+  uint32_t d, t;
+  uint32_t hidden_stride, delta_stride, gate_stride, out_stride; /* elements from row to row; 0: d */
+  int delta_f32;
+  mf_gate_kind gate_kind;
+  float post_eps, pre_eps;
+  float residual_scale, branch_scale; /* usually 1 */
+  float weight_bias;                  /* added to both norms' weights: 1 where a model stores them as differences from one */
+} mf_block_norm_args;
+
+/* Everything between two blocks of a layer, one launch and one pass over the rows: with
+ *   b = delta * rsqrt(mean(delta^2) + post_eps) * (post_weight + weight_bias)     (delta itself without post_weight)
+ * times its gate,
+ *   hidden = narrow(residual_scale * hidden + branch_scale * b)
+ *   out    = narrow(hidden * rsqrt(mean(hidden^2) + pre_eps) * (pre_weight + weight_bias))
+ * RMSNorm.encodeBF16W and Elementwise.encodeResidualAdd (Kernels/Primitives/RMSNorm.swift:52-64, Elementwise.swift:60-87) as
+ * mf_residual_rmsnorm joins them, with the norm behind the block (the layers that have one: one norm on either side of attention and
+ * MLP), the gate and the scales.  fp32 between the roundings named; as in mf_residual_rmsnorm the second norm is of the narrowed
+ * stream.  The two calls add the squares of a row in different orders.  out may share no memory with hidden, delta or gate, hidden
+ * none with delta or gate (MF_ERR_INVALID_ARGUMENT).  Any d >= 1; t = 0 does nothing; t <= MF_MAX_ROWS.  Faster where all
+ * tensors are 16-byte aligned and d and the strides are multiples of 8. */
+mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args* args);
+
 #ifdef __cplusplus
 }
 #endif

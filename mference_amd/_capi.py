@@ -20,6 +20,11 @@ STATIC_ACT_ELEMS = MAX_TOKENS * 32768  # MF_STATIC_ACT_ELEMS
 BITS_TERNARY, BITS_2, BITS_4, BITS_8 = 1, 2, 4, 8
 ROUTER_TOPK_SOFTMAX, ROUTER_FULL_SOFTMAX = 0, 1
 
+MAX_ADAPTERS = 1024        # MF_MAX_ADAPTERS
+MAX_ADAPTER_RANK = 256     # MF_MAX_ADAPTER_RANK
+MAX_ADAPTER_TARGETS = 4    # MF_MAX_ADAPTER_TARGETS
+GATE_NONE, GATE_ROW, GATE_ELEMENT, GATE_CHANNEL = 0, 1, 2, 3
+
 STATUS_NAMES = {
     0: "MF_OK", -1: "MF_ERR_INVALID_ARGUMENT", -2: "MF_ERR_DIMENSION_MISMATCH",
     -3: "MF_ERR_UNSUPPORTED_BITS", -4: "MF_ERR_SCRATCH_TOO_SMALL", -5: "MF_ERR_NO_DEVICE",
@@ -64,6 +69,26 @@ class LayerWeights(C.Structure):
 class Pair(C.Structure):
     _fields_ = [("token", C.c_uint32), ("expert", C.c_uint32), ("rank", C.c_uint32),
                 ("weight_bits", C.c_uint32)]
+
+
+class AdapterPool(C.Structure):
+    """mf_adapter_pool"""
+    _fields_ = [("num_adapters", C.c_uint32), ("rank", C.c_uint32), ("n", C.c_uint32),
+                ("ranks", C.c_void_p), ("scales", C.c_void_p)]
+
+
+class AdapterTarget(C.Structure):
+    """mf_adapter_target"""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("y", C.c_void_p), ("m", C.c_uint32), ("y_stride", C.c_uint32)]
+
+
+class BlockNormArgs(C.Structure):
+    """mf_block_norm_args"""
+    _fields_ = [("hidden", C.c_void_p), ("delta", C.c_void_p), ("gate", C.c_void_p), ("post_weight", C.c_void_p),
+                ("pre_weight", C.c_void_p), ("out", C.c_void_p), ("d", C.c_uint32), ("t", C.c_uint32),
+                ("hidden_stride", C.c_uint32), ("delta_stride", C.c_uint32), ("gate_stride", C.c_uint32), ("out_stride", C.c_uint32),
+                ("delta_f32", C.c_int), ("gate_kind", C.c_int), ("post_eps", C.c_float), ("pre_eps", C.c_float),
+                ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("weight_bias", C.c_float)]
 
 
 # every entry point include/mfmoe.h declares: name -> (restype, argtypes)
@@ -120,6 +145,11 @@ SIGNATURES = {
     "mf_moe_phase2_slots": (_I, [_P, _P, _P, _P, _P, C.POINTER(ExpertOffsets), _P, _P, _P, _U32, _P]),
     "mf_moe_ragged_qmm": (_I, [_P, _P, _P, _SZ, C.POINTER(ExpertOffsets), _P, _P, _P, _U32, _P, _P, _SZ]),
     "mf_moe_unpermute": (_I, [_P, _P, _P, _P, _P, _P, _U32, _P]),
+    "mf_adapter_plan_bytes": (_SZ, [_U32, _U32]),
+    "mf_adapter_group": (_I, [_P, _P, _P, _U32, _U32, _P, _SZ]),
+    "mf_adapter_workspace_bytes": (_SZ, [C.POINTER(AdapterPool), _U32, _U32]),
+    "mf_adapter_apply": (_I, [_P, _P, C.POINTER(AdapterPool), C.POINTER(AdapterTarget), _U32, _P, _U32, _P, _U32, _I, _P, _P, _SZ]),
+    "mf_block_norm": (_I, [_P, _P, C.POINTER(BlockNormArgs)]),
     "mf_group_pairs_host": (_I, [_P, _SZ, _I, _I, _I, _I, _P, _SZ, _P, _P, _P, _P,
                                  C.POINTER(_SZ), _P, C.POINTER(_SZ), _P]),
 }

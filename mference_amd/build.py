@@ -11,7 +11,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libmfmoe.so")
 SOURCES = ["format.hip", "gemv.hip", "int8_mlp.hip", "router.hip", "router_family.hip", "moe_decode.hip", "moe_fused.hip",
-           "moe_prefill.hip", "qmm_ring.hip", "qmm_resident.hip", "qmm_tile32.hip", "static_scratch.hip", "api.hip"]
+           "moe_prefill.hip", "qmm_ring.hip", "qmm_resident.hip", "qmm_tile32.hip", "static_scratch.hip", "adapters.hip", "block_norm.hip", "api.hip"]
 
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

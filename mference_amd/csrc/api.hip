@@ -7,6 +7,7 @@
 #include <new>
 #include <vector>
 
+#include "mf_adapters.h"
 #include "mf_internal.h"
 #include "mf_qmm.h"
 
@@ -945,6 +946,164 @@ mf_status mf_group_pairs_host(const mf_pair* pairs, size_t n_pairs, int query_co
   }
   *n_groups = ng;
   *n_tiles = nt;
+  return MF_OK;
+}
+
+/* ------------------------------------------- low-rank adapters, block norms */
+
+namespace {
+
+// The calls below may be made with any device current: the context's is, while one runs.
+class OnDevice {
+ public:
+  explicit OnDevice(const mf_ctx* ctx) {
+    if (hipGetDevice(&before_) == hipSuccess && before_ == ctx->device) before_ = -1;
+    else error_ = hipSetDevice(ctx->device);
+  }
+  ~OnDevice() {
+    if (before_ >= 0) (void)hipSetDevice(before_);
+  }
+  hipError_t error() const { return error_; }
+
+ private:
+  int before_ = -1;
+  hipError_t error_ = hipSuccess;
+};
+
+// rows of `width` bytes, `stride` bytes apart
+struct Rows {
+  const void* p;
+  uint64_t stride, width;
+};
+
+// Whether two sets of t rows can share a byte: not where their ranges are apart, nor where they are column ranges of one
+// buffer (rows of one stride) that are apart.
+bool rows_meet(const Rows& a, const Rows& b, uint64_t t) {
+  const auto pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+  if (pa + (t - 1) * a.stride + a.width <= pb || pb + (t - 1) * b.stride + b.width <= pa) return false;
+  if (a.stride != b.stride || t == 1) return true;
+  const uint64_t from_a = pb >= pa ? (pb - pa) % a.stride : (a.stride - (pa - pb) % a.stride) % a.stride;  // b's first column behind a's
+  return from_a < a.width || from_a + b.width > a.stride;
+}
+
+bool adapter_pool_ok(const mf_adapter_pool* p) {
+  return p && p->num_adapters >= 1 && p->num_adapters <= MF_MAX_ADAPTERS && p->rank >= 8 && p->rank <= MF_MAX_ADAPTER_RANK &&
+         p->rank % 8 == 0 && p->n > 0 && p->n % MF_GROUP_SIZE == 0;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+}  // namespace
+
+size_t mf_adapter_plan_bytes(uint32_t t, uint32_t num_adapters) {
+  if (t > MF_MAX_ROWS || num_adapters == 0 || num_adapters > MF_MAX_ADAPTERS) return 0;
+  return mf::AdapterPlan::words(t, num_adapters) * sizeof(uint32_t);
+}
+
+mf_status mf_adapter_group(mf_ctx* ctx, mf_stream stream, const int32_t* adapter_of_row, uint32_t t, uint32_t num_adapters,
+                           uint32_t* plan, size_t plan_bytes) {
+  if (!ctx || (!adapter_of_row && t) || !plan) return MF_ERR_INVALID_ARGUMENT;
+  if (t > MF_MAX_ROWS || num_adapters == 0 || num_adapters > MF_MAX_ADAPTERS) return MF_ERR_INVALID_ARGUMENT;
+  if (!mf::aligned16(plan) || !aligned4(adapter_of_row)) return MF_ERR_INVALID_ARGUMENT;
+  const size_t need = mf::AdapterPlan::words(t, num_adapters) * sizeof(uint32_t);
+  if (plan_bytes < need) return MF_ERR_SCRATCH_TOO_SMALL;
+  if (t && rows_meet({adapter_of_row, 4, static_cast<uint64_t>(t) * 4}, {plan, 1, need}, 1)) return MF_ERR_INVALID_ARGUMENT;
+  const OnDevice on(ctx);
+  MF_HIP(ctx, on.error());
+  MF_HIP(ctx, mf::launch_adapter_group(static_cast<hipStream_t>(stream), adapter_of_row, t, num_adapters, plan));
+  return MF_OK;
+}
+
+size_t mf_adapter_workspace_bytes(const mf_adapter_pool* pool, uint32_t num_targets, uint32_t t) {
+  if (!adapter_pool_ok(pool) || num_targets == 0 || num_targets > MF_MAX_ADAPTER_TARGETS || t > MF_MAX_ROWS) return 0;
+  return mf::adapter_workspace_bytes(num_targets, pool->rank, pool->n, t);
+}
+
+mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool* pool, const mf_adapter_target* targets,
+                           uint32_t num_targets, const uint16_t* x, uint32_t x_stride, const int32_t* adapter_of_row, uint32_t t,
+                           int y_f32, const uint32_t* plan, void* workspace, size_t workspace_bytes) {
+  if (!ctx || !pool || !targets) return MF_ERR_INVALID_ARGUMENT;
+  if (!adapter_pool_ok(pool)) return MF_ERR_DIMENSION_MISMATCH;
+  if (num_targets == 0 || num_targets > MF_MAX_ADAPTER_TARGETS || t > MF_MAX_ROWS) return MF_ERR_INVALID_ARGUMENT;
+  if ((pool->ranks && !aligned4(pool->ranks)) || (pool->scales && !aligned4(pool->scales))) return MF_ERR_INVALID_ARGUMENT;
+  if (t == 0) return MF_OK;
+  if (!x || !adapter_of_row || !workspace) return MF_ERR_INVALID_ARGUMENT;
+  if (x_stride < pool->n) return MF_ERR_DIMENSION_MISMATCH;
+  if (!mf::aligned2(x) || !aligned4(adapter_of_row) || !mf::aligned16(workspace) || (plan && !mf::aligned16(plan)))
+    return MF_ERR_INVALID_ARGUMENT;
+  const uint32_t size = y_f32 ? 4 : 2;
+  Rows ys[MF_MAX_ADAPTER_TARGETS];
+  const Rows xs = {x, 2ull * x_stride, 2ull * pool->n};
+  mf::AdapterArgs a{};
+  for (uint32_t k = 0; k < num_targets; ++k) {
+    const mf_adapter_target& g = targets[k];
+    if (!g.a || !g.b || !g.y) return MF_ERR_INVALID_ARGUMENT;
+    if (g.m == 0 || g.y_stride < g.m) return MF_ERR_DIMENSION_MISMATCH;
+    if (!mf::aligned16(g.a) || !mf::aligned16(g.b) || !(y_f32 ? aligned4(g.y) : mf::aligned2(g.y))) return MF_ERR_INVALID_ARGUMENT;
+    ys[k] = {g.y, static_cast<uint64_t>(size) * g.y_stride, static_cast<uint64_t>(size) * g.m};
+    if (rows_meet(ys[k], xs, t)) return MF_ERR_INVALID_ARGUMENT;
+    for (uint32_t j = 0; j < k; ++j)
+      if (rows_meet(ys[j], ys[k], t)) return MF_ERR_INVALID_ARGUMENT;
+    a.target[k] = {g.a, g.b, g.y, g.m, g.y_stride};
+  }
+  if (workspace_bytes < mf::adapter_workspace_bytes(num_targets, pool->rank, pool->n, t)) return MF_ERR_SCRATCH_TOO_SMALL;
+  a.ranks = pool->ranks;
+  a.scales = pool->scales;
+  a.x = x;
+  a.ids = adapter_of_row;
+  a.v = static_cast<float*>(workspace);
+  a.num_targets = num_targets;
+  a.num_adapters = pool->num_adapters;
+  a.rank = pool->rank;
+  a.n = pool->n;
+  a.t = t;
+  a.x_stride = x_stride;
+  a.cols = num_targets * pool->rank;
+  const OnDevice on(ctx);
+  MF_HIP(ctx, on.error());
+  MF_HIP(ctx, mf::launch_adapter_apply(static_cast<hipStream_t>(stream), a, y_f32 != 0));
+  return MF_OK;
+}
+
+mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args* args) {
+  if (!ctx || !args) return MF_ERR_INVALID_ARGUMENT;
+  mf_block_norm_args a = *args;
+  if (a.d == 0) return MF_ERR_DIMENSION_MISMATCH;
+  if (a.t > MF_MAX_ROWS || a.gate_kind < MF_GATE_NONE || a.gate_kind > MF_GATE_CHANNEL) return MF_ERR_INVALID_ARGUMENT;
+  if (a.t == 0) return MF_OK;
+  // a gate or a norm behind the block needs the block's output; the norm in front of the next one needs a place for its result
+  if ((a.gate_kind != MF_GATE_NONE) != (a.gate != nullptr) || (!a.delta && (a.gate || a.post_weight)) ||
+      (a.pre_weight != nullptr) != (a.out != nullptr) || (!a.delta && !a.out))
+    return MF_ERR_INVALID_ARGUMENT;
+  if (!a.hidden) return MF_ERR_INVALID_ARGUMENT;
+  if (!a.hidden_stride) a.hidden_stride = a.d;
+  if (!a.delta_stride) a.delta_stride = a.d;
+  if (!a.out_stride) a.out_stride = a.d;
+  const uint32_t gate_row = a.gate_kind == MF_GATE_ROW ? 1 : a.d;
+  if (!a.gate_stride) a.gate_stride = gate_row;
+  if (a.hidden_stride < a.d || (a.delta && a.delta_stride < a.d) || (a.out && a.out_stride < a.d) ||
+      (a.gate && a.gate_kind != MF_GATE_CHANNEL && a.gate_stride < gate_row))
+    return MF_ERR_DIMENSION_MISMATCH;
+  if (!mf::aligned2(a.hidden) || !mf::aligned2(a.gate) || !mf::aligned2(a.post_weight) || !mf::aligned2(a.pre_weight) ||
+      !mf::aligned2(a.out) || !(a.delta_f32 ? aligned4(a.delta) : mf::aligned2(a.delta)))
+    return MF_ERR_INVALID_ARGUMENT;
+  const uint64_t size = a.delta_f32 ? 4 : 2, d = a.d;
+  const Rows hidden = {a.hidden, 2ull * a.hidden_stride, 2 * d}, delta = {a.delta, size * a.delta_stride, size * d},
+             out = {a.out, 2ull * a.out_stride, 2 * d}, gate = {a.gate, 2ull * a.gate_stride, 2ull * gate_row};
+  // what is written shares nothing with what is read, nor with what else is written
+  const auto meets = [&](const Rows& written) {
+    const uint64_t rows = a.t;
+    if (a.delta && rows_meet(written, delta, rows)) return true;
+    if (a.gate && a.gate_kind != MF_GATE_CHANNEL && rows_meet(written, gate, rows)) return true;
+    const Rows all = {written.p, 1, (rows - 1) * written.stride + written.width};
+    for (const uint16_t* w : {a.pre_weight, a.post_weight, a.gate_kind == MF_GATE_CHANNEL ? a.gate : nullptr})
+      if (w && rows_meet(all, {w, 1, 2 * d}, 1)) return true;
+    return false;
+  };
+  if (meets(hidden) || (a.out && (meets(out) || rows_meet(out, hidden, a.t)))) return MF_ERR_INVALID_ARGUMENT;
+  const OnDevice on(ctx);
+  MF_HIP(ctx, on.error());
+  MF_HIP(ctx, mf::launch_block_norm(static_cast<hipStream_t>(stream), a));
   return MF_OK;
 }
 

@@ -1,0 +1,53 @@
+// The low-rank adapters as api.hip and adapters.hip see them.
+#pragma once
+
+#include "mf_internal.h"
+
+namespace mf {
+
+// mf_adapter_group's words.  Behind the two public lists: four words that say what the plan is of (t, adapters, tiles, rows a
+// tile), and the tiles: runs of at most tile_rows rows of one adapter, x = adapter | rows << 16, y = where its rows start in
+// the list.
+struct AdapterPlan {
+  uint32_t* rows;     // [t]
+  uint32_t* offsets;  // [n + 1]
+  uint32_t* header;   // [4]
+  uint2* tiles;       // [most_tiles]
+  uint32_t tile_rows, most_tiles;
+
+  // rows a tile: what a wave of the products holds at once.  Where a batch has few rows an adapter the wide tiles would be
+  // mostly empty.
+  static uint32_t rows_of_tile(uint32_t t, uint32_t n) { return t / 32 >= n ? 64 : 16; }
+  static uint32_t tiles_of(uint32_t t, uint32_t n) { return t / rows_of_tile(t, n) + (n < t ? n : t); }
+  static size_t header_word(uint32_t t, uint32_t n) { return (static_cast<size_t>(t) + n + 1 + 3) / 4 * 4; }
+  static size_t words(uint32_t t, uint32_t n) { return header_word(t, n) + 4 + 2 * static_cast<size_t>(tiles_of(t, n)); }
+  static AdapterPlan at(uint32_t* p, uint32_t t, uint32_t n) {
+    uint32_t* h = p + header_word(t, n);
+    return {p, p + t, h, reinterpret_cast<uint2*>(h + 4), rows_of_tile(t, n), tiles_of(t, n)};
+  }
+};
+
+struct AdapterArgs {
+  struct Target {
+    const uint16_t* a;
+    const uint16_t* b;
+    void* y;
+    uint32_t m, y_stride;
+  };
+  Target target[MF_MAX_ADAPTER_TARGETS];
+  const uint32_t* ranks;
+  const float* scales;
+  const uint16_t* x;
+  const int32_t* ids;
+  float* v;  // [t, cols]: c_a A x, targets side by side
+  uint32_t num_targets, num_adapters, rank, n, t, x_stride, cols;
+};
+
+hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, uint32_t n, uint32_t* plan);
+size_t adapter_workspace_bytes(uint32_t num_targets, uint32_t rank, uint32_t n, uint32_t t);
+hipError_t launch_adapter_apply(hipStream_t s, const AdapterArgs& a, bool y_f32);
+
+// block_norm.hip
+hipError_t launch_block_norm(hipStream_t s, const mf_block_norm_args& a);
+
+}  // namespace mf

@@ -43,6 +43,8 @@ __device__ __forceinline__ uint16_t f_to_bf16(float x) {
   uint32_t b = __float_as_uint(x);
   return static_cast<uint16_t>((b + 0x7FFFu + ((b >> 16) & 1u)) >> 16);
 }
+// to the nearest bf16, ties to even, a NaN whatever its payload stays one (the conversion instruction's rule)
+__device__ __forceinline__ uint16_t narrow_bf16(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
 __device__ __forceinline__ float round_bf16(float x) { return bf16_to_f(f_to_bf16(x)); }
 
 // ------------------------------------------------------------------- exp

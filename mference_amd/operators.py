@@ -17,7 +17,8 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._capi import (BITS_2, BITS_4, BITS_8, BITS_TERNARY, GROUP_SIZE, MAX_TOKENS, ROUTER_FULL_SOFTMAX,
+from ._capi import (BITS_2, BITS_4, BITS_8, BITS_TERNARY, GATE_CHANNEL, GATE_ELEMENT, GATE_NONE, GATE_ROW, GROUP_SIZE,
+                    MAX_ADAPTER_RANK, MAX_ADAPTER_TARGETS, MAX_ADAPTERS, MAX_TOKENS, ROUTER_FULL_SOFTMAX,
                     ROUTER_TOPK_SOFTMAX, ExpertOffsets, MfError, check)
 
 __all__ = [
@@ -25,6 +26,7 @@ __all__ = [
     "Elementwise", "FamilyRouters", "SharedExpertInt4", "MPPPrefillInt4QMM", "MoEExpertOffsets", "MoE", "MoELayerWeights",
     "PrefillMoEGrouping", "PrefillTokenExpertPair", "MfError", "BITS_2", "BITS_4", "BITS_TERNARY",
     "ROUTER_TOPK_SOFTMAX", "ROUTER_FULL_SOFTMAX", "bf16_tensor", "bf16_bits",
+    "AdapterGrouping", "AdapterPlan", "LowRankAdapters", "BlockNorm", "GATE_NONE", "GATE_ROW", "GATE_ELEMENT", "GATE_CHANNEL",
 ]
 
 MoEExpertOffsets = ExpertOffsets
@@ -229,6 +231,210 @@ class RMSNorm:
               self.context.handle)
 
 
+def _on(context: MetalContext, stream) -> int:
+    """the stream's handle; the current stream of the context's device (not of the current device) when none is given"""
+    if stream is None:
+        if _raw_stream is None:
+            return torch.cuda.current_stream(context.device).cuda_stream
+        return _raw_stream(context.device.index)
+    return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
+
+
+def _device_tensor(context: MetalContext, t: torch.Tensor, what: str, dtype) -> int:
+    """the address of a tensor that lies on the context's device and has the type asked for"""
+    if not t.is_cuda:
+        raise ValueError(f"libmfmoe operates on device memory; {what} is a CPU tensor")
+    if t.dtype is not dtype:
+        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
+    if t.get_device() != context.device.index:
+        raise ValueError(f"{what} lies on another device than the context")
+    return t.data_ptr()
+
+
+def _rows_of(t: torch.Tensor, what: str, rows: int, width: int) -> int:
+    """elements from row to row of a [rows, width] tensor whose rows are contiguous"""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
+        raise MfError(-2, f"{what} is {tuple(t.shape)}, not ({rows}, {width})")
+    if width > 1 and t.stride(1) != 1:
+        raise MfError(-1, f"the rows of {what} must be contiguous")
+    if rows < 2:
+        return width
+    stride = t.stride(0)
+    if stride < width:
+        raise MfError(-2, f"the rows of {what} overlap")
+    return stride
+
+
+class AdapterPlan:
+    """What AdapterGrouping.encode fills: the rows of a batch in the order of their adapters (mf_adapter_group)."""
+
+    def __init__(self, t: int, num_adapters: int, words: torch.Tensor):
+        self.t, self.num_adapters, self.words = t, num_adapters, words
+        self.rows = words[:t]                               # int32 [t]: row numbers, stably sorted, rows without an adapter last
+        self.offsets = words[t:t + num_adapters + 1]        # int32: where every adapter's rows start; then the rows without one
+
+
+class AdapterGrouping:
+    """mf_adapter_group: the rows of a batch by adapter, on the device, once for all projections of a step (what
+    MoE.encode_group is for routes).  A row whose adapter is not in [0, num_adapters) has none."""
+
+    def __init__(self, context: MetalContext, num_adapters: int):
+        if not 1 <= num_adapters <= MAX_ADAPTERS:
+            raise MfError(-1, f"num_adapters={num_adapters}")
+        self.context, self.num_adapters = context, num_adapters
+
+    def plan(self, t: int) -> AdapterPlan:
+        """room for the plan of t rows"""
+        need = int(_capi.lib().mf_adapter_plan_bytes(t, self.num_adapters)) if t >= 0 else 0
+        if need == 0:
+            raise MfError(-1, f"t={t}")
+        return AdapterPlan(t, self.num_adapters, torch.empty(need // 4, dtype=torch.int32, device=self.context.device))
+
+    def encode(self, adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> AdapterPlan:
+        """adapter_of_row int32 [t]"""
+        ids = _device_tensor(self.context, adapter_of_row, "adapter_of_row", torch.int32)
+        t = adapter_of_row.shape[0]
+        if adapter_of_row.dim() != 1 or (t > 1 and adapter_of_row.stride(0) != 1):
+            raise MfError(-1, "adapter_of_row must be a contiguous vector")
+        if plan is None:
+            plan = self.plan(t)
+        elif plan.t != t or plan.num_adapters != self.num_adapters:
+            raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
+        words = plan.words
+        check(_capi.lib().mf_adapter_group(self.context.handle, _on(self.context, stream), ids, t, self.num_adapters,
+                                           words.data_ptr(), words.numel() * 4), self.context.handle)
+        return plan
+
+
+class LowRankAdapters:
+    """mf_adapter_apply: the low-rank corrections of many requests, added to the results of projections that read the same x
+    (DequantInt4GEMV, MPPPrefillInt4QMM, SharedExpertInt4 leave them).  a[s] bf16 [num_adapters, rank, n] and
+    b[s] bf16 [num_adapters, m_s, rank] for every projection s; scales float32 and ranks int32 [num_adapters]."""
+
+    def __init__(self, context: MetalContext, a: Sequence[torch.Tensor], b: Sequence[torch.Tensor],
+                 scales: Optional[torch.Tensor] = None, ranks: Optional[torch.Tensor] = None):
+        a, b = ([a] if isinstance(a, torch.Tensor) else list(a)), ([b] if isinstance(b, torch.Tensor) else list(b))
+        if not 1 <= len(a) <= MAX_ADAPTER_TARGETS or len(a) != len(b):
+            raise MfError(-1, f"{len(a)} tensors a, {len(b)} tensors b")
+        if a[0].dim() != 3:
+            raise MfError(-2, "a must be [num_adapters, rank, n]")
+        self.context = context
+        self.num_adapters, self.rank, self.n = a[0].shape
+        self.a, self.b, self.scales, self.ranks = a, b, scales, ranks  # kept: the pool's addresses stay valid
+        self._targets = (_capi.AdapterTarget * len(a))()
+        for g, wa, wb in zip(self._targets, a, b):
+            if wa.shape != a[0].shape or wb.dim() != 3 or wb.shape[0] != self.num_adapters or wb.shape[2] != self.rank:
+                raise MfError(-2, f"a {tuple(wa.shape)}, b {tuple(wb.shape)}")
+            if not (wa.is_contiguous() and wb.is_contiguous()):
+                raise MfError(-1, "the adapter pool must be contiguous")
+            g.a = _device_tensor(context, wa, "a", torch.bfloat16)
+            g.b = _device_tensor(context, wb, "b", torch.bfloat16)
+            g.m = wb.shape[1]
+        self.pool = _capi.AdapterPool(self.num_adapters, self.rank, self.n, None, None)
+        for name, v, dtype in (("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
+            if v is not None:
+                if v.shape != (self.num_adapters,) or not v.is_contiguous():
+                    raise MfError(-2, f"{name} must be a vector of num_adapters")
+                setattr(self.pool, name, _device_tensor(context, v, name, dtype))
+        if self.workspace_bytes(1) == 0:
+            raise MfError(-2, f"num_adapters={self.num_adapters} rank={self.rank} n={self.n}")
+
+    def workspace_bytes(self, t: int) -> int:
+        """bytes that a call of t rows, or fewer, asks for"""
+        return int(_capi.lib().mf_adapter_workspace_bytes(C.byref(self.pool), len(self._targets), t))
+
+    def encode(self, x: torch.Tensor, adapter_of_row: torch.Tensor, ys, plan: Optional[AdapterPlan] = None,
+               workspace: Optional[torch.Tensor] = None, stream=None) -> None:
+        """ys[s][i] += scales[a] * b[s][a] @ (a[s][a] @ x[i]), a = adapter_of_row[i]; rows without an adapter stay as they
+        are.  x bf16 [t, n]; ys[s] bf16 or float32 [t, m_s], all of one type.  plan: AdapterGrouping's of the same rows, for
+        batches that mix many adapters.  Without a workspace the call takes one of its own from torch's allocator."""
+        ctx = self.context
+        if isinstance(ys, torch.Tensor):
+            ys = (ys,)
+        if len(ys) != len(self._targets):
+            raise MfError(-2, f"{len(ys)} results for {len(self._targets)} projections")
+        t = x.shape[0]
+        ids = _device_tensor(ctx, adapter_of_row, "adapter_of_row", torch.int32)
+        if adapter_of_row.dim() != 1 or adapter_of_row.shape[0] != t or (t > 1 and adapter_of_row.stride(0) != 1):
+            raise MfError(-2, f"adapter_of_row must be a contiguous vector of {t}")
+        x_ptr = _device_tensor(ctx, x, "x", torch.bfloat16)
+        x_stride = _rows_of(x, "x", t, self.n)
+        dtype = ys[0].dtype
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise ValueError(f"the results must be bfloat16 or float32, not {dtype}")
+        targets = self._targets
+        targets = type(targets).from_buffer_copy(targets)  # two threads may use one object
+        for g, y in zip(targets, ys):
+            g.y = _device_tensor(ctx, y, "y", dtype)
+            g.y_stride = _rows_of(y, "y", t, g.m)
+        if t == 0:
+            return
+        words = None
+        if plan is not None:
+            if plan.t != t or plan.num_adapters != self.num_adapters:
+                raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
+            words = plan.words.data_ptr()
+        if workspace is None:
+            workspace = torch.empty(self.workspace_bytes(t), dtype=torch.uint8, device=ctx.device)
+            if stream is not None:
+                workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), ctx.device))
+        elif not workspace.is_contiguous():
+            raise MfError(-1, "the workspace must be contiguous")
+        elif workspace.get_device() != ctx.device.index:
+            raise ValueError("the workspace lies on another device than the context")
+        check(_capi.lib().mf_adapter_apply(ctx.handle, _on(ctx, stream), C.byref(self.pool), targets, len(targets), x_ptr, x_stride,
+                                           ids, t, 1 if dtype is torch.float32 else 0, words, workspace.data_ptr(),
+                                           workspace.numel() * workspace.element_size()), ctx.handle)
+
+
+class BlockNorm:
+    """mf_block_norm: what stands between two blocks of a layer, in one launch -- the norm behind the block, its gate and scale,
+    the residual add, the norm in front of the next block (RMSNorm and Elementwise.encode_residual_add are its two halves)."""
+
+    def __init__(self, context: MetalContext):
+        self.context = context
+
+    def encode(self, hidden: torch.Tensor, delta: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               pre_weight: Optional[torch.Tensor] = None, post_weight: Optional[torch.Tensor] = None,
+               gate: Optional[torch.Tensor] = None, gate_kind: int = GATE_NONE, eps: float = 1e-6,
+               post_eps: Optional[float] = None, residual_scale: float = 1.0, branch_scale: float = 1.0,
+               weight_bias: float = 0.0, stream=None) -> None:
+        """hidden bf16 [t, d] is updated in place: residual_scale * hidden + branch_scale * gate * norm(delta); out gets its norm.
+        gate: GATE_ROW [t] or [t, 1] and GATE_ELEMENT [t, d] go through a sigmoid, GATE_CHANNEL [d] is taken as it is."""
+        ctx, bf16 = self.context, torch.bfloat16
+        if hidden.dim() != 2:
+            raise MfError(-2, "hidden must be [t, d]")
+        t, d = hidden.shape
+        a = _capi.BlockNormArgs()
+        a.d, a.t, a.gate_kind = d, t, gate_kind
+        a.hidden, a.hidden_stride = _device_tensor(ctx, hidden, "hidden", bf16), _rows_of(hidden, "hidden", t, d)
+        if delta is not None:
+            a.delta_f32 = 1 if delta.dtype is torch.float32 else 0
+            a.delta = _device_tensor(ctx, delta, "delta", torch.float32 if a.delta_f32 else bf16)
+            a.delta_stride = _rows_of(delta, "delta", t, d)
+        if out is not None:
+            a.out, a.out_stride = _device_tensor(ctx, out, "out", bf16), _rows_of(out, "out", t, d)
+        for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+            if w is not None:
+                if w.dim() != 1 or w.shape[0] != d or (d > 1 and w.stride(0) != 1):
+                    raise MfError(-2, f"{name} must be a contiguous vector of {d}")
+                setattr(a, name, _device_tensor(ctx, w, name, bf16))
+        if gate is not None:
+            a.gate = _device_tensor(ctx, gate, "gate", bf16)
+            if gate_kind == GATE_ROW:
+                if gate.numel() != t or gate.dim() > 2 or gate.shape[0] != t:
+                    raise MfError(-2, f"the gate must be one logit for each of {t} rows")
+                a.gate_stride = gate.stride(0) if t > 1 else 1
+                if a.gate_stride == 0 and t > 1:  # 0 means "not given" to the library
+                    raise MfError(-2, "a gate of one logit a row cannot be an expanded one")
+            elif gate_kind == GATE_ELEMENT:
+                a.gate_stride = _rows_of(gate, "gate", t, d)
+            elif gate.dim() != 1 or gate.shape[0] != d or (d > 1 and gate.stride(0) != 1):
+                raise MfError(-2, f"the gate must be a contiguous vector of {d}")
+        a.pre_eps, a.post_eps = eps, eps if post_eps is None else post_eps
+        a.residual_scale, a.branch_scale, a.weight_bias = residual_scale, branch_scale, weight_bias
+        check(_capi.lib().mf_block_norm(ctx.handle, _on(ctx, stream), C.byref(a)), ctx.handle)
+
 class SharedExpertInt4:
     """Kernels/MoE/SharedExpertInt4.swift:70-165 (also the dense SwiGLU MLP)."""
 
@@ -247,6 +453,37 @@ class SharedExpertInt4:
             gate.n, gate.rows, t, _ptr(y), _ptr(scratch_act),
             scratch_act.numel() * scratch_act.element_size()), self.context.handle)
 
+
+    def encode_adapted(self, x: torch.Tensor, gate: QuantizedTensor, up: QuantizedTensor, down: QuantizedTensor,
+                       y: torch.Tensor, gate_up_adapters: LowRankAdapters, down_adapters: LowRankAdapters,
+                       adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> None:
+        """The MLP with an adapter beside each of its three projections (the same adapter of a row in all of them): the
+        projections by themselves (mf_qmm), LowRankAdapters on their results, silu(gate) * up in between.  No counterpart in
+        the reference.  x bf16 [t, d], y bf16 [t, d]; buffers come from torch's allocator."""
+        if not (gate.rows == up.rows and gate.n == up.n and down.rows == gate.n and down.n == gate.rows):
+            raise MfError(-2, f"gate=({gate.rows},{gate.n}) up=({up.rows},{up.n}) down=({down.rows},{down.n})")
+        t, d, f = x.shape[0], gate.n, gate.rows
+        if not (x.is_contiguous() and y.is_contiguous()) or x.shape != (t, d) or y.shape != (t, d):
+            raise MfError(-2, f"x {tuple(x.shape)} and y {tuple(y.shape)} must be contiguous rows of {d}")
+        if t == 0:
+            return
+        if t * f >= 1 << 31:
+            raise MfError(-1, f"t={t} rows of f={f} are more than one call takes")
+        on = stream if isinstance(stream, torch.cuda.Stream) else \
+            torch.cuda.current_stream(self.context.device) if stream is None else torch.cuda.ExternalStream(int(stream), self.context.device)
+        with torch.cuda.stream(on):  # so that the allocator knows the stream of the buffers
+            g, u, act = (torch.empty((t, f), dtype=torch.bfloat16, device=x.device) for _ in range(3))
+            qmm, elementwise = MPPPrefillInt4QMM(self.context), Elementwise(self.context)
+            need = max(qmm.workspace_bytes(t, f, d), qmm.workspace_bytes(t, d, f), 256)
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+            for w, out in ((gate, g), (up, u)):
+                if qmm.encode(w, x, out, t, f, d, workspace=workspace, stream=on) == "unavailable":
+                    raise MfError(-1, "a projection refused its operands")
+            gate_up_adapters.encode(x, adapter_of_row, (g, u), plan=plan, stream=on)
+            elementwise.encode_silu_mul(g, u, act, t * f, stream=on)
+            if qmm.encode(down, act, y, t, d, f, workspace=workspace, stream=on) == "unavailable":
+                raise MfError(-1, "a projection refused its operands")
+            down_adapters.encode(act, adapter_of_row, y, plan=plan, stream=on)
 
     @staticmethod
     def scratch_bytes(d: int, f: int, t: int) -> int:
