@@ -673,7 +673,7 @@ typedef struct {
   const uint16_t* a;  /* bf16 [num_adapters, rank, n], 16-byte aligned */
   const uint16_t* b;  /* bf16 [num_adapters, m, rank], 16-byte aligned */
   void* y;            /* the projection's result, row i at element i * y_stride: updated in place */
-  uint32_t m;         /* any, from 1 on */
+  uint32_t m;         /* 1 .. 2^28 */
   uint32_t y_stride;  /* >= m */
 } mf_adapter_target;
 

@@ -1038,7 +1038,7 @@ mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool*
   for (uint32_t k = 0; k < num_targets; ++k) {
     const mf_adapter_target& g = targets[k];
     if (!g.a || !g.b || !g.y) return MF_ERR_INVALID_ARGUMENT;
-    if (g.m == 0 || g.y_stride < g.m) return MF_ERR_DIMENSION_MISMATCH;
+    if (g.m == 0 || g.m > 1u << 28 || g.y_stride < g.m) return MF_ERR_DIMENSION_MISMATCH;
     if (!mf::aligned16(g.a) || !mf::aligned16(g.b) || !(y_f32 ? aligned4(g.y) : mf::aligned2(g.y))) return MF_ERR_INVALID_ARGUMENT;
     ys[k] = {g.y, static_cast<uint64_t>(size) * g.y_stride, static_cast<uint64_t>(size) * g.m};
     if (rows_meet(ys[k], xs, t)) return MF_ERR_INVALID_ARGUMENT;
@@ -1059,6 +1059,7 @@ mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool*
   a.t = t;
   a.x_stride = x_stride;
   a.cols = num_targets * pool->rank;
+  if (plan) a.plan = mf::AdapterPlan::at(const_cast<uint32_t*>(plan), t, pool->num_adapters);  // (only read)
   const OnDevice on(ctx);
   MF_HIP(ctx, on.error());
   MF_HIP(ctx, mf::launch_adapter_apply(static_cast<hipStream_t>(stream), a, y_f32 != 0));

@@ -39,13 +39,14 @@ struct AdapterArgs {
   const float* scales;
   const uint16_t* x;
   const int32_t* ids;
-  float* v;  // [t, cols]: c_a A x, targets side by side
-  uint32_t num_targets, num_adapters, rank, n, t, x_stride, cols;
+  float* v;  // [splits, t, cols]: c_a A x in parts, targets side by side
+  uint32_t num_targets, num_adapters, rank, n, t, x_stride, cols, splits;
+  AdapterPlan plan;  // tiles null: the rows as they lie
 };
 
 hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, uint32_t n, uint32_t* plan);
 size_t adapter_workspace_bytes(uint32_t num_targets, uint32_t rank, uint32_t n, uint32_t t);
-hipError_t launch_adapter_apply(hipStream_t s, const AdapterArgs& a, bool y_f32);
+hipError_t launch_adapter_apply(hipStream_t s, AdapterArgs a, bool y_f32);
 
 // block_norm.hip
 hipError_t launch_block_norm(hipStream_t s, const mf_block_norm_args& a);
