@@ -14,35 +14,129 @@ namespace {
 
 __device__ __forceinline__ uint32_t adapter_key(int32_t id, uint32_t n) { return static_cast<uint32_t>(id) < n ? static_cast<uint32_t>(id) : n; }
 
-// A stable counting sort by one workgroup: thread k owns key k of the counts, and the rows are walked in order.
-__global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __restrict__ ids, uint32_t t, uint32_t n, AdapterPlan plan) {
-  __shared__ uint32_t start[MF_MAX_ADAPTERS + 2];
-  for (uint32_t k = threadIdx.x; k <= n; k += blockDim.x) {
-    uint32_t count = 0;
-    for (uint32_t i = 0; i < t; ++i) count += adapter_key(ids[i], n) == k;
-    start[k + 1] = count;
-  }
-  if (threadIdx.x == 0) start[0] = 0;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t tiles = 0;
-    for (uint32_t k = 0; k < n; ++k) {
-      const uint32_t count = start[k + 1];
-      for (uint32_t at = 0; at < count; at += plan.tile_rows)
-        plan.tiles[tiles++] = make_uint2(k | min(count - at, plan.tile_rows) << 16, start[k] + at);
-      start[k + 1] += start[k];
+// A stable counting sort.  A wave owns IT * 64 consecutive rows and takes 64 of them at a time: the lanes that hold the same key find
+// each other by a ballot for every bit of it, a row's place among its wave's rows of that key is the count so far plus the lanes in
+// front of it, and the lane in front raises the count.  No atomics: the order is the rows'.  Counts of a wave fit 16 bits (IT <= 16).
+template <int IT>
+struct RowRanks {
+  uint32_t key[IT], rank[IT];  // rank within the wave's rows of the key
+  uint64_t valid[IT];
+
+  __device__ __forceinline__ void find(const int32_t* __restrict__ ids, uint32_t first, uint32_t t, uint32_t n, uint16_t* counts) {
+    const uint32_t lane = threadIdx.x & 63, bits = 32 - __builtin_clz(n);
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      const uint32_t i = first + k * 64 + lane;
+      key[k] = i < t ? adapter_key(ids[i], n) : n;
     }
-    plan.header[0] = t;
-    plan.header[1] = n;
-    plan.header[2] = tiles;
-    plan.header[3] = plan.tile_rows;
+#pragma unroll
+    for (int k = 0; k < IT; ++k) {
+      valid[k] = __ballot(first + k * 64 + lane < t);
+      uint64_t same = valid[k];
+      for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = (key[k] >> b) & 1;
+        const uint64_t with = __ballot(set);
+        same &= set ? with : ~with;
+      }
+      const uint32_t in_front = __builtin_popcountll(same & ((1ull << lane) - 1));
+      if ((valid[k] >> lane) & 1) {
+        const uint32_t before = counts[key[k]];
+        rank[k] = before + in_front;
+        if (in_front == 0) counts[key[k]] = static_cast<uint16_t>(before + __builtin_popcountll(same));
+      }
+      asm volatile("" ::: "memory");  // the next 64 read what these have left
+      __builtin_amdgcn_wave_barrier();
+    }
   }
+};
+
+// exclusive sums over the workgroup of two numbers a thread
+__device__ __forceinline__ uint2 block_exclusive(uint2 v, uint2* part) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint2 sum = v;
+#pragma unroll
+  for (uint32_t by = 1; by < 64; by *= 2) {
+    const uint32_t x = __shfl_up(sum.x, by), y = __shfl_up(sum.y, by);
+    if (lane >= by) sum.x += x, sum.y += y;
+  }
+  if (lane == 63) part[wave] = sum;
   __syncthreads();
-  for (uint32_t k = threadIdx.x; k <= n; k += blockDim.x) {
-    plan.offsets[k] = start[k];
-    uint32_t at = start[k];
-    for (uint32_t i = 0; i < t; ++i)
-      if (adapter_key(ids[i], n) == k) plan.rows[at++] = i;
+  uint2 before = make_uint2(sum.x - v.x, sum.y - v.y);
+  for (uint32_t w = 0; w < wave; ++w) before.x += part[w].x, before.y += part[w].y;
+  return before;
+}
+
+// One workgroup for a run of rows.  COUNT: it leaves how many rows of every key the run has, and that is all.  Otherwise it adds up
+// those counts of all runs (a thread a key), knows from them where every key's rows start and where its own go, and writes its rows;
+// the lists of adapters and tiles are dealt out over the workgroups.  A batch of one run needs no counting launch in front.
+template <int IT, bool COUNT>
+__global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __restrict__ ids, uint32_t t, uint32_t n, AdapterPlan plan) {
+  __shared__ uint16_t counts[16 * (MF_MAX_ADAPTERS + 1)];  // [wave][key]; then where a wave's rows of a key start among the run's
+  __shared__ uint32_t starts[MF_MAX_ADAPTERS + 1];         // where the run's rows of a key go
+  __shared__ uint2 part[16];
+  const uint32_t waves = blockDim.x / 64, keys = n + 1, wave = threadIdx.x >> 6;
+  for (uint32_t k = threadIdx.x; k < waves * keys; k += blockDim.x) counts[k] = 0;
+  __syncthreads();
+  RowRanks<IT> mine;
+  const uint32_t first = (blockIdx.x * waves + wave) * (IT * 64);
+  mine.find(ids, first, t, n, counts + wave * keys);
+  __syncthreads();
+  uint2 total = make_uint2(0, 0);  // rows and tiles of thread k's key
+  uint32_t before = 0;             // its rows in the runs in front
+  for (uint32_t k = threadIdx.x; k < keys; k += blockDim.x) {  // (a second turn for the last key of the largest pool only)
+    uint32_t own = 0;
+    for (uint32_t w = 0; w < waves; ++w) {
+      const uint32_t c = counts[w * keys + k];
+      counts[w * keys + k] = static_cast<uint16_t>(own);  // at most 16 * 16 * 64 rows in front
+      own += c;
+    }
+    if constexpr (COUNT) {
+      plan.runs[static_cast<size_t>(blockIdx.x) * keys + k] = own;
+    } else if (k < n) {
+      total.x = own;
+      if (gridDim.x > 1) {
+        total.x = 0;
+        for (uint32_t r = 0; r < gridDim.x; ++r) {
+          const uint32_t c = plan.runs[static_cast<size_t>(r) * keys + k];
+          before += r < blockIdx.x ? c : 0;
+          total.x += c;
+        }
+      }
+      total.y = (total.x + plan.tile_rows - 1) / plan.tile_rows;
+    }
+  }
+  if constexpr (!COUNT) {
+    const uint2 at = block_exclusive(total, part);
+    const uint32_t k = threadIdx.x;
+    if (k < n) {
+      starts[k] = at.x + before;
+      if (k % gridDim.x == blockIdx.x) {
+        plan.offsets[k] = at.x;
+        for (uint32_t i = 0; i < total.y; ++i)
+          plan.tiles[at.y + i] = make_uint2(k | min(total.x - i * plan.tile_rows, plan.tile_rows) << 16, at.x + i * plan.tile_rows);
+      }
+    }
+    if (k == n - 1) {  // behind all adapters: the rows without one.  What of them lies in the runs in front is what the adapters leave.
+      const uint32_t with = at.x + total.x;
+      starts[n] = with;
+      if (blockIdx.x == 0) {
+        plan.offsets[n] = with;
+        plan.header[0] = t;
+        plan.header[1] = n;
+        plan.header[2] = at.y + total.y;
+        plan.header[3] = plan.tile_rows;
+      }
+    }
+    __syncthreads();
+    if (gridDim.x > 1) {
+      for (uint32_t r = threadIdx.x; r < blockIdx.x; r += blockDim.x) atomicAdd(&starts[n], plan.runs[static_cast<size_t>(r) * keys + n]);  // whole numbers: any order
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      if (!((mine.valid[i] >> (threadIdx.x & 63)) & 1)) continue;
+      plan.rows[starts[mine.key[i]] + counts[wave * keys + mine.key[i]] + mine.rank[i]] = first + i * 64 + (threadIdx.x & 63);
+    }
   }
 }
 
@@ -327,7 +421,21 @@ uint32_t shrink_splits(uint32_t t, uint32_t n) {
 }  // namespace
 
 hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, uint32_t n, uint32_t* plan) {
-  adapter_group_kernel<<<dim3(1), dim3(1024), 0, s>>>(ids, t, n, AdapterPlan::at(plan, t, n));
+  const AdapterPlan p = AdapterPlan::at(plan, t, n);
+  const uint32_t runs = AdapterPlan::runs_of(t), it = AdapterPlan::turns_of(t);
+  const auto go = [&](auto turns) {
+    constexpr int kTurns = decltype(turns)::value;
+    if (runs == 1) {  // threads for the rows, and one for every adapter
+      const uint32_t threads = std::max((t + kTurns * 64 - 1) / (kTurns * 64) * 64, (n + 63) / 64 * 64);
+      adapter_group_kernel<kTurns, false><<<dim3(1), dim3(threads), 0, s>>>(ids, t, n, p);
+      return;
+    }
+    adapter_group_kernel<kTurns, true><<<dim3(runs), dim3(1024), 0, s>>>(ids, t, n, p);
+    adapter_group_kernel<kTurns, false><<<dim3(runs), dim3(1024), 0, s>>>(ids, t, n, p);
+  };
+  if (it == 1) go(std::integral_constant<int, 1>{});
+  else if (it == 4) go(std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 16>{});
   return hipGetLastError();
 }
 

@@ -13,6 +13,7 @@ struct AdapterPlan {
   uint32_t* offsets;  // [n + 1]
   uint32_t* header;   // [4]
   uint2* tiles;       // [most_tiles]
+  uint32_t* runs;     // [runs][n + 1]: rows of every key in each run, where there are several
   uint32_t tile_rows, most_tiles;
 
   // rows a tile: what a wave of the products holds at once.  Where a batch has few rows an adapter the wide tiles would be
@@ -20,10 +21,15 @@ struct AdapterPlan {
   static uint32_t rows_of_tile(uint32_t t, uint32_t n) { return t / 32 >= n ? 64 : 16; }
   static uint32_t tiles_of(uint32_t t, uint32_t n) { return t / rows_of_tile(t, n) + (n < t ? n : t); }
   static size_t header_word(uint32_t t, uint32_t n) { return (static_cast<size_t>(t) + n + 1 + 3) / 4 * 4; }
-  static size_t words(uint32_t t, uint32_t n) { return header_word(t, n) + 4 + 2 * static_cast<size_t>(tiles_of(t, n)); }
+  // the sort: rows a lane takes one after the other, and workgroups of 1024 lanes
+  static uint32_t turns_of(uint32_t t) { return t <= 1024 ? 1 : t <= 4096 ? 4 : t <= 32768 ? 1 : t <= 262144 ? 4 : 16; }
+  static uint32_t runs_of(uint32_t t) { return t <= 4096 ? 1 : (t + 1024 * turns_of(t) - 1) / (1024 * turns_of(t)); }
+  static size_t words(uint32_t t, uint32_t n) {
+    return header_word(t, n) + 4 + 2 * static_cast<size_t>(tiles_of(t, n)) + (runs_of(t) > 1 ? static_cast<size_t>(runs_of(t)) * (n + 1) : 0);
+  }
   static AdapterPlan at(uint32_t* p, uint32_t t, uint32_t n) {
     uint32_t* h = p + header_word(t, n);
-    return {p, p + t, h, reinterpret_cast<uint2*>(h + 4), rows_of_tile(t, n), tiles_of(t, n)};
+    return {p, p + t, h, reinterpret_cast<uint2*>(h + 4), h + 4 + 2 * static_cast<size_t>(tiles_of(t, n)), rows_of_tile(t, n), tiles_of(t, n)};
   }
 };
 
