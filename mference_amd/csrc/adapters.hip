@@ -194,11 +194,13 @@ __device__ __forceinline__ f32x4_t mfma16(const uint4& a, const uint4& b, const 
 //
 // Operands of v_mfma_f32_16x16x32_bf16 are eight consecutive elements of a row a lane, of x (16 rows of the batch) and of A (16 ranks):
 // 16-byte loads straight into the registers that the instruction reads.  A workgroup takes RT * 16 rows, CF blocks of 16 ranks and a
-// window of the row length; its four waves take 64 elements (a line of 128 bytes) in turn and add their sums through LDS.  A rank
+// window of the row length; its eight waves take 64 elements (a line of 128 bytes) in turn and add their sums through LDS.  A rank
 // beyond the adapter's, and a row of another one, is a column or a row of the product that nobody reads.
+constexpr uint32_t kShrinkWaves = 8;
+
 template <int RT, int CF>
-__global__ __launch_bounds__(256) void adapter_shrink_kernel(const AdapterArgs a) {
-  __shared__ f32x4_t part[4][RT * CF][64];
+__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a) {
+  __shared__ f32x4_t part[kShrinkWaves][RT * CF][64];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t split = blockIdx.y % a.splits, group = blockIdx.y / a.splits;
   const uint32_t blocks = (a.rank + 15) / 16;  // of 16 ranks, a target
@@ -210,6 +212,7 @@ __global__ __launch_bounds__(256) void adapter_shrink_kernel(const AdapterArgs a
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
     const uint32_t rank = live_rank(a, adapter);
+    const float scale = a.scales ? a.scales[adapter] : 1.0f;
     const uint16_t* xp[RT];
     const uint16_t* wp[CF];
 #pragma unroll
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(256) void adapter_shrink_kernel(const AdapterArgs a
       uint4 xv[RT][2 * kUnits], wv[CF][2 * kUnits];
 #pragma unroll
       for (int k = 0; k < 2 * kUnits; ++k) {
-        const uint32_t at = (u + k / 2 * 4) * 64 + k % 2 * 32;
+        const uint32_t at = (u + k / 2 * kShrinkWaves) * 64 + k % 2 * 32;
 #pragma unroll
         for (int r = 0; r < RT; ++r) xv[r][k] = load_16_bytes(xp[r] + at);
 #pragma unroll
@@ -252,7 +255,7 @@ __global__ __launch_bounds__(256) void adapter_shrink_kernel(const AdapterArgs a
           for (int c = 0; c < CF; ++c) acc[r][c] = mfma16(xv[r][k], wv[c][k], acc[r][c]);
     };
     uint32_t u = u0 + wave;
-    for (; u + 4 < u1; u += 8) step(std::integral_constant<int, 2>{}, u);
+    for (; u + kShrinkWaves < u1; u += 2 * kShrinkWaves) step(std::integral_constant<int, 2>{}, u);
     if (u < u1) step(std::integral_constant<int, 1>{}, u);
     __syncthreads();  // (the parts of the adapter before have been read)
 #pragma unroll
@@ -260,16 +263,21 @@ __global__ __launch_bounds__(256) void adapter_shrink_kernel(const AdapterArgs a
 #pragma unroll
       for (int c = 0; c < CF; ++c) part[wave][r * CF + c][lane] = acc[r][c];
     __syncthreads();
-    const float scale = a.scales ? a.scales[adapter] : 1.0f;
-    for (uint32_t f = wave; f < RT * CF; f += 4) {
-      const f32x4_t sum = (part[0][f][lane] + part[1][f][lane]) + (part[2][f][lane] + part[3][f][lane]);
+    for (uint32_t f = wave; f < RT * CF; f += kShrinkWaves) {
+      f32x4_t sum[kShrinkWaves];
+#pragma unroll
+      for (uint32_t w = 0; w < kShrinkWaves; ++w) sum[w] = part[w][f][lane];
+#pragma unroll
+      for (uint32_t by = 1; by < kShrinkWaves; by *= 2)
+#pragma unroll
+        for (uint32_t w = 0; w < kShrinkWaves; w += 2 * by) sum[w] += sum[w + by];
       const uint32_t cb = group * CF + f % CF, target = cb / blocks, r = cb % blocks * 16 + (lane & 15);
       const uint32_t row0 = f / CF * 16 + (lane >> 4) * 4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t row = __shfl(meeting.row, row0 + i);
         if (target < a.num_targets && r < rank && ((lanes >> (row0 + i)) & 1))
-          a.v[(static_cast<size_t>(split) * a.t + row) * a.cols + target * a.rank + r] = sum[i] * scale;
+          a.v[(static_cast<size_t>(split) * a.t + row) * a.cols + target * a.rank + r] = sum[0][i] * scale;
       }
     }
   }
@@ -312,110 +320,186 @@ __device__ __forceinline__ uint4 keep_bf16(uint4 v, uint32_t n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// A workgroup takes RT * 16 rows and a run of a target's results.  It adds up the parts of v and leaves its terms in LDS as the
+// operands that the instruction reads; its waves then take 64 results in turn, the y and B of the next ones requested before the
+// present ones are worked on.
 template <int RT, bool F32>
 __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a) {
   constexpr int kTerms = F32 ? 3 : 2, kPer = F32 ? 4 : 8, kChunks = 16 / kPer;  // results to 16 bytes; such pieces a lane holds of a row
   using Elem = std::conditional_t<F32, float, uint16_t>;
-  const uint32_t lane = threadIdx.x & 63, q = lane >> 4;
-  uint32_t block = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), target = 0;
-  while (target < a.num_targets && block >= (a.target[target].m + 63) / 64) block -= (a.target[target++].m + 63) / 64;
-  if (target >= a.num_targets) return;
+  extern __shared__ uint4 operand[];  // [32 ranks][RT][kTerms][lane]
+  const uint32_t lane = threadIdx.x & 63, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t run = blockIdx.x, target = 0;
+  while (run >= a.first_run[target + 1]) ++target;
+  run -= a.first_run[target];
   const AdapterArgs::Target tg = a.target[target];
-  const uint32_t m0 = block * 64;
+  const uint32_t m_blocks = (tg.m + 63) / 64, end = min(m_blocks, (run + 1) * a.run_blocks);
   Meeting<RT * 16> meeting(a, blockIdx.y, lane);
   uint32_t adapter, lead;
   uint64_t lanes;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
-    const uint32_t rank = live_rank(a, adapter);
+    const uint16_t* bp = tg.b + static_cast<size_t>(adapter) * tg.m * a.rank;
     Elem* yp[RT];
-    const float* vp[RT];
-    uint4 yv[RT][kChunks];
+    bool mine[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const uint32_t at = r * 16 + (lane & 15);
-      const bool mine = (lanes >> at) & 1;
-      const uint32_t row = __shfl(meeting.row, mine ? at : lead);
-      vp[r] = a.v + static_cast<size_t>(row) * a.cols + target * a.rank;
-      yp[r] = static_cast<Elem*>(tg.y) + static_cast<size_t>(row) * tg.y_stride;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint32_t m = m0 + c * 4 * kPer + q * kPer;
-        if (mine && m + kPer <= tg.m) yv[r][c] = load_16_bytes(yp[r] + m);
-      }
+      mine[r] = (lanes >> at) & 1;
+      yp[r] = static_cast<Elem*>(tg.y) + static_cast<size_t>(__shfl(meeting.row, mine[r] ? at : lead)) * tg.y_stride;
     }
-    f32x4_t acc[RT][4];
+    const auto load_y = [&](uint32_t block, uint4 (&yv)[RT][kChunks]) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[r][j] = f32x4_t{0, 0, 0, 0};
-    for (uint32_t k0 = 0; k0 < rank; k0 += 32) {
-      const uint32_t k = k0 + q * 8, have = k < rank ? min(rank - k, 8u) : 0;
-      uint4 bv[4];
+        for (int c = 0; c < kChunks; ++c) {
+          const uint32_t m = block * 64 + c * 4 * kPer + q * kPer;
+          if (mine[r] && m + kPer <= tg.m) yv[r][c] = load_16_bytes(yp[r] + m);
+        }
+    };
+    const auto load_b = [&](uint32_t block, uint32_t k, uint4 (&bv)[4]) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t p = lane & 15;
-        const uint32_t m = m0 + (F32 ? 16 * j + p : 32 * (j >> 1) + 8 * (p >> 2) + 4 * (j & 1) + (p & 3));
-        bv[j] = make_uint4(0, 0, 0, 0);
-        if (have) bv[j] = *reinterpret_cast<const uint4*>(tg.b + (static_cast<size_t>(adapter) * tg.m + min(m, tg.m - 1)) * a.rank + k);
-        if (have < 8) bv[j] = keep_bf16(bv[j], have);
+        const uint32_t m = block * 64 + (F32 ? 16 * j + p : 32 * (j >> 1) + 8 * (p >> 2) + 4 * (j & 1) + (p & 3));
+        if (k < a.rank) bv[j] = *reinterpret_cast<const uint4*>(bp + static_cast<size_t>(min(m, tg.m - 1)) * a.rank + k);
+      }
+    };
+    uint32_t block = run * a.run_blocks + wave;
+    uint4 yv[RT][kChunks], bv[4];
+    if (block < end) {
+      load_y(block, yv);
+      load_b(block, q * 8, bv);
+    }
+    const uint32_t rank = live_rank(a, adapter), kb = (rank + 31) / 32;
+    __syncthreads();  // (the operands of the adapter before have been read)
+    for (uint32_t slot = threadIdx.x; slot < kb * RT * 64; slot += 256) {
+      const uint32_t at = slot / 64 % RT * 16 + (slot & 15), k = slot / (64 * RT) * 32 + (slot >> 4) % 4 * 8, have = k < rank ? min(rank - k, 8u) : 0;
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      const uint32_t row = __shfl(meeting.row, at);
+      if (have && ((lanes >> at) & 1)) {
+        const float* p = a.v + static_cast<size_t>(row) * a.cols + target * a.rank + k;
+        const size_t part = static_cast<size_t>(a.t) * a.cols;
+        for (uint32_t s = 0; s < a.splits; s += 4) {  // four parts requested at once
+          float4 lo[4], hi[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const float4* w = reinterpret_cast<const float4*>(p + min(s + i, a.splits - 1) * part);
+            lo[i] = w[0], hi[i] = w[1];
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            if (s + i >= a.splits) continue;
+            v[0] += lo[i].x, v[1] += lo[i].y, v[2] += lo[i].z, v[3] += lo[i].w;
+            v[4] += hi[i].x, v[5] += hi[i].y, v[6] += hi[i].z, v[7] += hi[i].w;
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<uint32_t>(e) < have ? v[e] : 0.0f;
+      uint4 terms[kTerms];
+      split_terms<kTerms>(v, terms);
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) operand[(slot / 64 * kTerms + i) * 64 + (slot & 63)] = terms[i];
+    }
+    __syncthreads();
+    for (; block < end; block += 4) {
+      uint4 next_y[RT][kChunks], next_b[4];
+      if (block + 4 < end) {
+        load_y(block + 4, next_y);
+        load_b(block + 4, q * 8, next_b);
+      }
+      f32x4_t acc[RT][4];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[r][j] = f32x4_t{0, 0, 0, 0};
+      for (uint32_t b = 0; b < kb; ++b) {
+        const uint32_t k = b * 32 + q * 8, have = k < rank ? min(rank - k, 8u) : 0;
+        if (b) load_b(block, k, bv);
+        if (rank % 32) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bv[j] = have < 8 ? keep_bf16(bv[j], have) : bv[j];
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = kTerms - 1; i >= 0; --i) {  // the small terms first
+            const uint4 term = operand[((b * RT + r) * kTerms + i) * 64 + lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[r][j] = mfma16(bv[j], term, acc[r][j]);
+          }
       }
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (have) {
-          for (uint32_t s = 0; s < a.splits; ++s) {
-            const float4* p = reinterpret_cast<const float4*>(vp[r] + static_cast<size_t>(s) * a.t * a.cols + k);
-            const float4 lo = p[0], hi = p[1];
-            v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-            v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
-          }
-        }
+        if (!mine[r]) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = static_cast<uint32_t>(e) < have ? v[e] : 0.0f;
-        uint4 terms[kTerms];
-        split_terms<kTerms>(v, terms);
+        for (int c = 0; c < kChunks; ++c) {
+          const uint32_t m = block * 64 + c * 4 * kPer + q * kPer;
+          float add[kPer];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+          for (int e = 0; e < kPer; ++e) add[e] = acc[r][F32 ? c : 2 * c + e / 4][e % 4];
+          if (m + kPer <= tg.m) {
+            uint32_t w[4] = {yv[r][c].x, yv[r][c].y, yv[r][c].z, yv[r][c].w};
 #pragma unroll
-          for (int s = kTerms - 1; s >= 0; --s) acc[r][j] = mfma16(bv[j], terms[s], acc[r][j]);  // the small ones first
-      }
-    }
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (F32) w[e] = __float_as_uint(__uint_as_float(w[e]) + add[e]);
+              else w[e] = static_cast<uint32_t>(narrow_bf16(bf16_lo(w[e]) + add[2 * e])) | static_cast<uint32_t>(narrow_bf16(bf16_hi(w[e]) + add[2 * e + 1])) << 16;
+            }
+            __builtin_memcpy(yp[r] + m, w, 16);
+          } else {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      if (!((lanes >> (r * 16 + (lane & 15))) & 1)) continue;
-#pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const uint32_t m = m0 + c * 4 * kPer + q * kPer;
-        float add[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) add[e] = acc[r][F32 ? c : 2 * c + e / 4][e % 4];
-        if (m + kPer <= tg.m) {
-          uint32_t w[4] = {yv[r][c].x, yv[r][c].y, yv[r][c].z, yv[r][c].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (F32) w[e] = __float_as_uint(__uint_as_float(w[e]) + add[e]);
-            else w[e] = static_cast<uint32_t>(narrow_bf16(bf16_lo(w[e]) + add[2 * e])) | static_cast<uint32_t>(narrow_bf16(bf16_hi(w[e]) + add[2 * e + 1])) << 16;
-          }
-          __builtin_memcpy(yp[r] + m, w, 16);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            if (m + e >= tg.m) continue;
-            if constexpr (F32) yp[r][m + e] += add[e];
-            else yp[r][m + e] = narrow_bf16(bf16_to_f(yp[r][m + e]) + add[e]);
+            for (int e = 0; e < kPer; ++e) {
+              if (m + e >= tg.m) continue;
+              if constexpr (F32) yp[r][m + e] += add[e];
+              else yp[r][m + e] = narrow_bf16(bf16_to_f(yp[r][m + e]) + add[e]);
+            }
           }
         }
       }
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) yv[r][c] = next_y[r][c];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bv[j] = next_b[j];
     }
   }
 }
 
-// Parts of the sum over n: as many as give the chip a workgroup a CU or two, but at least four units of 64 elements a part, and few
-// where there are many rows (every part of v is written and read again).
+// Parts of the sum over n: workgroups for one and a half times the CUs, of eight units of 64 elements (one a wave) or more, and few
+// parts where there are many rows (every part of v is written and read again).
+constexpr uint32_t kMostSplits = 16, kShrinkGroups = 384;
 uint32_t shrink_splits(uint32_t t, uint32_t n) {
-  const uint32_t tiles = (t + 15) / 16, units = n / 64;
-  return std::max(1u, std::min({512u / tiles, units / 4, 32u}));
+  return std::max(1u, std::min({kShrinkGroups / ((t + 15) / 16), n / 64 / kShrinkWaves, kMostSplits}));
+}
+
+template <int RT>
+void launch_shrink(hipStream_t s, const AdapterArgs& a, uint32_t tiles, uint32_t turns) {
+  const uint32_t blocks = (a.rank + 15) / 16 * a.num_targets;
+  const auto go = [&](auto cf) {
+    constexpr int kCols = decltype(cf)::value;
+    adapter_shrink_kernel<RT, kCols><<<dim3(tiles, (blocks + kCols - 1) / kCols * a.splits, turns), dim3(kShrinkWaves * 64), 0, s>>>(a);
+  };
+  if (blocks == 1) go(std::integral_constant<int, 1>{});
+  else if (blocks == 2) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, 4>{});
+}
+
+template <int RT, bool F32>
+hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t turns) {
+  uint32_t blocks = 0;
+  for (uint32_t k = 0; k < a.num_targets; ++k) blocks += (a.target[k].m + 63) / 64;
+  // runs of results: workgroups for eight times the CUs where there is so much to do
+  a.run_blocks = std::max<uint32_t>(1, static_cast<uint32_t>(static_cast<uint64_t>(blocks) * tiles / (4 * 2048))) * 4;
+  a.first_run[0] = 0;
+  for (uint32_t k = 0; k < MF_MAX_ADAPTER_TARGETS; ++k)
+    a.first_run[k + 1] = k < a.num_targets ? a.first_run[k] + ((a.target[k].m + 63) / 64 + a.run_blocks - 1) / a.run_blocks : 0xFFFFFFFFu;
+  const size_t lds = static_cast<size_t>((a.rank + 31) / 32) * RT * (F32 ? 3 : 2) * 1024;
+  hipError_t e = allow_lds<adapter_expand_kernel<RT, F32>>(lds, 64 * 1024);
+  if (e != hipSuccess) return e;
+  adapter_expand_kernel<RT, F32><<<dim3(a.first_run[a.num_targets], tiles, turns), dim3(256), lds, s>>>(a);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -440,35 +524,25 @@ hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, u
 }
 
 size_t adapter_workspace_bytes(uint32_t num_targets, uint32_t rank, uint32_t n, uint32_t t) {
-  // rows times parts, and no less than for any smaller t: parts fall as 512 / (t / 16)
-  const uint64_t most = std::max<uint64_t>(t, std::min<uint64_t>(512 * 16, static_cast<uint64_t>(t) * shrink_splits(1, n)));
+  // rows times parts, and no less than for any smaller t: the parts fall as one over the tiles of 16 rows
+  const uint64_t most = std::max<uint64_t>(t, std::min<uint64_t>(kShrinkGroups * 16, static_cast<uint64_t>(t) * shrink_splits(1, n)));
   return most * num_targets * rank * sizeof(float);
 }
 
 hipError_t launch_adapter_apply(hipStream_t s, AdapterArgs a, bool y_f32) {
-  constexpr int kCols = 4;
   a.splits = shrink_splits(a.t, a.n);
-  const uint32_t col_blocks = (a.rank + 15) / 16 * a.num_targets, groups = (col_blocks + kCols - 1) / kCols;
   const bool planned = a.plan.tiles != nullptr;
-  // consecutive rows: several adapters of a tile at once where a batch has few tiles
-  const uint32_t tiles16 = std::max((a.t + 15) / 16, planned ? a.plan.most_tiles * (a.plan.tile_rows / 16) : 0);
-  const uint32_t turns = planned ? 1 : std::min({a.t, a.num_adapters, tiles16 > 16 ? 2u : 16u});
-  adapter_shrink_kernel<1, kCols><<<dim3(tiles16, groups * a.splits, turns), dim3(256), 0, s>>>(a);
-  hipError_t e = hipGetLastError();
+  const bool wide = planned ? a.plan.tile_rows == 64 : a.t > 256;  // 32 rows a workgroup instead of 16
+  const uint32_t rows = wide ? 32 : 16;
+  const uint32_t tiles = std::max((a.t + rows - 1) / rows, planned ? a.plan.most_tiles * (a.plan.tile_rows / rows) : 0);
+  // consecutive rows of a short batch: the adapters of a tile side by side
+  const uint32_t turns = planned || tiles > 4 ? 1 : std::min({a.t, a.num_adapters, 16u});
+  if (wide) launch_shrink<2>(s, a, tiles, turns);
+  else launch_shrink<1>(s, a, tiles, turns);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  uint32_t blocks = 0;
-  for (uint32_t k = 0; k < a.num_targets; ++k) blocks += (a.target[k].m + 63) / 64;
-  const uint32_t wide = planned ? a.plan.tile_rows == 64 : a.t > 256;
-  if (wide) {
-    const dim3 grid((blocks + 3) / 4, std::max((a.t + 63) / 64, planned ? a.plan.most_tiles : 0), turns);
-    if (y_f32) adapter_expand_kernel<4, true><<<grid, dim3(256), 0, s>>>(a);
-    else adapter_expand_kernel<4, false><<<grid, dim3(256), 0, s>>>(a);
-  } else {
-    const dim3 grid((blocks + 3) / 4, tiles16, turns);
-    if (y_f32) adapter_expand_kernel<1, true><<<grid, dim3(256), 0, s>>>(a);
-    else adapter_expand_kernel<1, false><<<grid, dim3(256), 0, s>>>(a);
-  }
-  return hipGetLastError();
+  if (wide) return y_f32 ? launch_expand<2, true>(s, a, tiles, turns) : launch_expand<2, false>(s, a, tiles, turns);
+  return y_f32 ? launch_expand<1, true>(s, a, tiles, turns) : launch_expand<1, false>(s, a, tiles, turns);
 }
 
 }  // namespace mf
