@@ -663,7 +663,7 @@ mf_status mf_moe_unpermute(mf_moe* h, mf_stream stream, const float* route_parti
 typedef struct {
   uint32_t num_adapters;  /* 1 .. MF_MAX_ADAPTERS */
   uint32_t rank;          /* a multiple of 8, 8 .. MF_MAX_ADAPTER_RANK */
-  uint32_t n;             /* length of a row of x, a multiple of 64 */
+  uint32_t n;             /* length of a row of x, a multiple of 64, 64 .. 2^22 */
   const uint32_t* ranks;  /* device [num_adapters], values 0 .. rank (larger ones count as rank); NULL: all `rank` */
   const float* scales;    /* device [num_adapters], c_a; NULL: all 1 */
 } mf_adapter_pool;

@@ -148,8 +148,8 @@ SIGNATURES = {
     "mf_adapter_plan_bytes": (_SZ, [_U32, _U32]),
     "mf_adapter_group": (_I, [_P, _P, _P, _U32, _U32, _P, _SZ]),
     "mf_adapter_workspace_bytes": (_SZ, [C.POINTER(AdapterPool), _U32, _U32]),
-    "mf_adapter_apply": (_I, [_P, _P, C.POINTER(AdapterPool), C.POINTER(AdapterTarget), _U32, _P, _U32, _P, _U32, _I, _P, _P, _SZ]),
-    "mf_block_norm": (_I, [_P, _P, C.POINTER(BlockNormArgs)]),
+    "mf_adapter_apply": (_I, [_P, _P, C.POINTER(AdapterPool), _P, _U32, _P, _U32, _P, _U32, _I, _P, _P, _SZ]),
+    "mf_block_norm": (_I, [_P, _P, _P]),
     "mf_group_pairs_host": (_I, [_P, _SZ, _I, _I, _I, _I, _P, _SZ, _P, _P, _P, _P,
                                  C.POINTER(_SZ), _P, C.POINTER(_SZ), _P]),
 }

@@ -20,7 +20,6 @@ __device__ __forceinline__ uint32_t adapter_key(int32_t id, uint32_t n) { return
 template <int IT>
 struct RowRanks {
   uint32_t key[IT], rank[IT];  // rank within the wave's rows of the key
-  uint64_t valid[IT];
 
   __device__ __forceinline__ void find(const int32_t* __restrict__ ids, uint32_t first, uint32_t t, uint32_t n, uint16_t* counts) {
     const uint32_t lane = threadIdx.x & 63, bits = 32 - __builtin_clz(n);
@@ -31,15 +30,15 @@ struct RowRanks {
     }
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      valid[k] = __ballot(first + k * 64 + lane < t);
-      uint64_t same = valid[k];
+      const bool valid = first + k * 64 + lane < t;
+      uint64_t same = __ballot(valid);
       for (uint32_t b = 0; b < bits; ++b) {
         const bool set = (key[k] >> b) & 1;
         const uint64_t with = __ballot(set);
         same &= set ? with : ~with;
       }
-      const uint32_t in_front = __builtin_popcountll(same & ((1ull << lane) - 1));
-      if ((valid[k] >> lane) & 1) {
+      const uint32_t in_front = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(same >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(same), 0));
+      if (valid) {
         const uint32_t before = counts[key[k]];
         rank[k] = before + in_front;
         if (in_front == 0) counts[key[k]] = static_cast<uint16_t>(before + __builtin_popcountll(same));
@@ -96,10 +95,15 @@ __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __re
       total.x = own;
       if (gridDim.x > 1) {
         total.x = 0;
-        for (uint32_t r = 0; r < gridDim.x; ++r) {
-          const uint32_t c = plan.runs[static_cast<size_t>(r) * keys + k];
-          before += r < blockIdx.x ? c : 0;
-          total.x += c;
+        for (uint32_t r = 0; r < gridDim.x; r += 16) {  // sixteen requested at once
+          uint32_t c[16];
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) c[i] = plan.runs[static_cast<size_t>(min(r + i, gridDim.x - 1)) * keys + k];
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) {
+            before += r + i < blockIdx.x ? c[i] : 0;
+            total.x += r + i < gridDim.x ? c[i] : 0;
+          }
         }
       }
       total.y = (total.x + plan.tile_rows - 1) / plan.tile_rows;
@@ -134,8 +138,8 @@ __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __re
     }
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if (!((mine.valid[i] >> (threadIdx.x & 63)) & 1)) continue;
-      plan.rows[starts[mine.key[i]] + counts[wave * keys + mine.key[i]] + mine.rank[i]] = first + i * 64 + (threadIdx.x & 63);
+      const uint32_t row = first + i * 64 + (threadIdx.x & 63);
+      if (row < t) plan.rows[starts[mine.key[i]] + counts[wave * keys + mine.key[i]] + mine.rank[i]] = row;
     }
   }
 }
@@ -144,27 +148,34 @@ __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __re
 
 __device__ __forceinline__ uint32_t live_rank(const AdapterArgs& a, uint32_t adapter) { return a.ranks ? min(a.ranks[adapter], a.rank) : a.rank; }
 
-// ROWS rows of the batch, a lane each (ROWS <= 64; the lanes behind hold none), and the adapters that they meet.  With a plan they are
+// ROWS rows of the batch, a lane each (ROWS <= 32; the lanes behind hold none), and the adapters that they meet.  With a plan they are
 // (a part of) one of its tiles, of one adapter; without one they are consecutive rows, whose adapters are taken one after the other in
 // the order of their first rows.  Every wave finds them for itself.
 template <int ROWS>
 struct Meeting {
+  static_assert(ROWS <= 32, "the lanes' bits are a word");
   uint32_t row;    // this lane's
   uint32_t key;    // its adapter, num_adapters where it has no row or no adapter
-  uint64_t left;   // lanes whose adapter is still to come
+  uint32_t left;   // lanes whose adapter is still to come
 
-  // PLAN_ROWS: rows of a tile of the plan
   __device__ __forceinline__ Meeting(const AdapterArgs& a, uint32_t tile, uint32_t lane) : row(0), key(a.num_adapters) {
-    if (a.plan.tiles && a.plan.header[0] == a.t && a.plan.header[1] == a.num_adapters) {
-      const uint32_t parts = a.plan.tile_rows / ROWS, of = tile / parts, from = tile % parts * ROWS;
-      if (of < a.plan.header[2] && of < a.plan.most_tiles) {
-        const uint2 rec = a.plan.tiles[of];
-        const uint32_t count = rec.x >> 16;
-        if (lane < ROWS && from + lane < count && rec.y + from + lane < a.t) {
-          row = a.plan.rows[rec.y + from + lane];
-          if (row < a.t) key = min(rec.x & 0xFFFFu, a.num_adapters);
-          else row = 0;
-        }
+    bool planned = false;
+    uint4 head = make_uint4(0, 0, 0, 0);
+    uint2 rec = make_uint2(0, 0);
+    uint32_t of = 0, from = 0;
+    if (a.plan.tiles) {
+      const uint32_t parts = a.plan.tile_rows / ROWS;
+      of = tile / parts, from = tile % parts * ROWS;
+      head = *reinterpret_cast<const uint4*>(a.plan.header);
+      rec = a.plan.tiles[min(of, a.plan.most_tiles - 1)];
+      planned = head.x == a.t && head.y == a.num_adapters;  // (what another batch left is not used)
+    }
+    if (planned) {
+      const uint32_t count = rec.x >> 16, at = rec.y + from + lane;
+      if (of < min(head.z, a.plan.most_tiles) && lane < ROWS && from + lane < count && at < a.t) {
+        row = a.plan.rows[at];
+        if (row < a.t) key = min(rec.x & 0xFFFFu, a.num_adapters);
+        else row = 0;
       }
     } else {
       const uint32_t r = tile * ROWS + lane;
@@ -173,14 +184,14 @@ struct Meeting {
         key = adapter_key(a.ids[r], a.num_adapters);
       }
     }
-    left = __ballot(key < a.num_adapters);
+    left = static_cast<uint32_t>(__ballot(key < a.num_adapters));
   }
   // the next adapter, and the lanes that have it; false when there is none left
-  __device__ __forceinline__ bool next(uint32_t& adapter, uint64_t& lanes, uint32_t& lead) {
+  __device__ __forceinline__ bool next(uint32_t& adapter, uint32_t& lanes, uint32_t& lead) {
     if (!left) return false;
-    lead = static_cast<uint32_t>(__builtin_ctzll(left));
+    lead = static_cast<uint32_t>(__builtin_ctz(left));
     adapter = __builtin_amdgcn_readlane(key, lead);
-    lanes = __ballot(key == adapter);
+    lanes = static_cast<uint32_t>(__ballot(key == adapter));
     left &= ~lanes;
     return true;
   }
@@ -192,92 +203,151 @@ __device__ __forceinline__ f32x4_t mfma16(const uint4& a, const uint4& b, const 
 
 // ------------------------------------------------------------------ v = c A x
 //
-// Operands of v_mfma_f32_16x16x32_bf16 are eight consecutive elements of a row a lane, of x (16 rows of the batch) and of A (16 ranks):
-// 16-byte loads straight into the registers that the instruction reads.  A workgroup takes RT * 16 rows, CF blocks of 16 ranks and a
-// window of the row length; its eight waves take 64 elements (a line of 128 bytes) in turn and add their sums through LDS.  A rank
-// beyond the adapter's, and a row of another one, is a column or a row of the product that nobody reads.
-constexpr uint32_t kShrinkWaves = 8;
+// v_mfma_f32_16x16x32_bf16 wants eight consecutive elements of a row a lane, and neighbouring lanes on different rows.  Loaded that
+// way a request touches 64 lines of memory for its 1024 bytes; so eight lanes take a line of 128 bytes, and the operands come from
+// LDS, where every wave has a place of its own: no barrier.  The 16-byte pieces of a row lie there exclusive-ored with the row's
+// number, so that neither side meets a bank twice.  A rank beyond the adapter's, and a row of another one, is a column or a row of
+// the product that nobody reads.
+constexpr int kWaves = 8;
 
+// What a wave stages at once: 64 elements of RT * 16 rows of x and of CF * 16 rows of A
 template <int RT, int CF>
-__global__ __launch_bounds__(kShrinkWaves * 64) void adapter_shrink_kernel(const AdapterArgs a) {
-  __shared__ f32x4_t part[kShrinkWaves][RT * CF][64];
+struct Stage {
+  static constexpr int kLoads = 2 * (RT + CF), kBytes = kLoads * 1024;
+  const uint16_t* x[2 * RT];  // the lane's row of each request, its piece of the line included
+  const uint16_t* w[CF];      // the adapter's rows of each block of 16 ranks
+  uint32_t in_w[CF][2];       // the lane's place there
+
+  __device__ __forceinline__ void rows_of_x(const AdapterArgs& a, uint32_t my_row, uint32_t lanes, uint32_t lead) {
+    const uint32_t lane = threadIdx.x & 63, piece = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) {
+      const uint32_t at = i * 8 + (lane >> 3);
+      const uint32_t row = __shfl(my_row, (lanes >> at) & 1 ? at : lead);
+      x[i] = a.x + static_cast<size_t>(row) * a.x_stride + piece * 8;
+    }
+  }
+  // block c of 16 ranks: from rank `first` on of the adapter's A, of which `have` exist
+  __device__ __forceinline__ void rows_of_a(int c, const uint16_t* adapter, uint32_t n, uint32_t first, uint32_t have) {
+    const uint32_t lane = threadIdx.x & 63, piece = (lane & 7) ^ (lane >> 3);
+    w[c] = first < have ? adapter + static_cast<size_t>(first) * n : adapter;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t r = i * 8 + (lane >> 3);
+      in_w[c][i] = (first + r < have ? r * n : 0) + piece * 8;
+    }
+  }
+
+  // The wave's part of the products over the units of 64 elements from u0 to u1, WAVES apart, left in `part` [block][lane].  It
+  // requests UNITS of them before it uses the first.  place: kBytes of LDS.
+  template <int WAVES, int UNITS>
+  __device__ __forceinline__ void multiply(uint32_t u0, uint32_t u1, uint4* place, f32x4_t* part) const {
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    f32x4_t acc[RT][CF];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < CF; ++c) acc[r][c] = f32x4_t{0, 0, 0, 0};
+    for (uint32_t u = u0 + wave; u < u1; u += UNITS * WAVES) {
+      uint4 v[UNITS][kLoads];
+#pragma unroll
+      for (int k = 0; k < UNITS; ++k) {
+        if (u + k * WAVES >= u1) break;
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i) v[k][i] = load_16_bytes(x[i] + (u + k * WAVES) * 64);
+#pragma unroll
+        for (int i = 0; i < 2 * CF; ++i) v[k][2 * RT + i] = *reinterpret_cast<const uint4*>(w[i / 2] + (u + k * WAVES) * 64 + in_w[i / 2][i % 2]);
+      }
+      issue_fence();
+#pragma unroll
+      for (int k = 0; k < UNITS; ++k) {
+        if (u + k * WAVES >= u1) break;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) place[i * 64 + lane] = v[k][i];
+        lane_order();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t at = (lane & 15) * 8 + ((h * 4 + (lane >> 4)) ^ (lane & 7));
+          uint4 xo[RT], wo[CF];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) xo[r] = place[r * 128 + at];
+#pragma unroll
+          for (int c = 0; c < CF; ++c) wo[c] = place[(RT + c) * 128 + at];
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int c = 0; c < CF; ++c) acc[r][c] = mfma16(xo[r], wo[c], acc[r][c]);
+        }
+        lane_order();
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < CF; ++c) part[(r * CF + c) * 64 + lane] = acc[r][c];
+  }
+  // other lanes' LDS stores in front of this come before this lane's loads behind it (a wave's LDS instructions run in order)
+  static __device__ __forceinline__ void lane_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// the waves' parts of a block, `apart` from each other
+template <int WAVES>
+__device__ __forceinline__ f32x4_t add_parts(const f32x4_t* part, uint32_t apart) {
+  f32x4_t sum[WAVES];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) sum[w] = part[w * apart + (threadIdx.x & 63)];
+#pragma unroll
+  for (int by = 1; by < WAVES; by *= 2)
+#pragma unroll
+    for (int w = 0; w < WAVES; w += 2 * by) sum[w] += sum[w + by];
+  return sum[0];
+}
+
+template <int RT, int CF> constexpr int kUnitsAhead = RT + CF <= 2 ? 4 : RT + CF <= 3 ? 3 : 2;
+
+// The first of two launches: v to memory, in parts over n.
+template <int RT, int CF>
+__global__ __launch_bounds__(kWaves * 64, RT + CF <= 4 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a) {
+  using S = Stage<RT, CF>;
+  __shared__ uint4 places[kWaves * S::kBytes / 16];  // a wave's place holds its part of the sums when it is done
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint4* place = places + wave * (S::kBytes / 16);
   const uint32_t split = blockIdx.y % a.splits, group = blockIdx.y / a.splits;
   const uint32_t blocks = (a.rank + 15) / 16;  // of 16 ranks, a target
   const uint32_t units = a.n / 64, u0 = units * split / a.splits, u1 = units * (split + 1) / a.splits;
-  const uint32_t in_row = (lane >> 4) * 8;
   Meeting<RT * 16> meeting(a, blockIdx.x, lane);
   uint32_t adapter, lead;
-  uint64_t lanes;
+  uint32_t lanes;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
     const uint32_t rank = live_rank(a, adapter);
     const float scale = a.scales ? a.scales[adapter] : 1.0f;
-    const uint16_t* xp[RT];
-    const uint16_t* wp[CF];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const uint32_t at = r * 16 + (lane & 15);
-      const uint32_t row = __shfl(meeting.row, (lanes >> at) & 1 ? at : lead);
-      xp[r] = a.x + static_cast<size_t>(row) * a.x_stride + in_row;
-    }
+    S stage;
+    stage.rows_of_x(a, meeting.row, lanes, lead);
     bool any = false;
 #pragma unroll
     for (int c = 0; c < CF; ++c) {
       const uint32_t cb = group * CF + c, target = cb / blocks, first = cb % blocks * 16;
       const bool live = target < a.num_targets && first < rank;
       any |= live;
-      const uint32_t r = first + (lane & 15);
-      wp[c] = a.target[live ? target : 0].a + (static_cast<size_t>(adapter) * a.rank + (live && r < rank ? r : 0)) * a.n + in_row;
+      stage.rows_of_a(c, a.target[live ? target : 0].a + static_cast<size_t>(adapter) * a.rank * a.n, a.n, first, live ? rank : 0);
     }
     if (!any) continue;
-    f32x4_t acc[RT][CF];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int c = 0; c < CF; ++c) acc[r][c] = f32x4_t{0, 0, 0, 0};
-    const auto step = [&](auto n_units, uint32_t u) {  // that many of the wave's units, all requested before the first is used
-      constexpr int kUnits = decltype(n_units)::value;
-      uint4 xv[RT][2 * kUnits], wv[CF][2 * kUnits];
-#pragma unroll
-      for (int k = 0; k < 2 * kUnits; ++k) {
-        const uint32_t at = (u + k / 2 * kShrinkWaves) * 64 + k % 2 * 32;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) xv[r][k] = load_16_bytes(xp[r] + at);
-#pragma unroll
-        for (int c = 0; c < CF; ++c) wv[c][k] = *reinterpret_cast<const uint4*>(wp[c] + at);
-      }
-#pragma unroll
-      for (int k = 0; k < 2 * kUnits; ++k)
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int c = 0; c < CF; ++c) acc[r][c] = mfma16(xv[r][k], wv[c][k], acc[r][c]);
-    };
-    uint32_t u = u0 + wave;
-    for (; u + kShrinkWaves < u1; u += 2 * kShrinkWaves) step(std::integral_constant<int, 2>{}, u);
-    if (u < u1) step(std::integral_constant<int, 1>{}, u);
     __syncthreads();  // (the parts of the adapter before have been read)
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-      for (int c = 0; c < CF; ++c) part[wave][r * CF + c][lane] = acc[r][c];
+    stage.template multiply<kWaves, kUnitsAhead<RT, CF>>(u0, u1, place, reinterpret_cast<f32x4_t*>(place));
     __syncthreads();
-    for (uint32_t f = wave; f < RT * CF; f += kShrinkWaves) {
-      f32x4_t sum[kShrinkWaves];
-#pragma unroll
-      for (uint32_t w = 0; w < kShrinkWaves; ++w) sum[w] = part[w][f][lane];
-#pragma unroll
-      for (uint32_t by = 1; by < kShrinkWaves; by *= 2)
-#pragma unroll
-        for (uint32_t w = 0; w < kShrinkWaves; w += 2 * by) sum[w] += sum[w + by];
+    for (uint32_t f = wave; f < RT * CF; f += kWaves) {
+      const f32x4_t sum = add_parts<kWaves>(reinterpret_cast<f32x4_t*>(places) + f * 64, S::kBytes / 16);
       const uint32_t cb = group * CF + f % CF, target = cb / blocks, r = cb % blocks * 16 + (lane & 15);
       const uint32_t row0 = f / CF * 16 + (lane >> 4) * 4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t row = __shfl(meeting.row, row0 + i);
         if (target < a.num_targets && r < rank && ((lanes >> (row0 + i)) & 1))
-          a.v[(static_cast<size_t>(split) * a.t + row) * a.cols + target * a.rank + r] = sum[0][i] * scale;
+          a.v[(static_cast<size_t>(split) * a.t + row) * a.cols + target * a.rank + r] = sum[i] * scale;
       }
     }
   }
@@ -320,94 +390,69 @@ __device__ __forceinline__ uint4 keep_bf16(uint4 v, uint32_t n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A workgroup takes RT * 16 rows and a run of a target's results.  It adds up the parts of v and leaves its terms in LDS as the
-// operands that the instruction reads; its waves then take 64 results in turn, the y and B of the next ones requested before the
-// present ones are worked on.
-template <int RT, bool F32>
-__global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a) {
-  constexpr int kTerms = F32 ? 3 : 2, kPer = F32 ? 4 : 8, kChunks = 16 / kPer;  // results to 16 bytes; such pieces a lane holds of a row
+// A workgroup's share of the results of one adapter's rows: its waves take 64 results in turn, the y and B of the next ones requested
+// before the present ones are worked on.
+template <int RT, bool F32, int WAVES>
+struct Expand {
+  static constexpr int kTerms = F32 ? 3 : 2, kPer = F32 ? 4 : 8, kChunks = 16 / kPer;  // results to 16 bytes; such pieces a lane holds of a row
   using Elem = std::conditional_t<F32, float, uint16_t>;
-  extern __shared__ uint4 operand[];  // [32 ranks][RT][kTerms][lane]
-  const uint32_t lane = threadIdx.x & 63, q = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint32_t run = blockIdx.x, target = 0;
-  while (run >= a.first_run[target + 1]) ++target;
-  run -= a.first_run[target];
-  const AdapterArgs::Target tg = a.target[target];
-  const uint32_t m_blocks = (tg.m + 63) / 64, end = min(m_blocks, (run + 1) * a.run_blocks);
-  Meeting<RT * 16> meeting(a, blockIdx.y, lane);
-  uint32_t adapter, lead;
-  uint64_t lanes;
-  for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
-    if (turn % gridDim.z != blockIdx.z) continue;
-    const uint16_t* bp = tg.b + static_cast<size_t>(adapter) * tg.m * a.rank;
-    Elem* yp[RT];
-    bool mine[RT];
+
+  const uint16_t* bp;
+  uint32_t m, rank_of_pool, q, in_b[4];  // in_b: the lane's elements of a block of 64 rows of B
+  Elem* yp[RT];
+  bool mine[RT];
+  uint4 yv[RT][kChunks], bv[4];
+
+  __device__ __forceinline__ void load_y(uint32_t block, uint4 (&v)[RT][kChunks]) const {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const uint32_t at = block * 64 + c * 4 * kPer + q * kPer;
+        if (mine[r] && at + kPer <= m) v[r][c] = load_16_bytes(yp[r] + at);
+      }
+  }
+  static __device__ __forceinline__ uint32_t row_of_b(int j, uint32_t p) { return F32 ? 16 * j + p : 32 * (j >> 1) + 8 * (p >> 2) + 4 * (j & 1) + (p & 3); }
+  __device__ __forceinline__ void load_b(uint32_t block, uint32_t k0, uint4 (&v)[4]) const {
+    const uint16_t* base = bp + static_cast<size_t>(block) * 64 * rank_of_pool + k0;
+    const uint32_t rows = m - block * 64;
+    if (k0 + q * 8 >= rank_of_pool) return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t in = in_b[j];
+      if (rows < 64) in = min(row_of_b(j, threadIdx.x & 15), rows - 1) * rank_of_pool + q * 8;
+      v[j] = *reinterpret_cast<const uint4*>(base + in);
+    }
+  }
+  // requests the wave's first results
+  __device__ __forceinline__ Expand(const AdapterArgs& a, const AdapterArgs::Target& tg, uint32_t adapter, uint32_t my_row, uint32_t lanes,
+                                    uint32_t lead, uint32_t block, uint32_t end) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t p = lane & 15;
+    q = lane >> 4;
+    m = tg.m, rank_of_pool = a.rank;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) in_b[j] = row_of_b(j, p) * a.rank + q * 8;
+    bp = tg.b + static_cast<size_t>(adapter) * m * a.rank;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const uint32_t at = r * 16 + (lane & 15);
+      const uint32_t at = r * 16 + p;
       mine[r] = (lanes >> at) & 1;
-      yp[r] = static_cast<Elem*>(tg.y) + static_cast<size_t>(__shfl(meeting.row, mine[r] ? at : lead)) * tg.y_stride;
+      yp[r] = static_cast<Elem*>(tg.y) + static_cast<size_t>(__shfl(my_row, mine[r] ? at : lead)) * tg.y_stride;
     }
-    const auto load_y = [&](uint32_t block, uint4 (&yv)[RT][kChunks]) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const uint32_t m = block * 64 + c * 4 * kPer + q * kPer;
-          if (mine[r] && m + kPer <= tg.m) yv[r][c] = load_16_bytes(yp[r] + m);
-        }
-    };
-    const auto load_b = [&](uint32_t block, uint32_t k, uint4 (&bv)[4]) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t p = lane & 15;
-        const uint32_t m = block * 64 + (F32 ? 16 * j + p : 32 * (j >> 1) + 8 * (p >> 2) + 4 * (j & 1) + (p & 3));
-        if (k < a.rank) bv[j] = *reinterpret_cast<const uint4*>(bp + static_cast<size_t>(min(m, tg.m - 1)) * a.rank + k);
-      }
-    };
-    uint32_t block = run * a.run_blocks + wave;
-    uint4 yv[RT][kChunks], bv[4];
     if (block < end) {
       load_y(block, yv);
-      load_b(block, q * 8, bv);
+      load_b(block, 0, bv);
     }
-    const uint32_t rank = live_rank(a, adapter), kb = (rank + 31) / 32;
-    __syncthreads();  // (the operands of the adapter before have been read)
-    for (uint32_t slot = threadIdx.x; slot < kb * RT * 64; slot += 256) {
-      const uint32_t at = slot / 64 % RT * 16 + (slot & 15), k = slot / (64 * RT) * 32 + (slot >> 4) % 4 * 8, have = k < rank ? min(rank - k, 8u) : 0;
-      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      const uint32_t row = __shfl(meeting.row, at);
-      if (have && ((lanes >> at) & 1)) {
-        const float* p = a.v + static_cast<size_t>(row) * a.cols + target * a.rank + k;
-        const size_t part = static_cast<size_t>(a.t) * a.cols;
-        for (uint32_t s = 0; s < a.splits; s += 4) {  // four parts requested at once
-          float4 lo[4], hi[4];
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const float4* w = reinterpret_cast<const float4*>(p + min(s + i, a.splits - 1) * part);
-            lo[i] = w[0], hi[i] = w[1];
-          }
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            if (s + i >= a.splits) continue;
-            v[0] += lo[i].x, v[1] += lo[i].y, v[2] += lo[i].z, v[3] += lo[i].w;
-            v[4] += hi[i].x, v[5] += hi[i].y, v[6] += hi[i].z, v[7] += hi[i].w;
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = static_cast<uint32_t>(e) < have ? v[e] : 0.0f;
-      uint4 terms[kTerms];
-      split_terms<kTerms>(v, terms);
-#pragma unroll
-      for (int i = 0; i < kTerms; ++i) operand[(slot / 64 * kTerms + i) * 64 + (slot & 63)] = terms[i];
-    }
-    __syncthreads();
-    for (; block < end; block += 4) {
+  }
+  // operand: [32 ranks][RT][kTerms][lane], the terms of v
+  __device__ __forceinline__ void run(uint32_t block, uint32_t end, uint32_t rank, const uint4* operand) {
+    const uint32_t lane = threadIdx.x & 63, kb = (rank + 31) / 32;
+    for (; block < end; block += WAVES) {
       uint4 next_y[RT][kChunks], next_b[4];
-      if (block + 4 < end) {
-        load_y(block + 4, next_y);
-        load_b(block + 4, q * 8, next_b);
+      if (block + WAVES < end) {
+        load_y(block + WAVES, next_y);
+        load_b(block + WAVES, 0, next_b);
       }
       f32x4_t acc[RT][4];
 #pragma unroll
@@ -416,7 +461,7 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
         for (int j = 0; j < 4; ++j) acc[r][j] = f32x4_t{0, 0, 0, 0};
       for (uint32_t b = 0; b < kb; ++b) {
         const uint32_t k = b * 32 + q * 8, have = k < rank ? min(rank - k, 8u) : 0;
-        if (b) load_b(block, k, bv);
+        if (b) load_b(block, b * 32, bv);
         if (rank % 32) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) bv[j] = have < 8 ? keep_bf16(bv[j], have) : bv[j];
@@ -435,24 +480,24 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
         if (!mine[r]) continue;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          const uint32_t m = block * 64 + c * 4 * kPer + q * kPer;
+          const uint32_t at = block * 64 + c * 4 * kPer + q * kPer;
           float add[kPer];
 #pragma unroll
           for (int e = 0; e < kPer; ++e) add[e] = acc[r][F32 ? c : 2 * c + e / 4][e % 4];
-          if (m + kPer <= tg.m) {
+          if (at + kPer <= m) {
             uint32_t w[4] = {yv[r][c].x, yv[r][c].y, yv[r][c].z, yv[r][c].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if constexpr (F32) w[e] = __float_as_uint(__uint_as_float(w[e]) + add[e]);
               else w[e] = static_cast<uint32_t>(narrow_bf16(bf16_lo(w[e]) + add[2 * e])) | static_cast<uint32_t>(narrow_bf16(bf16_hi(w[e]) + add[2 * e + 1])) << 16;
             }
-            __builtin_memcpy(yp[r] + m, w, 16);
+            __builtin_memcpy(yp[r] + at, w, 16);
           } else {
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
-              if (m + e >= tg.m) continue;
-              if constexpr (F32) yp[r][m + e] += add[e];
-              else yp[r][m + e] = narrow_bf16(bf16_to_f(yp[r][m + e]) + add[e]);
+              if (at + e >= m) continue;
+              if constexpr (F32) yp[r][at + e] += add[e];
+              else yp[r][at + e] = narrow_bf16(bf16_to_f(yp[r][at + e]) + add[e]);
             }
           }
         }
@@ -465,41 +510,197 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterArgs a
       for (int j = 0; j < 4; ++j) bv[j] = next_b[j];
     }
   }
+};
+
+// Slot `slot` of the operand: eight ranks (k on) of the tile's row `at`
+template <int RT>
+__device__ __forceinline__ void place_of_slot(uint32_t slot, uint32_t& at, uint32_t& k) {
+  at = slot / 64 % RT * 16 + (slot & 15);
+  k = slot / (64 * RT) * 32 + (slot >> 4) % 4 * 8;
+}
+template <int RT, int TERMS>
+__device__ __forceinline__ void store_terms(uint4* operand, uint32_t slot, const float (&v)[8]) {
+  uint4 terms[TERMS];
+  split_terms<TERMS>(v, terms);
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) operand[(slot / 64 * TERMS + i) * 64 + (slot & 63)] = terms[i];
 }
 
-// Parts of the sum over n: workgroups for one and a half times the CUs, of eight units of 64 elements (one a wave) or more, and few
-// parts where there are many rows (every part of v is written and read again).
-constexpr uint32_t kMostSplits = 16, kShrinkGroups = 384;
+// which target, and which of its blocks of 64 results, a workgroup has
+struct Share {
+  uint32_t target, first, end;
+  __device__ __forceinline__ Share(const AdapterArgs& a, uint32_t run) : target(0) {
+    while (run >= a.first_run[target + 1]) ++target;
+    first = (run - a.first_run[target]) * a.run_blocks;
+    end = min((a.target[target].m + 63) / 64, first + a.run_blocks);
+  }
+};
+
+// The second of two launches.  A workgroup takes RT * 16 rows and a run of a target's results, and adds up the parts of v itself.
+constexpr uint32_t kExpandWaves = 4;
+
+template <int RT, bool F32>
+__global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a) {
+  extern __shared__ uint4 operand[];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Share share(a, blockIdx.x);
+  const AdapterArgs::Target tg = a.target[share.target];
+  Meeting<RT * 16> meeting(a, blockIdx.y, lane);
+  uint32_t adapter, lead;
+  uint32_t lanes;
+  for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
+    if (turn % gridDim.z != blockIdx.z) continue;
+    Expand<RT, F32, kExpandWaves> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
+    const uint32_t rank = live_rank(a, adapter);
+    __syncthreads();  // (the operands of the adapter before have been read)
+    for (uint32_t slot = threadIdx.x; slot < (rank + 31) / 32 * RT * 64; slot += kExpandWaves * 64) {
+      uint32_t at, k;
+      place_of_slot<RT>(slot, at, k);
+      const uint32_t have = k < rank ? min(rank - k, 8u) : 0, row = __shfl(meeting.row, at);
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (have && ((lanes >> at) & 1)) {
+        const float* p = a.v + static_cast<size_t>(row) * a.cols + share.target * a.rank + k;
+        const size_t part = static_cast<size_t>(a.t) * a.cols;
+        for (uint32_t s = 0; s < a.splits; s += 4) {  // four parts requested at once
+          float4 lo[4], hi[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const float4* w = reinterpret_cast<const float4*>(p + min(s + i, a.splits - 1) * part);
+            lo[i] = w[0], hi[i] = w[1];
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            if (s + i >= a.splits) continue;
+            v[0] += lo[i].x, v[1] += lo[i].y, v[2] += lo[i].z, v[3] += lo[i].w;
+            v[4] += hi[i].x, v[5] += hi[i].y, v[6] += hi[i].z, v[7] += hi[i].w;
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<uint32_t>(e) < have ? v[e] : 0.0f;
+      store_terms<RT, Expand<RT, F32, kExpandWaves>::kTerms>(operand, slot, v);
+    }
+    __syncthreads();
+    expand.run(share.first + wave, share.end, rank, operand);
+  }
+}
+
+// ------------------------------------------------------------------ both in one launch
+//
+// Every workgroup makes the v of its rows and its target for itself, over the whole of n, and goes on to its results: nothing goes
+// through memory in between, and there is no second launch.  Workgroups that share rows make the same v, on compute units that
+// would have nothing else to do.
+template <int CF, bool F32>
+__global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const AdapterArgs a) {
+  constexpr int kTerms = F32 ? 3 : 2, kLd = CF * 16 + 4;
+  using S = Stage<1, CF>;
+  __shared__ uint4 lds[kWaves * S::kBytes / 16 + kTerms * 64];
+  __shared__ float vs[16 * kLd];  // [row][rank]
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint4* place = lds + wave * (S::kBytes / 16);  // the wave's; its part of the sums, and rows of B, later on
+  uint4* operand = lds + kWaves * (S::kBytes / 16);
+  const Share share(a, blockIdx.x);
+  const AdapterArgs::Target tg = a.target[share.target];
+  Meeting<16> meeting(a, blockIdx.y, lane);
+  uint32_t adapter, lead;
+  uint32_t lanes;
+  for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
+    if (turn % gridDim.z != blockIdx.z) continue;
+    S stage;
+    stage.rows_of_x(a, meeting.row, lanes, lead);
+    Expand<1, F32, kWaves> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
+#pragma unroll
+    for (int c = 0; c < CF; ++c) stage.rows_of_a(c, tg.a + static_cast<size_t>(adapter) * a.rank * a.n, a.n, c * 16, a.rank);  // not waiting for its own rank
+    if (turn) __syncthreads();  // (the parts of the adapter before have been read)
+    stage.template multiply<kWaves, kUnitsAhead<1, CF>>(0, a.n / 64, place, reinterpret_cast<f32x4_t*>(place));
+    const uint32_t rank = live_rank(a, adapter);
+    const float scale = a.scales ? a.scales[adapter] : 1.0f;
+    __syncthreads();
+    if (wave < CF) {
+      const f32x4_t sum = add_parts<kWaves>(reinterpret_cast<f32x4_t*>(lds) + wave * 64, S::kBytes / 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vs[((lane >> 4) * 4 + i) * kLd + wave * 16 + (lane & 15)] = sum[i] * scale;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t at, k;
+      place_of_slot<1>(lane, at, k);
+      float v[8];
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) v[e] = k + e < rank ? vs[at * kLd + k + e] : 0.0f;
+      store_terms<1, kTerms>(operand, lane, v);
+    }
+    __syncthreads();
+    if (rank) expand.run(share.first + wave, share.end, rank, operand);
+  }
+}
+
+// Parts of the sum over n: as many as give 16 rows two workgroups a CU over all their tiles, of eight units of 64 elements (one a wave)
+// or more, and few parts where there are many rows (every part of v is written and read again).
+constexpr uint32_t kMostSplits = 16, kShrinkGroups = 512;
 uint32_t shrink_splits(uint32_t t, uint32_t n) {
-  return std::max(1u, std::min({kShrinkGroups / ((t + 15) / 16), n / 64 / kShrinkWaves, kMostSplits}));
+  return std::max(1u, std::min({kShrinkGroups / ((t + 15) / 16), n / 64 / kWaves, t > 256 ? 4u : kMostSplits}));
+}
+
+// deals the results of all targets to workgroups: about `groups` of them for a tile's rows
+void deal_results(AdapterArgs& a, uint32_t groups, uint32_t waves) {
+  uint32_t blocks = 0;
+  for (uint32_t k = 0; k < a.num_targets; ++k) blocks += (a.target[k].m + 63) / 64;
+  a.run_blocks = std::max(1u, (blocks + groups - 1) / groups);
+  a.run_blocks = (a.run_blocks + waves - 1) / waves * waves;
+  a.first_run[0] = 0;
+  for (uint32_t k = 0; k < MF_MAX_ADAPTER_TARGETS; ++k)
+    a.first_run[k + 1] = k < a.num_targets ? a.first_run[k] + ((a.target[k].m + 63) / 64 + a.run_blocks - 1) / a.run_blocks : 0xFFFFFFFFu;
 }
 
 template <int RT>
-void launch_shrink(hipStream_t s, const AdapterArgs& a, uint32_t tiles, uint32_t turns) {
+hipError_t launch_shrink(hipStream_t s, const AdapterArgs& a, uint32_t tiles, uint32_t turns) {
   const uint32_t blocks = (a.rank + 15) / 16 * a.num_targets;
   const auto go = [&](auto cf) {
     constexpr int kCols = decltype(cf)::value;
-    adapter_shrink_kernel<RT, kCols><<<dim3(tiles, (blocks + kCols - 1) / kCols * a.splits, turns), dim3(kShrinkWaves * 64), 0, s>>>(a);
+    adapter_shrink_kernel<RT, kCols><<<dim3(tiles, (blocks + kCols - 1) / kCols * a.splits, turns), dim3(kWaves * 64), 0, s>>>(a);
   };
   if (blocks == 1) go(std::integral_constant<int, 1>{});
-  else if (blocks == 2) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 2>{});
+  return hipGetLastError();
 }
 
 template <int RT, bool F32>
 hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t turns) {
-  uint32_t blocks = 0;
-  for (uint32_t k = 0; k < a.num_targets; ++k) blocks += (a.target[k].m + 63) / 64;
-  // runs of results: workgroups for eight times the CUs where there is so much to do
-  a.run_blocks = std::max<uint32_t>(1, static_cast<uint32_t>(static_cast<uint64_t>(blocks) * tiles / (4 * 2048))) * 4;
-  a.first_run[0] = 0;
-  for (uint32_t k = 0; k < MF_MAX_ADAPTER_TARGETS; ++k)
-    a.first_run[k + 1] = k < a.num_targets ? a.first_run[k] + ((a.target[k].m + 63) / 64 + a.run_blocks - 1) / a.run_blocks : 0xFFFFFFFFu;
+  deal_results(a, std::max(1u, 8192 / (tiles * turns)), kExpandWaves);
   const size_t lds = static_cast<size_t>((a.rank + 31) / 32) * RT * (F32 ? 3 : 2) * 1024;
-  hipError_t e = allow_lds<adapter_expand_kernel<RT, F32>>(lds, 64 * 1024);
+  const hipError_t e = allow_lds<adapter_expand_kernel<RT, F32>>(lds, 64 * 1024);
   if (e != hipSuccess) return e;
-  adapter_expand_kernel<RT, F32><<<dim3(a.first_run[a.num_targets], tiles, turns), dim3(256), lds, s>>>(a);
+  adapter_expand_kernel<RT, F32><<<dim3(a.first_run[a.num_targets], tiles, turns), dim3(kExpandWaves * 64), lds, s>>>(a);
   return hipGetLastError();
+}
+
+struct Tiling {
+  uint32_t tiles, turns;
+  Tiling(const AdapterArgs& a, uint32_t rows) {
+    const bool planned = a.plan.tiles != nullptr;
+    tiles = std::max((a.t + rows - 1) / rows, planned ? a.plan.most_tiles * (a.plan.tile_rows / rows) : 0);
+    // consecutive rows of a short batch: the adapters of a tile side by side
+    turns = planned || tiles > 4 ? 1 : std::min({a.t, a.num_adapters, 16u});
+  }
+};
+
+template <bool F32>
+hipError_t launch_fused(hipStream_t s, AdapterArgs& a) {
+  const Tiling g(a, 16);
+  deal_results(a, std::max(1u, 256 / (g.tiles * g.turns)), kWaves);
+  const dim3 grid(a.first_run[a.num_targets], g.tiles, g.turns), block(kWaves * 64);
+  if (a.rank <= 16) adapter_fused_kernel<1, F32><<<grid, block, 0, s>>>(a);
+  else adapter_fused_kernel<2, F32><<<grid, block, 0, s>>>(a);
+  return hipGetLastError();
+}
+
+template <int RT, bool F32>
+hipError_t launch_two(hipStream_t s, AdapterArgs& a) {
+  const Tiling g(a, RT * 16);
+  a.splits = shrink_splits(a.t, a.n);
+  const hipError_t e = launch_shrink<RT>(s, a, g.tiles, g.turns);
+  return e != hipSuccess ? e : launch_expand<RT, F32>(s, a, g.tiles, g.turns);
 }
 
 }  // namespace
@@ -530,19 +731,18 @@ size_t adapter_workspace_bytes(uint32_t num_targets, uint32_t rank, uint32_t n, 
 }
 
 hipError_t launch_adapter_apply(hipStream_t s, AdapterArgs a, bool y_f32) {
-  a.splits = shrink_splits(a.t, a.n);
-  const bool planned = a.plan.tiles != nullptr;
-  const bool wide = planned ? a.plan.tile_rows == 64 : a.t > 256;  // 32 rows a workgroup instead of 16
-  const uint32_t rows = wide ? 32 : 16;
-  const uint32_t tiles = std::max((a.t + rows - 1) / rows, planned ? a.plan.most_tiles * (a.plan.tile_rows / rows) : 0);
-  // consecutive rows of a short batch: the adapters of a tile side by side
-  const uint32_t turns = planned || tiles > 4 ? 1 : std::min({a.t, a.num_adapters, 16u});
-  if (wide) launch_shrink<2>(s, a, tiles, turns);
-  else launch_shrink<1>(s, a, tiles, turns);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  if (wide) return y_f32 ? launch_expand<2, true>(s, a, tiles, turns) : launch_expand<2, false>(s, a, tiles, turns);
-  return y_f32 ? launch_expand<1, true>(s, a, tiles, turns) : launch_expand<1, false>(s, a, tiles, turns);
+  uint64_t results = 0;
+  for (uint32_t k = 0; k < a.num_targets; ++k) results += a.target[k].m;
+  results *= a.t;
+  // One launch where v costs a workgroup little (two blocks of ranks, half a megabyte of x and A) and the results are not so many that
+  // their streaming decides: us a pass in one launch / in two, two projections -- one row of 2048, rank 16, 8.1 / 11.3; rank 64 9.9 / 10.2
+  // (left to two); of 5120, rank 32, 10.0 / 10.3, rank 64 14.7 / 10.8; of 17408, rank 8, 16.4 / 11.0; eight rows of eight adapters, 5120,
+  // rank 16, 12.1 / 16.4; 2048 rows, 2048 to 2048, rank 32, 21.8 / 25.6; 4096 rows 33.8 / 36.6; 512 rows, 5120 to 17408 (18 million results), 39.9 / 35.3
+  if (a.rank <= 32 && static_cast<uint64_t>(a.rank + 16) * a.n * sizeof(uint16_t) <= (512u << 10) && results <= (16u << 20))
+    return y_f32 ? launch_fused<true>(s, a) : launch_fused<false>(s, a);
+  const bool wide = a.plan.tiles ? a.plan.tile_rows == 64 : a.t > 256;  // 32 rows a workgroup instead of 16
+  if (wide) return y_f32 ? launch_two<2, true>(s, a) : launch_two<2, false>(s, a);
+  return y_f32 ? launch_two<1, true>(s, a) : launch_two<1, false>(s, a);
 }
 
 }  // namespace mf

@@ -988,7 +988,7 @@ bool rows_meet(const Rows& a, const Rows& b, uint64_t t) {
 
 bool adapter_pool_ok(const mf_adapter_pool* p) {
   return p && p->num_adapters >= 1 && p->num_adapters <= MF_MAX_ADAPTERS && p->rank >= 8 && p->rank <= MF_MAX_ADAPTER_RANK &&
-         p->rank % 8 == 0 && p->n > 0 && p->n % MF_GROUP_SIZE == 0;
+         p->rank % 8 == 0 && p->n > 0 && p->n <= 1u << 22 && p->n % MF_GROUP_SIZE == 0;
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }

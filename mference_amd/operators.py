@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from struct import Struct
 from typing import Optional, Sequence
 from weakref import ref as _ref
 
@@ -240,29 +241,35 @@ def _on(context: MetalContext, stream) -> int:
     return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
 
 
-def _device_tensor(context: MetalContext, t: torch.Tensor, what: str, dtype) -> int:
+def _address(t: torch.Tensor, what: str, dtype, device: int) -> int:
     """the address of a tensor that lies on the context's device and has the type asked for"""
-    if not t.is_cuda:
-        raise ValueError(f"libmfmoe operates on device memory; {what} is a CPU tensor")
-    if t.dtype is not dtype:
-        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
-    if t.get_device() != context.device.index:
+    if t.dtype is not dtype or t.get_device() != device:
+        if not t.is_cuda:
+            raise ValueError(f"libmfmoe operates on device memory; {what} is a CPU tensor")
+        if t.dtype is not dtype:
+            raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
         raise ValueError(f"{what} lies on another device than the context")
     return t.data_ptr()
 
 
-def _rows_of(t: torch.Tensor, what: str, rows: int, width: int) -> int:
-    """elements from row to row of a [rows, width] tensor whose rows are contiguous"""
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != width:
-        raise MfError(-2, f"{what} is {tuple(t.shape)}, not ({rows}, {width})")
+def _row_stride(t: torch.Tensor, what: str, shape) -> int:
+    """elements from row to row of a tensor of this shape [rows, width] whose rows are contiguous"""
+    if t.shape != shape:
+        raise MfError(-2, f"{what} is {tuple(t.shape)}, not {tuple(shape)}")
+    rows, width = shape
+    if t.is_contiguous() or rows == 1 and (width == 1 or t.stride(1) == 1):
+        return width
     if width > 1 and t.stride(1) != 1:
         raise MfError(-1, f"the rows of {what} must be contiguous")
-    if rows < 2:
-        return width
     stride = t.stride(0)
     if stride < width:
         raise MfError(-2, f"the rows of {what} overlap")
     return stride
+
+
+def _vector(t: torch.Tensor, what: str, size: int) -> None:
+    if t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
+        raise MfError(-2, f"{what} must be a contiguous vector of {size}")
 
 
 class AdapterPlan:
@@ -292,17 +299,16 @@ class AdapterGrouping:
 
     def encode(self, adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> AdapterPlan:
         """adapter_of_row int32 [t]"""
-        ids = _device_tensor(self.context, adapter_of_row, "adapter_of_row", torch.int32)
+        ctx = self.context
+        ids = _address(adapter_of_row, "adapter_of_row", torch.int32, ctx.device.index)
         t = adapter_of_row.shape[0]
-        if adapter_of_row.dim() != 1 or (t > 1 and adapter_of_row.stride(0) != 1):
-            raise MfError(-1, "adapter_of_row must be a contiguous vector")
+        _vector(adapter_of_row, "adapter_of_row", t)
         if plan is None:
             plan = self.plan(t)
         elif plan.t != t or plan.num_adapters != self.num_adapters:
             raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
         words = plan.words
-        check(_capi.lib().mf_adapter_group(self.context.handle, _on(self.context, stream), ids, t, self.num_adapters,
-                                           words.data_ptr(), words.numel() * 4), self.context.handle)
+        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, words.data_ptr(), words.numel() * 4), ctx.handle)
         return plan
 
 
@@ -321,27 +327,26 @@ class LowRankAdapters:
         self.context = context
         self.num_adapters, self.rank, self.n = a[0].shape
         self.a, self.b, self.scales, self.ranks = a, b, scales, ranks  # kept: the pool's addresses stay valid
-        self._targets = (_capi.AdapterTarget * len(a))()
-        for g, wa, wb in zip(self._targets, a, b):
+        device = context.device.index
+        self._fixed = []  # a, b and m of every projection
+        for wa, wb in zip(a, b):
             if wa.shape != a[0].shape or wb.dim() != 3 or wb.shape[0] != self.num_adapters or wb.shape[2] != self.rank:
                 raise MfError(-2, f"a {tuple(wa.shape)}, b {tuple(wb.shape)}")
             if not (wa.is_contiguous() and wb.is_contiguous()):
                 raise MfError(-1, "the adapter pool must be contiguous")
-            g.a = _device_tensor(context, wa, "a", torch.bfloat16)
-            g.b = _device_tensor(context, wb, "b", torch.bfloat16)
-            g.m = wb.shape[1]
+            self._fixed.append((_address(wa, "a", torch.bfloat16, device), _address(wb, "b", torch.bfloat16, device), wb.shape[1]))
+        self._pack = Struct("@" + "PPPII" * len(a)).pack  # mf_adapter_target [len(a)]
         self.pool = _capi.AdapterPool(self.num_adapters, self.rank, self.n, None, None)
         for name, v, dtype in (("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
             if v is not None:
-                if v.shape != (self.num_adapters,) or not v.is_contiguous():
-                    raise MfError(-2, f"{name} must be a vector of num_adapters")
-                setattr(self.pool, name, _device_tensor(context, v, name, dtype))
+                _vector(v, name, self.num_adapters)
+                setattr(self.pool, name, _address(v, name, dtype, device))
         if self.workspace_bytes(1) == 0:
             raise MfError(-2, f"num_adapters={self.num_adapters} rank={self.rank} n={self.n}")
 
     def workspace_bytes(self, t: int) -> int:
         """bytes that a call of t rows, or fewer, asks for"""
-        return int(_capi.lib().mf_adapter_workspace_bytes(C.byref(self.pool), len(self._targets), t))
+        return int(_capi.lib().mf_adapter_workspace_bytes(C.byref(self.pool), len(self._fixed), t))
 
     def encode(self, x: torch.Tensor, adapter_of_row: torch.Tensor, ys, plan: Optional[AdapterPlan] = None,
                workspace: Optional[torch.Tensor] = None, stream=None) -> None:
@@ -349,42 +354,39 @@ class LowRankAdapters:
         are.  x bf16 [t, n]; ys[s] bf16 or float32 [t, m_s], all of one type.  plan: AdapterGrouping's of the same rows, for
         batches that mix many adapters.  Without a workspace the call takes one of its own from torch's allocator."""
         ctx = self.context
+        device = ctx.device.index
         if isinstance(ys, torch.Tensor):
             ys = (ys,)
-        if len(ys) != len(self._targets):
-            raise MfError(-2, f"{len(ys)} results for {len(self._targets)} projections")
+        if len(ys) != len(self._fixed):
+            raise MfError(-2, f"{len(ys)} results for {len(self._fixed)} projections")
         t = x.shape[0]
-        ids = _device_tensor(ctx, adapter_of_row, "adapter_of_row", torch.int32)
-        if adapter_of_row.dim() != 1 or adapter_of_row.shape[0] != t or (t > 1 and adapter_of_row.stride(0) != 1):
-            raise MfError(-2, f"adapter_of_row must be a contiguous vector of {t}")
-        x_ptr = _device_tensor(ctx, x, "x", torch.bfloat16)
-        x_stride = _rows_of(x, "x", t, self.n)
+        ids = _address(adapter_of_row, "adapter_of_row", torch.int32, device)
+        _vector(adapter_of_row, "adapter_of_row", t)
+        x_ptr = _address(x, "x", torch.bfloat16, device)
+        x_stride = _row_stride(x, "x", (t, self.n))
         dtype = ys[0].dtype
         if dtype is not torch.bfloat16 and dtype is not torch.float32:
             raise ValueError(f"the results must be bfloat16 or float32, not {dtype}")
-        targets = self._targets
-        targets = type(targets).from_buffer_copy(targets)  # two threads may use one object
-        for g, y in zip(targets, ys):
-            g.y = _device_tensor(ctx, y, "y", dtype)
-            g.y_stride = _rows_of(y, "y", t, g.m)
-        if t == 0:
-            return
+        targets = []
+        for (a, b, m), y in zip(self._fixed, ys):
+            targets += (a, b, _address(y, "y", dtype, device), m, _row_stride(y, "y", (t, m)))
         words = None
         if plan is not None:
             if plan.t != t or plan.num_adapters != self.num_adapters:
                 raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
             words = plan.words.data_ptr()
+        if t == 0:
+            return
         if workspace is None:
             workspace = torch.empty(self.workspace_bytes(t), dtype=torch.uint8, device=ctx.device)
             if stream is not None:
                 workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), ctx.device))
         elif not workspace.is_contiguous():
             raise MfError(-1, "the workspace must be contiguous")
-        elif workspace.get_device() != ctx.device.index:
+        elif workspace.get_device() != device:
             raise ValueError("the workspace lies on another device than the context")
-        check(_capi.lib().mf_adapter_apply(ctx.handle, _on(ctx, stream), C.byref(self.pool), targets, len(targets), x_ptr, x_stride,
-                                           ids, t, 1 if dtype is torch.float32 else 0, words, workspace.data_ptr(),
-                                           workspace.numel() * workspace.element_size()), ctx.handle)
+        check(_capi.lib().mf_adapter_apply(ctx.handle, _on(ctx, stream), C.byref(self.pool), self._pack(*targets), len(ys), x_ptr, x_stride, ids, t,
+                                           1 if dtype is torch.float32 else 0, words, workspace.data_ptr(), workspace.nbytes), ctx.handle)
 
 
 class BlockNorm:
@@ -402,38 +404,41 @@ class BlockNorm:
         """hidden bf16 [t, d] is updated in place: residual_scale * hidden + branch_scale * gate * norm(delta); out gets its norm.
         gate: GATE_ROW [t] or [t, 1] and GATE_ELEMENT [t, d] go through a sigmoid, GATE_CHANNEL [d] is taken as it is."""
         ctx, bf16 = self.context, torch.bfloat16
-        if hidden.dim() != 2:
+        device, shape = ctx.device.index, hidden.shape
+        if len(shape) != 2:
             raise MfError(-2, "hidden must be [t, d]")
-        t, d = hidden.shape
-        a = _capi.BlockNormArgs()
-        a.d, a.t, a.gate_kind = d, t, gate_kind
-        a.hidden, a.hidden_stride = _device_tensor(ctx, hidden, "hidden", bf16), _rows_of(hidden, "hidden", t, d)
+        t, d = shape
+        h_ptr, h_stride = _address(hidden, "hidden", bf16, device), _row_stride(hidden, "hidden", shape)
+        d_ptr = d_stride = f32 = o_ptr = o_stride = g_ptr = g_stride = pre = post = 0
         if delta is not None:
-            a.delta_f32 = 1 if delta.dtype is torch.float32 else 0
-            a.delta = _device_tensor(ctx, delta, "delta", torch.float32 if a.delta_f32 else bf16)
-            a.delta_stride = _rows_of(delta, "delta", t, d)
+            f32 = 1 if delta.dtype is torch.float32 else 0
+            d_ptr, d_stride = _address(delta, "delta", torch.float32 if f32 else bf16, device), _row_stride(delta, "delta", shape)
         if out is not None:
-            a.out, a.out_stride = _device_tensor(ctx, out, "out", bf16), _rows_of(out, "out", t, d)
-        for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
-            if w is not None:
-                if w.dim() != 1 or w.shape[0] != d or (d > 1 and w.stride(0) != 1):
-                    raise MfError(-2, f"{name} must be a contiguous vector of {d}")
-                setattr(a, name, _device_tensor(ctx, w, name, bf16))
+            o_ptr, o_stride = _address(out, "out", bf16, device), _row_stride(out, "out", shape)
+        if pre_weight is not None:
+            _vector(pre_weight, "pre_weight", d)
+            pre = _address(pre_weight, "pre_weight", bf16, device)
+        if post_weight is not None:
+            _vector(post_weight, "post_weight", d)
+            post = _address(post_weight, "post_weight", bf16, device)
         if gate is not None:
-            a.gate = _device_tensor(ctx, gate, "gate", bf16)
+            g_ptr = _address(gate, "gate", bf16, device)
             if gate_kind == GATE_ROW:
                 if gate.numel() != t or gate.dim() > 2 or gate.shape[0] != t:
                     raise MfError(-2, f"the gate must be one logit for each of {t} rows")
-                a.gate_stride = gate.stride(0) if t > 1 else 1
-                if a.gate_stride == 0 and t > 1:  # 0 means "not given" to the library
+                g_stride = gate.stride(0) if t > 1 else 1
+                if g_stride == 0 and t > 1:  # 0 means "not given" to the library
                     raise MfError(-2, "a gate of one logit a row cannot be an expanded one")
             elif gate_kind == GATE_ELEMENT:
-                a.gate_stride = _rows_of(gate, "gate", t, d)
-            elif gate.dim() != 1 or gate.shape[0] != d or (d > 1 and gate.stride(0) != 1):
-                raise MfError(-2, f"the gate must be a contiguous vector of {d}")
-        a.pre_eps, a.post_eps = eps, eps if post_eps is None else post_eps
-        a.residual_scale, a.branch_scale, a.weight_bias = residual_scale, branch_scale, weight_bias
-        check(_capi.lib().mf_block_norm(ctx.handle, _on(ctx, stream), C.byref(a)), ctx.handle)
+                g_stride = _row_stride(gate, "gate", shape)
+            else:
+                _vector(gate, "gate", d)
+        args = self._pack(h_ptr, d_ptr, g_ptr, post, pre, o_ptr, d, t, h_stride, d_stride, g_stride, o_stride, f32, gate_kind,
+                          eps if post_eps is None else post_eps, eps, residual_scale, branch_scale, weight_bias)
+        check(_capi.lib().mf_block_norm(ctx.handle, _on(ctx, stream), args), ctx.handle)
+
+    _pack = Struct("@6P6I2i5f4x").pack  # mf_block_norm_args
+
 
 class SharedExpertInt4:
     """Kernels/MoE/SharedExpertInt4.swift:70-165 (also the dense SwiGLU MLP)."""

@@ -253,7 +253,18 @@ def test_operators_refuse_before_the_library():
 
 def test_rows_of_a_tensor():
     whole = torch.zeros(6, 40)
-    assert ops._rows_of(whole[:, 8:24], "x", 6, 16) == 40 and ops._rows_of(whole[::2], "x", 3, 40) == 80 and ops._rows_of(whole[:1], "x", 1, 40) == 40
-    for bad in (whole.t(), whole[:, ::2], whole[0].expand(6, 40), whole[:, :20]):
+    for v, stride in ((whole, 40), (whole[:, 8:24], 40), (whole[::2], 80), (whole[:1], 40), (whole[:1, 3:5], 2), (whole[:, :1], 40), (whole[:0], 40)):
+        assert ops._row_stride(v, "x", v.shape) == stride
+    for bad in (whole.t(), whole[:, ::2], whole[0].expand(6, 40), whole[:1].expand(2, 40)):
         with pytest.raises(ops.MfError):
-            ops._rows_of(bad, "x", 6, 40 if bad.shape[1] != 20 else 40)
+            ops._row_stride(bad, "x", bad.shape)
+    with pytest.raises(ops.MfError):
+        ops._row_stride(whole, "x", (6, 41))
+
+
+def test_packed_arguments_are_the_structures():
+    """the operators pack their arguments by hand: the same bytes as the ctypes structures'"""
+    values = tuple(range(1 << 40, (1 << 40) + 6)) + (7, 8, 9, 10, 11, 12, 1, 2, 0.5, 0.25, 2.0, 4.0, 1.0)
+    assert ops.BlockNorm._pack(*values) == bytes(_capi.BlockNormArgs(*values))
+    one, two = (1 << 40, 1 << 41, 1 << 42, 96, 192), (1 << 43, 1 << 44, 1 << 45, 64, 192)
+    assert ops.Struct("@" + "PPPII" * 2).pack(*one, *two) == bytes(_capi.AdapterTarget(*one)) + bytes(_capi.AdapterTarget(*two))
