@@ -156,7 +156,9 @@ struct Meeting {
   static_assert(ROWS <= 32, "the lanes' bits are a word");
   uint32_t row;    // this lane's
   uint32_t key;    // its adapter, num_adapters where it has no row or no adapter
-  uint32_t left;   // lanes whose adapter is still to come
+  // Lanes whose adapter is still to come.  A word: a 64-bit shift by a register reads a second one behind it, and where the amount lay in
+  // the last register of a wave some lanes got a wrong mask and took another row's x.
+  uint32_t left;
 
   __device__ __forceinline__ Meeting(const AdapterArgs& a, uint32_t tile, uint32_t lane) : row(0), key(a.num_adapters) {
     bool planned = false;
@@ -217,11 +219,14 @@ struct Stage {
   const uint16_t* x[2 * RT];  // the lane's row of each request, its piece of the line included
   const uint16_t* w[CF];      // the adapter's rows of each block of 16 ranks
   uint32_t in_w[CF][2];       // the lane's place there
+  uint32_t used;              // bit i: one of the rows of x of request i is the adapter's (the others need not be there)
 
   __device__ __forceinline__ void rows_of_x(const AdapterArgs& a, uint32_t my_row, uint32_t lanes, uint32_t lead) {
     const uint32_t lane = threadIdx.x & 63, piece = (lane & 7) ^ (lane >> 3);
+    used = 0;
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i) {
+      used |= (lanes >> (i * 8)) & 0xFFu ? 1u << i : 0u;
       const uint32_t at = i * 8 + (lane >> 3);
       const uint32_t row = __shfl(my_row, (lanes >> at) & 1 ? at : lead);
       x[i] = a.x + static_cast<size_t>(row) * a.x_stride + piece * 8;
@@ -254,7 +259,8 @@ struct Stage {
       for (int k = 0; k < UNITS; ++k) {
         if (u + k * WAVES >= u1) break;
 #pragma unroll
-        for (int i = 0; i < 2 * RT; ++i) v[k][i] = load_16_bytes(x[i] + (u + k * WAVES) * 64);
+        for (int i = 0; i < 2 * RT; ++i)
+          if (used >> i & 1) v[k][i] = load_16_bytes(x[i] + (u + k * WAVES) * 64);
 #pragma unroll
         for (int i = 0; i < 2 * CF; ++i) v[k][2 * RT + i] = *reinterpret_cast<const uint4*>(w[i / 2] + (u + k * WAVES) * 64 + in_w[i / 2][i % 2]);
       }
@@ -263,7 +269,8 @@ struct Stage {
       for (int k = 0; k < UNITS; ++k) {
         if (u + k * WAVES >= u1) break;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) place[i * 64 + lane] = v[k][i];
+        for (int i = 0; i < kLoads; ++i)
+          if (i >= 2 * RT || (used >> i & 1)) place[i * 64 + lane] = v[k][i];
         lane_order();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -276,7 +283,7 @@ struct Stage {
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int c = 0; c < CF; ++c) acc[r][c] = mfma16(xo[r], wo[c], acc[r][c]);
+            for (int c = 0; c < CF; ++c) acc[r][c] = mfma16(wo[c], xo[r], acc[r][c]);
         }
         lane_order();
       }
@@ -293,12 +300,12 @@ struct Stage {
   }
 };
 
-// the waves' parts of a block, `apart` from each other
+// the waves' parts of four sums, `apart` from each other
 template <int WAVES>
 __device__ __forceinline__ f32x4_t add_parts(const f32x4_t* part, uint32_t apart) {
   f32x4_t sum[WAVES];
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) sum[w] = part[w * apart + (threadIdx.x & 63)];
+  for (int w = 0; w < WAVES; ++w) sum[w] = part[w * apart];
 #pragma unroll
   for (int by = 1; by < WAVES; by *= 2)
 #pragma unroll
@@ -306,21 +313,22 @@ __device__ __forceinline__ f32x4_t add_parts(const f32x4_t* part, uint32_t apart
   return sum[0];
 }
 
-template <int RT, int CF> constexpr int kUnitsAhead = RT + CF <= 2 ? 4 : RT + CF <= 3 ? 3 : 2;
+// units requested at once: what 128 registers a lane hold
+template <int RT, int CF> constexpr int kUnitsAhead = 6 - RT - CF;
 
 // The first of two launches: v to memory, in parts over n.
 template <int RT, int CF>
-__global__ __launch_bounds__(kWaves * 64, RT + CF <= 4 ? 4 : 2) void adapter_shrink_kernel(const AdapterArgs a) {
+__global__ __launch_bounds__(kWaves * 64, 4) void adapter_shrink_kernel(const AdapterArgs a) {
   using S = Stage<RT, CF>;
   __shared__ uint4 places[kWaves * S::kBytes / 16];  // a wave's place holds its part of the sums when it is done
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint4* place = places + wave * (S::kBytes / 16);
-  const uint32_t split = blockIdx.y % a.splits, group = blockIdx.y / a.splits;
+  // parts side by side: with eight of them (or their multiples) every XCD has a window of x and A of its own
+  const uint32_t split = blockIdx.x % a.splits, group = blockIdx.y;
   const uint32_t blocks = (a.rank + 15) / 16;  // of 16 ranks, a target
   const uint32_t units = a.n / 64, u0 = units * split / a.splits, u1 = units * (split + 1) / a.splits;
-  Meeting<RT * 16> meeting(a, blockIdx.x, lane);
-  uint32_t adapter, lead;
-  uint32_t lanes;
+  Meeting<RT * 16> meeting(a, blockIdx.x / a.splits, lane);
+  uint32_t adapter, lanes, lead;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
     const uint32_t rank = live_rank(a, adapter);
@@ -340,15 +348,11 @@ __global__ __launch_bounds__(kWaves * 64, RT + CF <= 4 ? 4 : 2) void adapter_shr
     stage.template multiply<kWaves, kUnitsAhead<RT, CF>>(u0, u1, place, reinterpret_cast<f32x4_t*>(place));
     __syncthreads();
     for (uint32_t f = wave; f < RT * CF; f += kWaves) {
-      const f32x4_t sum = add_parts<kWaves>(reinterpret_cast<f32x4_t*>(places) + f * 64, S::kBytes / 16);
-      const uint32_t cb = group * CF + f % CF, target = cb / blocks, r = cb % blocks * 16 + (lane & 15);
-      const uint32_t row0 = f / CF * 16 + (lane >> 4) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t row = __shfl(meeting.row, row0 + i);
-        if (target < a.num_targets && r < rank && ((lanes >> (row0 + i)) & 1))
-          a.v[(static_cast<size_t>(split) * a.t + row) * a.cols + target * a.rank + r] = sum[i] * scale;
-      }
+      const f32x4_t sum = add_parts<kWaves>(reinterpret_cast<f32x4_t*>(places) + f * 64 + lane, S::kBytes / 16) * scale;
+      const uint32_t cb = group * CF + f % CF, target = cb / blocks, r = cb % blocks * 16 + (lane >> 4) * 4;
+      const uint32_t at = f / CF * 16 + (lane & 15), row = __shfl(meeting.row, at);
+      if (target < a.num_targets && r < rank && ((lanes >> at) & 1))  // (four ranks: rank of the pool is a multiple of eight)
+        *reinterpret_cast<f32x4_t*>(a.v + (static_cast<size_t>(split) * a.t + row) * a.cols + target * a.rank + r) = sum;
     }
   }
 }
@@ -546,8 +550,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
   const Share share(a, blockIdx.x);
   const AdapterArgs::Target tg = a.target[share.target];
   Meeting<RT * 16> meeting(a, blockIdx.y, lane);
-  uint32_t adapter, lead;
-  uint32_t lanes;
+  uint32_t adapter, lanes, lead;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
     Expand<RT, F32, kExpandWaves> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
@@ -561,15 +564,16 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
       if (have && ((lanes >> at) & 1)) {
         const float* p = a.v + static_cast<size_t>(row) * a.cols + share.target * a.rank + k;
         const size_t part = static_cast<size_t>(a.t) * a.cols;
-        for (uint32_t s = 0; s < a.splits; s += 4) {  // four parts requested at once
-          float4 lo[4], hi[4];
+        constexpr uint32_t kAhead = RT == 1 ? 8 : 4;  // parts requested at once
+        for (uint32_t s = 0; s < a.splits; s += kAhead) {
+          float4 lo[kAhead], hi[kAhead];
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
+          for (uint32_t i = 0; i < kAhead; ++i) {
             const float4* w = reinterpret_cast<const float4*>(p + min(s + i, a.splits - 1) * part);
             lo[i] = w[0], hi[i] = w[1];
           }
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
+          for (uint32_t i = 0; i < kAhead; ++i) {
             if (s + i >= a.splits) continue;
             v[0] += lo[i].x, v[1] += lo[i].y, v[2] += lo[i].z, v[3] += lo[i].w;
             v[4] += hi[i].x, v[5] += hi[i].y, v[6] += hi[i].z, v[7] += hi[i].w;
@@ -581,7 +585,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
       store_terms<RT, Expand<RT, F32, kExpandWaves>::kTerms>(operand, slot, v);
     }
     __syncthreads();
-    expand.run(share.first + wave, share.end, rank, operand);
+    if (rank) expand.run(share.first + wave, share.end, rank, operand);
   }
 }
 
@@ -592,18 +596,20 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
 // would have nothing else to do.
 template <int CF, bool F32>
 __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const AdapterArgs a) {
-  constexpr int kTerms = F32 ? 3 : 2, kLd = CF * 16 + 4;
+  constexpr int kTerms = F32 ? 3 : 2;
   using S = Stage<1, CF>;
   __shared__ uint4 lds[kWaves * S::kBytes / 16 + kTerms * 64];
-  __shared__ float vs[16 * kLd];  // [row][rank]
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint4* place = lds + wave * (S::kBytes / 16);  // the wave's; its part of the sums, and rows of B, later on
+  uint4* place = lds + wave * (S::kBytes / 16);  // the wave's; its part of the sums later on
   uint4* operand = lds + kWaves * (S::kBytes / 16);
-  const Share share(a, blockIdx.x);
+  const uint32_t runs = a.first_run[a.num_targets];
+  // workgroups of one tile share x and A: on one XCD where there are tiles for all of them (200 mixed rows of 2816, rank 24, two times
+  // 2112: 14.3 -> 12.9 us, 1500 rows of 2048, rank 32, two times 2048: 21.2 -> 20.4)
+  const uint32_t tile = a.by_xcd ? blockIdx.x / 8 / runs * 8 + blockIdx.x % 8 : blockIdx.x / runs;
+  const Share share(a, (a.by_xcd ? blockIdx.x / 8 : blockIdx.x) % runs);
   const AdapterArgs::Target tg = a.target[share.target];
-  Meeting<16> meeting(a, blockIdx.y, lane);
-  uint32_t adapter, lead;
-  uint32_t lanes;
+  Meeting<16> meeting(a, tile, lane);
+  uint32_t adapter, lanes, lead;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
     S stage;
@@ -616,27 +622,28 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const Ada
     const uint32_t rank = live_rank(a, adapter);
     const float scale = a.scales ? a.scales[adapter] : 1.0f;
     __syncthreads();
-    if (wave < CF) {
-      const f32x4_t sum = add_parts<kWaves>(reinterpret_cast<f32x4_t*>(lds) + wave * 64, S::kBytes / 16);
+    if (wave < CF) {  // a block of ranks a wave; a lane of the operand has eight of a row: its own four and those of the lane 16 behind
+      const f32x4_t lo = add_parts<kWaves>(reinterpret_cast<f32x4_t*>(lds) + wave * 64 + lane, S::kBytes / 16) * scale;
+      f32x4_t hi;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vs[((lane >> 4) * 4 + i) * kLd + wave * 16 + (lane & 15)] = sum[i] * scale;
-    }
-    __syncthreads();
-    if (wave == 0) {
-      uint32_t at, k;
-      place_of_slot<1>(lane, at, k);
+      for (int e = 0; e < 4; ++e) hi[e] = __shfl_down(lo[e], 16);
+      const uint32_t k = wave * 16 + (lane >> 4) * 4;
       float v[8];
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) v[e] = k + e < rank ? vs[at * kLd + k + e] : 0.0f;
-      store_terms<1, kTerms>(operand, lane, v);
+      for (uint32_t e = 0; e < 8; ++e) v[e] = k + e < rank ? (e < 4 ? lo[e] : hi[e - 4]) : 0.0f;
+      if ((lane & 16) == 0) store_terms<1, kTerms>(operand, wave * 32 + (lane >> 5) * 16 + (lane & 15), v);
+    }
+    if (CF == 1 && wave == 1) {  // the ranks from 16 on: none
+      const float none[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (lane >= 32) store_terms<1, kTerms>(operand, lane, none);
     }
     __syncthreads();
     if (rank) expand.run(share.first + wave, share.end, rank, operand);
   }
 }
 
-// Parts of the sum over n: as many as give 16 rows two workgroups a CU over all their tiles, of eight units of 64 elements (one a wave)
-// or more, and few parts where there are many rows (every part of v is written and read again).
+// Parts of the sum over n: for two workgroups a CU, of eight units of 64 elements (one a wave) or more; few of them where there are
+// many rows, since every part of v is written and read again (777 rows, rank 64, two projections: four parts 13.0 + 12.6 us, eight 13.0 + 15.0).
 constexpr uint32_t kMostSplits = 16, kShrinkGroups = 512;
 uint32_t shrink_splits(uint32_t t, uint32_t n) {
   return std::max(1u, std::min({kShrinkGroups / ((t + 15) / 16), n / 64 / kWaves, t > 256 ? 4u : kMostSplits}));
@@ -658,7 +665,7 @@ hipError_t launch_shrink(hipStream_t s, const AdapterArgs& a, uint32_t tiles, ui
   const uint32_t blocks = (a.rank + 15) / 16 * a.num_targets;
   const auto go = [&](auto cf) {
     constexpr int kCols = decltype(cf)::value;
-    adapter_shrink_kernel<RT, kCols><<<dim3(tiles, (blocks + kCols - 1) / kCols * a.splits, turns), dim3(kWaves * 64), 0, s>>>(a);
+    adapter_shrink_kernel<RT, kCols><<<dim3(tiles * a.splits, (blocks + kCols - 1) / kCols, turns), dim3(kWaves * 64), 0, s>>>(a);
   };
   if (blocks == 1) go(std::integral_constant<int, 1>{});
   else go(std::integral_constant<int, 2>{});
@@ -689,7 +696,8 @@ template <bool F32>
 hipError_t launch_fused(hipStream_t s, AdapterArgs& a) {
   const Tiling g(a, 16);
   deal_results(a, std::max(1u, 256 / (g.tiles * g.turns)), kWaves);
-  const dim3 grid(a.first_run[a.num_targets], g.tiles, g.turns), block(kWaves * 64);
+  a.by_xcd = g.tiles >= 32;
+  const dim3 grid(a.first_run[a.num_targets] * (a.by_xcd ? (g.tiles + 7) / 8 * 8 : g.tiles), 1, g.turns), block(kWaves * 64);
   if (a.rank <= 16) adapter_fused_kernel<1, F32><<<grid, block, 0, s>>>(a);
   else adapter_fused_kernel<2, F32><<<grid, block, 0, s>>>(a);
   return hipGetLastError();

@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int kAbiVersion = 2;  // 2: mf_moe_config.gate_group_size
+constexpr int kAbiVersion = 3;  // 2: mf_moe_config.gate_group_size; 3: low-rank adapters, block norms
 // rows of router logits a handle holds for mf_moe_router calls that bring no logits buffer
 constexpr uint32_t kRouterRows = 256;
 

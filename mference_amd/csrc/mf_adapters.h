@@ -46,7 +46,7 @@ struct AdapterArgs {
   const uint16_t* x;
   const int32_t* ids;
   float* v;  // [splits, t, cols]: c_a A x in parts, targets side by side
-  uint32_t num_targets, num_adapters, rank, n, t, x_stride, cols, splits;
+  uint32_t num_targets, num_adapters, rank, n, t, x_stride, cols, splits, by_xcd;
   uint32_t run_blocks, first_run[MF_MAX_ADAPTER_TARGETS + 1];  // a workgroup's share of the results: blocks of 64, and where each target's begin
   AdapterPlan plan;  // tiles null: the rows as they lie
 };

@@ -276,6 +276,9 @@ class AdapterPlan:
     """What AdapterGrouping.encode fills: the rows of a batch in the order of their adapters (mf_adapter_group)."""
 
     def __init__(self, t: int, num_adapters: int, words: torch.Tensor):
+        need = int(_capi.lib().mf_adapter_plan_bytes(t, num_adapters)) if t >= 0 and num_adapters > 0 else 0
+        if need == 0 or words.dtype is not torch.int32 or words.dim() != 1 or not words.is_contiguous() or words.numel() * 4 < need:
+            raise MfError(-1, f"t={t}, num_adapters={num_adapters}: {need // 4} contiguous int32 words")
         self.t, self.num_adapters, self.words = t, num_adapters, words
         self.rows = words[:t]                               # int32 [t]: row numbers, stably sorted, rows without an adapter last
         self.offsets = words[t:t + num_adapters + 1]        # int32: where every adapter's rows start; then the rows without one
@@ -293,9 +296,7 @@ class AdapterGrouping:
     def plan(self, t: int) -> AdapterPlan:
         """room for the plan of t rows"""
         need = int(_capi.lib().mf_adapter_plan_bytes(t, self.num_adapters)) if t >= 0 else 0
-        if need == 0:
-            raise MfError(-1, f"t={t}")
-        return AdapterPlan(t, self.num_adapters, torch.empty(need // 4, dtype=torch.int32, device=self.context.device))
+        return AdapterPlan(t, self.num_adapters, torch.empty(need // 4, dtype=torch.int32, device=self.context.device if need else "cpu"))
 
     def encode(self, adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> AdapterPlan:
         """adapter_of_row int32 [t]"""
@@ -308,7 +309,8 @@ class AdapterGrouping:
         elif plan.t != t or plan.num_adapters != self.num_adapters:
             raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
         words = plan.words
-        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, words.data_ptr(), words.numel() * 4), ctx.handle)
+        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, _address(words, "the plan", torch.int32, ctx.device.index),
+                                           words.numel() * 4), ctx.handle)
         return plan
 
 
@@ -374,7 +376,7 @@ class LowRankAdapters:
         if plan is not None:
             if plan.t != t or plan.num_adapters != self.num_adapters:
                 raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
-            words = plan.words.data_ptr()
+            words = _address(plan.words, "the plan", torch.int32, device)
         if t == 0:
             return
         if workspace is None:

@@ -268,3 +268,12 @@ def test_packed_arguments_are_the_structures():
     assert ops.BlockNorm._pack(*values) == bytes(_capi.BlockNormArgs(*values))
     one, two = (1 << 40, 1 << 41, 1 << 42, 96, 192), (1 << 43, 1 << 44, 1 << 45, 64, 192)
     assert ops.Struct("@" + "PPPII" * 2).pack(*one, *two) == bytes(_capi.AdapterTarget(*one)) + bytes(_capi.AdapterTarget(*two))
+
+
+def test_a_plan_has_room():
+    need = _capi.lib().mf_adapter_plan_bytes(40, 3) // 4
+    assert ops.AdapterPlan(40, 3, torch.zeros(need, dtype=torch.int32)).rows.numel() == 40
+    for t, n, words in ((40, 3, torch.zeros(need - 1, dtype=torch.int32)), (40, 3, torch.zeros(need, dtype=torch.int64)), (40, 3, torch.zeros(2 * need, dtype=torch.int32)[::2]),
+                        (-1, 3, torch.zeros(need, dtype=torch.int32)), (40, 0, torch.zeros(need, dtype=torch.int32))):
+        with pytest.raises(ops.MfError):
+            ops.AdapterPlan(t, n, words)
