@@ -323,11 +323,14 @@ __global__ __launch_bounds__(kWaves * 64, 4) void adapter_shrink_kernel(const Ad
   __shared__ uint4 places[kWaves * S::kBytes / 16];  // a wave's place holds its part of the sums when it is done
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint4* place = places + wave * (S::kBytes / 16);
-  // parts side by side: with eight of them (or their multiples) every XCD has a window of x and A of its own
-  const uint32_t split = blockIdx.x % a.splits, group = blockIdx.y;
+  // Parts side by side: with eight of them (or their multiples) every XCD has a window of x and A of its own.  The groups of ranks that
+  // read the same part of x are on one XCD too, and run together.
+  // (3875 rows of 11392, rank 64, two targets: 54 -> 46 us)
   const uint32_t blocks = (a.rank + 15) / 16;  // of 16 ranks, a target
+  const uint32_t groups = (blocks * a.num_targets + CF - 1) / CF;
+  const uint32_t pair = blockIdx.x / 8 / groups * 8 + blockIdx.x % 8, group = blockIdx.x / 8 % groups, split = pair % a.splits;
   const uint32_t units = a.n / 64, u0 = units * split / a.splits, u1 = units * (split + 1) / a.splits;
-  Meeting<RT * 16> meeting(a, blockIdx.x / a.splits, lane);
+  Meeting<RT * 16> meeting(a, pair / a.splits, lane);  // (none behind the last pair)
   uint32_t adapter, lanes, lead;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
@@ -649,11 +652,13 @@ uint32_t shrink_splits(uint32_t t, uint32_t n) {
   return std::max(1u, std::min({kShrinkGroups / ((t + 15) / 16), n / 64 / kWaves, t > 256 ? 4u : kMostSplits}));
 }
 
-// deals the results of all targets to workgroups: about `groups` of them for a tile's rows
-void deal_results(AdapterArgs& a, uint32_t groups, uint32_t waves) {
-  uint32_t blocks = 0;
+// deals the results of all targets to workgroups, `least` blocks of 64 or more each, and so many that there are no more than `most`
+// workgroups; but fewer where less than `fill` would be left
+void deal_results(AdapterArgs& a, uint32_t tiles, uint32_t least, uint32_t fill, uint32_t most, uint32_t waves) {
+  uint64_t blocks = 0;
   for (uint32_t k = 0; k < a.num_targets; ++k) blocks += (a.target[k].m + 63) / 64;
-  a.run_blocks = std::max(1u, (blocks + groups - 1) / groups);
+  blocks *= tiles;
+  a.run_blocks = static_cast<uint32_t>(std::max<uint64_t>((blocks + most - 1) / most, std::min<uint64_t>(least, (blocks + fill - 1) / fill)));
   a.run_blocks = (a.run_blocks + waves - 1) / waves * waves;
   a.first_run[0] = 0;
   for (uint32_t k = 0; k < MF_MAX_ADAPTER_TARGETS; ++k)
@@ -665,7 +670,7 @@ hipError_t launch_shrink(hipStream_t s, const AdapterArgs& a, uint32_t tiles, ui
   const uint32_t blocks = (a.rank + 15) / 16 * a.num_targets;
   const auto go = [&](auto cf) {
     constexpr int kCols = decltype(cf)::value;
-    adapter_shrink_kernel<RT, kCols><<<dim3(tiles * a.splits, (blocks + kCols - 1) / kCols, turns), dim3(kWaves * 64), 0, s>>>(a);
+    adapter_shrink_kernel<RT, kCols><<<dim3((tiles * a.splits + 7) / 8 * 8 * ((blocks + kCols - 1) / kCols), 1, turns), dim3(kWaves * 64), 0, s>>>(a);
   };
   if (blocks == 1) go(std::integral_constant<int, 1>{});
   else go(std::integral_constant<int, 2>{});
@@ -674,7 +679,10 @@ hipError_t launch_shrink(hipStream_t s, const AdapterArgs& a, uint32_t tiles, ui
 
 template <int RT, bool F32>
 hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t turns) {
-  deal_results(a, std::max(1u, 8192 / (tiles * turns)), kExpandWaves);
+  // Four blocks a wave pay for its start, if a few workgroups a CU remain (us a pass with one block a wave / so): 3875 rows, rank 64, two
+  // times 4608, 63 / 52; 1402 rows, rank 32, two times 6251 in fp32, 47 / 38; 4096 rows, rank 16, two times 17408, 139 / 135 (six blocks: 144);
+  // 62 rows, rank 16, two times 8256, 12 / 9; there 2048 workgroups were no gain.
+  deal_results(a, tiles * turns, 16, RT == 1 ? 1024 : 2048, 8192, kExpandWaves);
   const size_t lds = static_cast<size_t>((a.rank + 31) / 32) * RT * (F32 ? 3 : 2) * 1024;
   const hipError_t e = allow_lds<adapter_expand_kernel<RT, F32>>(lds, 64 * 1024);
   if (e != hipSuccess) return e;
@@ -683,19 +691,24 @@ hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t
 }
 
 struct Tiling {
-  uint32_t tiles, turns;
+  uint32_t tiles, turns, shrink_turns;
   Tiling(const AdapterArgs& a, uint32_t rows) {
     const bool planned = a.plan.tiles != nullptr;
     tiles = std::max((a.t + rows - 1) / rows, planned ? a.plan.most_tiles * (a.plan.tile_rows / rows) : 0);
-    // consecutive rows of a short batch: the adapters of a tile side by side
-    turns = planned || tiles > 4 ? 1 : std::min({a.t, a.num_adapters, 16u});
+    // Consecutive rows of a short batch: the adapters of a tile side by side, for the first product only up to four tiles, since its
+    // workgroups are many and most would find none (us a pass, one / four at once: 80 rows of several requests, rank 16, 2048 to two times
+    // 2048, 13.4 / 7.0, of one request 6.8 / 6.9; the second product of rank 64, two times 4096, 15.4 / 9.4 and 7.9 / 8.1, the first 8.0 / 7.2 and
+    // 5.1 / 6.2.  1000 rows, two at once: 14.4 / 11.9 and 9.6 / 11.4, left at one)
+    shrink_turns = planned || tiles > 4 ? 1 : std::min({a.t, a.num_adapters, 16u});
+    turns = planned || tiles > 16 ? 1 : std::min({a.t, a.num_adapters, tiles > 4 ? 4u : 16u});
   }
 };
 
 template <bool F32>
 hipError_t launch_fused(hipStream_t s, AdapterArgs& a) {
   const Tiling g(a, 16);
-  deal_results(a, std::max(1u, 256 / (g.tiles * g.turns)), kWaves);
+  const uint32_t rows = g.tiles * g.turns, groups = std::max(1u, 256 / rows) * rows;  // one workgroup a CU, or one for all results of a tile
+  deal_results(a, rows, 1, groups, groups, kWaves);
   a.by_xcd = g.tiles >= 32;
   const dim3 grid(a.first_run[a.num_targets] * (a.by_xcd ? (g.tiles + 7) / 8 * 8 : g.tiles), 1, g.turns), block(kWaves * 64);
   if (a.rank <= 16) adapter_fused_kernel<1, F32><<<grid, block, 0, s>>>(a);
@@ -707,7 +720,7 @@ template <int RT, bool F32>
 hipError_t launch_two(hipStream_t s, AdapterArgs& a) {
   const Tiling g(a, RT * 16);
   a.splits = shrink_splits(a.t, a.n);
-  const hipError_t e = launch_shrink<RT>(s, a, g.tiles, g.turns);
+  const hipError_t e = launch_shrink<RT>(s, a, g.tiles, g.shrink_turns);
   return e != hipSuccess ? e : launch_expand<RT, F32>(s, a, g.tiles, g.turns);
 }
 
