@@ -646,10 +646,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const Ada
 }
 
 // Parts of the sum over n: for two workgroups a CU, of eight units of 64 elements (one a wave) or more; few of them where there are
-// many rows, since every part of v is written and read again (777 rows, rank 64, two projections: four parts 13.0 + 12.6 us, eight 13.0 + 15.0).
+// many rows, since every part of v is written and read again (777 rows of 4096, rank 64, two targets: four parts 11.6 + 13.4 us, five 12.7 +
+// 14.5, eight 13.0 + 15.0), unless a workgroup has all ranks (2000 rows of 16384, rank 16, two times 1024: four 26.4 + 11.4 us, eight 18.7 + 13.0).
 constexpr uint32_t kMostSplits = 16, kShrinkGroups = 512;
-uint32_t shrink_splits(uint32_t t, uint32_t n) {
-  return std::max(1u, std::min({kShrinkGroups / ((t + 15) / 16), n / 64 / kWaves, t > 256 ? 4u : kMostSplits}));
+uint32_t shrink_splits(uint32_t t, uint32_t n, uint32_t blocks) {
+  const bool all = t > 256 && blocks <= 2;
+  return std::max(1u, std::min({kShrinkGroups * (all ? 2 : 1) / ((t + 15) / 16), n / 64 / kWaves, t <= 256 ? kMostSplits : all ? 8u : 4u}));
 }
 
 // deals the results of all targets to workgroups, `least` blocks of 64 or more each, and so many that there are no more than `most`
@@ -719,7 +721,7 @@ hipError_t launch_fused(hipStream_t s, AdapterArgs& a) {
 template <int RT, bool F32>
 hipError_t launch_two(hipStream_t s, AdapterArgs& a) {
   const Tiling g(a, RT * 16);
-  a.splits = shrink_splits(a.t, a.n);
+  a.splits = shrink_splits(a.t, a.n, (a.rank + 15) / 16 * a.num_targets);
   const hipError_t e = launch_shrink<RT>(s, a, g.tiles, g.shrink_turns);
   return e != hipSuccess ? e : launch_expand<RT, F32>(s, a, g.tiles, g.turns);
 }
@@ -747,7 +749,7 @@ hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, u
 
 size_t adapter_workspace_bytes(uint32_t num_targets, uint32_t rank, uint32_t n, uint32_t t) {
   // rows times parts, and no less than for any smaller t: the parts fall as one over the tiles of 16 rows
-  const uint64_t most = std::max<uint64_t>(t, std::min<uint64_t>(kShrinkGroups * 16, static_cast<uint64_t>(t) * shrink_splits(1, n)));
+  const uint64_t most = std::max<uint64_t>(t, std::min<uint64_t>(kShrinkGroups * 2 * 16, static_cast<uint64_t>(t) * shrink_splits(1, n, 1)));
   return most * num_targets * rank * sizeof(float);
 }
 
