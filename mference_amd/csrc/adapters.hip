@@ -685,9 +685,9 @@ hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t
   // times 4608, 63 / 52; 1402 rows, rank 32, two times 6251 in fp32, 47 / 38; 4096 rows, rank 16, two times 17408, 139 / 135 (six blocks: 144);
   // 62 rows, rank 16, two times 8256, 12 / 9; there 2048 workgroups were no gain.
   deal_results(a, tiles * turns, 16, RT == 1 ? 1024 : 2048, 8192, kExpandWaves);
-  const size_t lds = static_cast<size_t>((a.rank + 31) / 32) * RT * (F32 ? 3 : 2) * 1024;
-  const hipError_t e = allow_lds<adapter_expand_kernel<RT, F32>>(lds, 64 * 1024);
-  if (e != hipSuccess) return e;
+  constexpr uint32_t kBlock = RT * (F32 ? 3 : 2) * 1024;  // of 32 ranks
+  static_assert(MF_MAX_ADAPTER_RANK / 32 * kBlock <= 48 * 1024, "what a launch may ask for without further ado");
+  const uint32_t lds = (a.rank + 31) / 32 * kBlock;
   adapter_expand_kernel<RT, F32><<<dim3(a.first_run[a.num_targets], tiles, turns), dim3(kExpandWaves * 64), lds, s>>>(a);
   return hipGetLastError();
 }

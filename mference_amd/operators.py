@@ -241,6 +241,11 @@ def _on(context: MetalContext, stream) -> int:
     return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
 
 
+def _used_on(context: MetalContext, t: torch.Tensor, stream) -> None:
+    """tells torch's allocator that a tensor of the current stream is used on the one that a call was given"""
+    t.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), context.device))
+
+
 def _address(t: torch.Tensor, what: str, dtype, device: int) -> int:
     """the address of a tensor that lies on the context's device and has the type asked for"""
     if t.dtype is not dtype or t.get_device() != device:
@@ -302,10 +307,12 @@ class AdapterGrouping:
         """adapter_of_row int32 [t]"""
         ctx = self.context
         ids = _address(adapter_of_row, "adapter_of_row", torch.int32, ctx.device.index)
-        t = adapter_of_row.shape[0]
+        t = adapter_of_row.numel()
         _vector(adapter_of_row, "adapter_of_row", t)
         if plan is None:
             plan = self.plan(t)
+            if stream is not None:
+                _used_on(ctx, plan.words, stream)
         elif plan.t != t or plan.num_adapters != self.num_adapters:
             raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
         words = plan.words
@@ -337,6 +344,7 @@ class LowRankAdapters:
             if not (wa.is_contiguous() and wb.is_contiguous()):
                 raise MfError(-1, "the adapter pool must be contiguous")
             self._fixed.append((_address(wa, "a", torch.bfloat16, device), _address(wb, "b", torch.bfloat16, device), wb.shape[1]))
+        self.ms = [wb.shape[1] for wb in b]
         self._pack = Struct("@" + "PPPII" * len(a)).pack  # mf_adapter_target [len(a)]
         self.pool = _capi.AdapterPool(self.num_adapters, self.rank, self.n, None, None)
         for name, v, dtype in (("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
@@ -361,7 +369,7 @@ class LowRankAdapters:
             ys = (ys,)
         if len(ys) != len(self._fixed):
             raise MfError(-2, f"{len(ys)} results for {len(self._fixed)} projections")
-        t = x.shape[0]
+        t = adapter_of_row.numel()
         ids = _address(adapter_of_row, "adapter_of_row", torch.int32, device)
         _vector(adapter_of_row, "adapter_of_row", t)
         x_ptr = _address(x, "x", torch.bfloat16, device)
@@ -382,7 +390,7 @@ class LowRankAdapters:
         if workspace is None:
             workspace = torch.empty(self.workspace_bytes(t), dtype=torch.uint8, device=ctx.device)
             if stream is not None:
-                workspace.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), ctx.device))
+                _used_on(ctx, workspace, stream)
         elif not workspace.is_contiguous():
             raise MfError(-1, "the workspace must be contiguous")
         elif workspace.get_device() != device:
@@ -426,7 +434,7 @@ class BlockNorm:
         if gate is not None:
             g_ptr = _address(gate, "gate", bf16, device)
             if gate_kind == GATE_ROW:
-                if gate.numel() != t or gate.dim() > 2 or gate.shape[0] != t:
+                if gate.numel() != t or gate.dim() not in (1, 2) or gate.shape[0] != t:
                     raise MfError(-2, f"the gate must be one logit for each of {t} rows")
                 g_stride = gate.stride(0) if t > 1 else 1
                 if g_stride == 0 and t > 1:  # 0 means "not given" to the library
@@ -460,7 +468,6 @@ class SharedExpertInt4:
             gate.n, gate.rows, t, _ptr(y), _ptr(scratch_act),
             scratch_act.numel() * scratch_act.element_size()), self.context.handle)
 
-
     def encode_adapted(self, x: torch.Tensor, gate: QuantizedTensor, up: QuantizedTensor, down: QuantizedTensor,
                        y: torch.Tensor, gate_up_adapters: LowRankAdapters, down_adapters: LowRankAdapters,
                        adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> None:
@@ -472,6 +479,11 @@ class SharedExpertInt4:
         t, d, f = x.shape[0], gate.n, gate.rows
         if not (x.is_contiguous() and y.is_contiguous()) or x.shape != (t, d) or y.shape != (t, d):
             raise MfError(-2, f"x {tuple(x.shape)} and y {tuple(y.shape)} must be contiguous rows of {d}")
+        for adapters, n, ms in ((gate_up_adapters, d, [f, f]), (down_adapters, f, [d])):  # in front of the first launch
+            if adapters.n != n or adapters.ms != ms:
+                raise MfError(-2, f"adapters of {adapters.n} to {adapters.ms} beside projections of {n} to {ms}")
+        device = self.context.device.index
+        _address(x, "x", torch.bfloat16, device), _address(y, "y", torch.bfloat16, device)
         if t == 0:
             return
         if t * f >= 1 << 31:

@@ -461,3 +461,66 @@ def test_block_with_adapters(gpu, t, d, f):
     side.synchronize()
     off = float((again.double() - ys.double()).norm() / ys.double().norm())
     assert off < 0.01, off
+
+
+def test_mlp_refuses_other_adapters(gpu):
+    """adapters of other sizes, too few of them, results of another type: refused in front of the first launch, y as it was"""
+    g = gen(5)
+    rn = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    q = ops.Quantization(gpu)
+    t, d, f, n, r = 12, 256, 384, 3, 8
+    gate, up, down = (q.quantize_affine(rn(m, k) * k ** -0.5, 4) for m, k in ((f, d), (f, d), (d, f)))
+    pool = lambda n_in, *ms: ops.LowRankAdapters(gpu, [rn(n, r, n_in).bfloat16() for _ in ms], [rn(n, m, r).bfloat16() for m in ms])  # noqa: E731
+    x, y, ids = rn(t, d).bfloat16(), rn(t, d).bfloat16(), make_ids("mixed", t, n, 0.0, seed=1)
+    before, mlp = y.clone(), ops.SharedExpertInt4(gpu)
+    right = (pool(d, f, f), pool(f, d))
+    for gu, dn in ((pool(d, f), right[1]), (pool(f, f, f), right[1]), (right[0], pool(d, d)), (right[0], pool(f, f)), (right[0], pool(f, d, d))):
+        with pytest.raises(ops.MfError):
+            mlp.encode_adapted(x, gate, up, down, y, gu, dn, ids)
+    for bad_x, bad_y in ((x.half(), y), (x, y.half()), (x[:, :-64], y), (x, y[:-1])):
+        with pytest.raises((ops.MfError, ValueError)):
+            mlp.encode_adapted(bad_x, gate, up, down, bad_y, *right, ids)
+    torch.cuda.synchronize()
+    assert torch.equal(y, before)
+
+
+def test_operators_refuse_numbers_in_place_of_vectors(gpu):
+    g = gen(6)
+    a, b = torch.zeros(2, 8, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(2, 16, 8, device="cuda", dtype=torch.bfloat16)
+    low, number = ops.LowRankAdapters(gpu, a, b), torch.zeros((), device="cuda", dtype=torch.int32)
+    x, y = (torch.randn(1, m, generator=g, device="cuda").bfloat16() for m in (64, 16))
+    with pytest.raises(ops.MfError):
+        low.encode(x, number, y)
+    with pytest.raises(ops.MfError):
+        low.encode(x[0], number.reshape(1), y)
+    with pytest.raises(ops.MfError):
+        ops.AdapterGrouping(gpu, 2).encode(number)
+    with pytest.raises(ops.MfError):
+        ops.BlockNorm(gpu).encode(x, x.clone(), gate=torch.zeros((), device="cuda", dtype=torch.bfloat16), gate_kind=ops.GATE_ROW)
+    with pytest.raises(ops.MfError):
+        ops.BlockNorm(gpu).encode(x[0], x[0].clone())
+
+
+def test_buffers_of_a_call_on_another_stream(gpu):
+    """a plan and a workspace that the calls take themselves, for a stream that is not the current one: their memory is not handed
+    out again while that stream may still use it"""
+    g = gen(7)
+    t, n, m, k, r = 300, 4096, 512, 4, 64
+    a, b = (torch.randn(s, generator=g, device="cuda").bfloat16() for s in ((k, r, n), (k, m, r)))
+    low, grouping = ops.LowRankAdapters(gpu, a, b), ops.AdapterGrouping(gpu, k)
+    x, ids = torch.randn(t, n, generator=g, device="cuda").bfloat16(), make_ids("mixed", t, k, 0.1, seed=2)
+    want = torch.zeros(t, m, device="cuda")
+    low.encode(x, ids, want, plan=grouping.encode(ids))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(8):
+        y = torch.zeros(t, m, device="cuda")
+        side.wait_stream(torch.cuda.current_stream())
+        plan = grouping.encode(ids, stream=side)
+        words = plan.words.numel()
+        low.encode(x, ids, y, plan=plan, stream=side)
+        del plan
+        torch.full((words,), -1, dtype=torch.int32, device="cuda")
+        torch.full((low.workspace_bytes(t),), 255, dtype=torch.uint8, device="cuda")
+        side.synchronize()
+        assert torch.equal(y, want)
