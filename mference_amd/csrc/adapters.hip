@@ -684,7 +684,7 @@ hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t
   // Four blocks a wave pay for its start, if a few workgroups a CU remain (us a pass with one block a wave / so): 3875 rows, rank 64, two
   // times 4608, 63 / 52; 1402 rows, rank 32, two times 6251 in fp32, 47 / 38; 4096 rows, rank 16, two times 17408, 139 / 135 (six blocks: 144);
   // 62 rows, rank 16, two times 8256, 12 / 9; there 2048 workgroups were no gain.
-  deal_results(a, tiles * turns, 16, RT == 1 ? 1024 : 2048, 8192, kExpandWaves);
+  deal_results(a, tiles > 16 ? tiles : tiles * turns, 16, RT == 1 ? 1024 : 2048, 8192, kExpandWaves);
   constexpr uint32_t kBlock = RT * (F32 ? 3 : 2) * 1024;  // of 32 ranks
   static_assert(MF_MAX_ADAPTER_RANK / 32 * kBlock <= 48 * 1024, "what a launch may ask for without further ado");
   const uint32_t lds = (a.rank + 31) / 32 * kBlock;
@@ -693,16 +693,19 @@ hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t
 }
 
 struct Tiling {
-  uint32_t tiles, turns, shrink_turns;
+  uint32_t tiles, turns, shrink_turns, expand_turns;
   Tiling(const AdapterArgs& a, uint32_t rows) {
     const bool planned = a.plan.tiles != nullptr;
     tiles = std::max((a.t + rows - 1) / rows, planned ? a.plan.most_tiles * (a.plan.tile_rows / rows) : 0);
-    // Consecutive rows of a short batch: the adapters of a tile side by side, for the first product only up to four tiles, since its
-    // workgroups are many and most would find none (us a pass, one / four at once: 80 rows of several requests, rank 16, 2048 to two times
-    // 2048, 13.4 / 7.0, of one request 6.8 / 6.9; the second product of rank 64, two times 4096, 15.4 / 9.4 and 7.9 / 8.1, the first 8.0 / 7.2 and
-    // 5.1 / 6.2.  1000 rows, two at once: 14.4 / 11.9 and 9.6 / 11.4, left at one)
-    shrink_turns = planned || tiles > 4 ? 1 : std::min({a.t, a.num_adapters, 16u});
-    turns = planned || tiles > 16 ? 1 : std::min({a.t, a.num_adapters, tiles > 4 ? 4u : 16u});
+    // Consecutive rows of a short batch: the adapters of a tile side by side.  Us a pass, all of one tile's after one another / side by
+    // side: 80 rows of several requests, one launch of rank 16, 2048 to two times 2048, 13.4 / 7.0, of one request 6.8 / 6.9, but 1000 rows
+    // of one request 9.6 / 11.4; the second of two launches of rank 64, two times 4096, 80 rows 15.4 / 9.4 (one request 7.9 / 8.1), 777 rows, two
+    // times 2048, 13.5 / 11.0 (9.5 / 9.8), 2000 rows 32.4 / 34.1; the first, whose workgroups are many, 1000 rows of 8192, 12.7 / 11.1, 200 rows
+    // of 5120 10.2 / 13.4, 1402 rows 12.0 / 13.6.
+    const auto at_once = [&](uint32_t most) { return planned ? 1 : std::min({a.t, a.num_adapters, most}); };
+    turns = at_once(tiles <= 4 ? 16 : tiles <= 16 ? 4 : 1);
+    shrink_turns = at_once(tiles <= 4 ? 16 : tiles > 16 && tiles <= 32 ? 2 : 1);
+    expand_turns = at_once(tiles <= 4 ? 16 : tiles <= 16 ? 4 : tiles <= 48 ? 2 : 1);
   }
 };
 
@@ -723,7 +726,7 @@ hipError_t launch_two(hipStream_t s, AdapterArgs& a) {
   const Tiling g(a, RT * 16);
   a.splits = shrink_splits(a.t, a.n, (a.rank + 15) / 16 * a.num_targets);
   const hipError_t e = launch_shrink<RT>(s, a, g.tiles, g.shrink_turns);
-  return e != hipSuccess ? e : launch_expand<RT, F32>(s, a, g.tiles, g.turns);
+  return e != hipSuccess ? e : launch_expand<RT, F32>(s, a, g.tiles, g.expand_turns);
 }
 
 }  // namespace
