@@ -134,6 +134,59 @@ class RMSNorm {
   mf_ctx* ctx_;
 };
 
+// The three classes below have no counterpart in the reference: low-rank adapters of many requests beside shared projections, and
+// everything between two blocks of a layer in one launch.
+
+// Rows of a batch by adapter, on the device, once for all projections of a step.
+class AdapterGrouping {
+ public:
+  AdapterGrouping(const MetalContext& context, uint32_t numAdapters) : ctx_(context.raw()), n_(numAdapters) {}
+  size_t planBytes(uint32_t t) const { return mf_adapter_plan_bytes(t, n_); }
+  void encode(mf_stream cb, const int32_t* adapterOfRow, uint32_t t, uint32_t* plan, size_t planBytes) const {
+    check(mf_adapter_group(ctx_, cb, adapterOfRow, t, n_, plan, planBytes), ctx_);
+  }
+
+ private:
+  mf_ctx* ctx_;
+  uint32_t n_;
+};
+
+// Adds the rows' corrections to the results of DequantInt4GEMV, MPPPrefillInt4QMM or SharedExpertInt4 (targets: one to four
+// projections that read the same x).  plan: AdapterGrouping's of the same rows, or null.
+class LowRankAdapters {
+ public:
+  LowRankAdapters(const MetalContext& context, const mf_adapter_pool& pool) : ctx_(context.raw()), pool_(pool) {}
+  size_t workspaceBytes(uint32_t numTargets, uint32_t t) const { return mf_adapter_workspace_bytes(&pool_, numTargets, t); }
+  void encode(mf_stream cb, const mf_adapter_target* targets, uint32_t numTargets, const uint16_t* x, uint32_t xStride,
+              const int32_t* adapterOfRow, uint32_t t, bool float32, const uint32_t* plan, void* workspace,
+              size_t workspaceBytes) const {
+    check(mf_adapter_apply(ctx_, cb, &pool_, targets, numTargets, x, xStride, adapterOfRow, t, float32 ? 1 : 0, plan, workspace,
+                           workspaceBytes), ctx_);
+  }
+
+ private:
+  mf_ctx* ctx_;
+  mf_adapter_pool pool_;
+};
+
+// The norm behind a block, its gate and scale, the residual add and the norm in front of the next block.
+class BlockNorm {
+ public:
+  explicit BlockNorm(const MetalContext& context) : ctx_(context.raw()) {}
+  // arguments that change nothing: no gate, scales of one, rows one behind the other
+  static mf_block_norm_args arguments(uint16_t* hidden, const void* delta, uint32_t t, uint32_t d, float eps) {
+    mf_block_norm_args a{};
+    a.hidden = hidden, a.delta = delta, a.t = t, a.d = d;
+    a.post_eps = a.pre_eps = eps;
+    a.residual_scale = a.branch_scale = 1.0f;
+    return a;
+  }
+  void encode(mf_stream cb, const mf_block_norm_args& args) const { check(mf_block_norm(ctx_, cb, &args), ctx_); }
+
+ private:
+  mf_ctx* ctx_;
+};
+
 // The router calls of MoEDeepseekV4 (Kernels/MoE/MoEDeepseekV4.swift:92-151): learned top-k on
 // sqrt(softplus(logit)) + correction bias, and weighting of hash-routed experts.  routeScale is the
 // operator's constant as in the reference (:31-87); `logits` fp32 [tokens, numExperts] stands in for
