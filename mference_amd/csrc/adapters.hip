@@ -67,7 +67,10 @@ __device__ __forceinline__ uint2 block_exclusive(uint2 v, uint2* part) {
 
 // One workgroup for a run of rows.  COUNT: it leaves how many rows of every key the run has, and that is all.  Otherwise it adds up
 // those counts of all runs (a thread a key), knows from them where every key's rows start and where its own go, and writes its rows;
-// the lists of adapters and tiles are dealt out over the workgroups.  A batch of one run needs no counting launch in front.
+// the lists of adapters and tiles are dealt out over the workgroups.  A batch of one run needs no counting launch in front: up to 4096
+// rows, where one workgroup's turns still cost less than a second launch.  Four bytes a row are read and written: what it takes is latency (ids,
+// ballots, two scans, scattered stores): 200 rows 2.7 us, 16384 rows 3.7 + 6.7 us.  Calls of the simple form (a thread an adapter that
+// reads all rows) took 27 and 1829 us.
 template <int IT, bool COUNT>
 __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __restrict__ ids, uint32_t t, uint32_t n, AdapterPlan plan) {
   __shared__ uint16_t counts[16 * (MF_MAX_ADAPTERS + 1)];  // [wave][key]; then where a wave's rows of a key start among the run's
@@ -316,7 +319,11 @@ __device__ __forceinline__ f32x4_t add_parts(const f32x4_t* part, uint32_t apart
 // units requested at once: what 128 registers a lane hold
 template <int RT, int CF> constexpr int kUnitsAhead = 6 - RT - CF;
 
-// The first of two launches: v to memory, in parts over n.
+// The first of two launches: v to memory, in parts over n.  It reads x once for every RT * 16 rows and two blocks of ranks, and those
+// rows of A; matrix instructions are a few percent of its time.  Bound by the loads' latency: a wave has two to four
+// units in flight and often no more than three turns.  777 rows of 4096, rank 64, two targets: 11.1 us, 14.5 MB from memory; 4096 rows of
+// 5120, rank 16, two targets: 18.9 us, 45.6 MB = 2.4 TB/s; eight rows of 17408, rank 16: 5.6 us.
+// The simple form of both launches (a dot product a wave, a result a thread) took 932 and 4263 us for the two prompts.
 template <int RT, int CF>
 __global__ __launch_bounds__(kWaves * 64, 4) void adapter_shrink_kernel(const AdapterArgs a) {
   using S = Stage<RT, CF>;
@@ -543,7 +550,12 @@ struct Share {
   }
 };
 
-// The second of two launches.  A workgroup takes RT * 16 rows and a run of a target's results, and adds up the parts of v itself.
+// The second of two launches.  A workgroup takes RT * 16 rows and a run of a target's results, and adds up the parts of v itself: a
+// third launch that did would cost more.  Long batches are bound by y, which is read and written once: 4096 rows, rank 16, two times 17408,
+// 137 us, 345 MB read and 285 written = 4.6 TB/s, where a copy reaches 4.8.  Short ones are bound by a chain of requests (rows and
+// adapters 1.1 us, parts of v 2.9, products and y 1.8): 777 rows, rank 64, two times 2048, 10.9 us; eight rows, 5120 in fp32, 6.5 us.  Tried: eight
+// waves (no gain), y past the caches (no gain), whole lines of y in 8-byte pieces (199 us where it took 146), B of the next 32 ranks requested a
+// turn ahead (43 registers more; at rank 64 52 -> 55 us, 36 -> 40).
 constexpr uint32_t kExpandWaves = 4;
 
 template <int RT, bool F32>
@@ -596,7 +608,10 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
 //
 // Every workgroup makes the v of its rows and its target for itself, over the whole of n, and goes on to its results: nothing goes
 // through memory in between, and there is no second launch.  Workgroups that share rows make the same v, on compute units that
-// would have nothing else to do.
+// would have nothing else to do.  One row of 2048, rank 16, two times 512: 5.6 us (ids 0.8, addresses 0.7, the loop over n 1.3, the
+// waves' sums 1.0, results 0.8; the rest starts and ends the launch).  Four rows of 5120, rank 32, two times 17408: 10.4 us, of which 4.2 are
+// the loop, which draws 410 KB of x and A through a CU's L1, 40 bytes a clock of 64.  200 mixed rows of 2816, rank 24, two
+// times 2112: 11.5 us, 25 MB from memory.  Sixteen waves, and more units in flight, were no gain.
 template <int CF, bool F32>
 __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const AdapterArgs a) {
   constexpr int kTerms = F32 ? 3 : 2;
@@ -761,9 +776,10 @@ hipError_t launch_adapter_apply(hipStream_t s, AdapterArgs a, bool y_f32) {
   for (uint32_t k = 0; k < a.num_targets; ++k) results += a.target[k].m;
   results *= a.t;
   // One launch where v costs a workgroup little (two blocks of ranks, half a megabyte of x and A) and the results are not so many that
-  // their streaming decides: us a pass in one launch / in two, two projections -- one row of 2048, rank 16, 8.1 / 11.3; rank 64 9.9 / 10.2
-  // (left to two); of 5120, rank 32, 10.0 / 10.3, rank 64 14.7 / 10.8; of 17408, rank 8, 16.4 / 11.0; eight rows of eight adapters, 5120,
-  // rank 16, 12.1 / 16.4; 2048 rows, 2048 to 2048, rank 32, 21.8 / 25.6; 4096 rows 33.8 / 36.6; 512 rows, 5120 to 17408 (18 million results), 39.9 / 35.3
+  // their streaming decides.  Us of one launch / of the two (which cost one more to start), two projections: one row of 2048, rank 16, 5.4 /
+  // 8.8; of 5120, rank 32, 9.8 / 9.7; of 17408, rank 8, 14.5 / 10.4; eight rows of eight adapters, 5120, rank 16, 9.6 / 11.2; 1000 rows of
+  // 17408, rank 16, 31.5 / 19.9; 2048 to 2048, rank 32, 2000 rows 21.7 / 26.6, 4000 rows 33.0 / 37.9; to 4096 (33 million results) 52.3 / 50.6;
+  // 512 rows, 5120 to 17408 (18 million), 33.0 / 30.4.
   if (a.rank <= 32 && static_cast<uint64_t>(a.rank + 16) * a.n * sizeof(uint16_t) <= (512u << 10) && results <= (16u << 20))
     return y_f32 ? launch_fused<true>(s, a) : launch_fused<false>(s, a);
   const bool wide = a.plan.tiles ? a.plan.tile_rows == 64 : a.t > 256;  // 32 rows a workgroup instead of 16

@@ -272,9 +272,18 @@ def _row_stride(t: torch.Tensor, what: str, shape) -> int:
     return stride
 
 
-def _vector(t: torch.Tensor, what: str, size: int) -> None:
-    if t.dim() != 1 or t.shape[0] != size or not t.is_contiguous():
-        raise MfError(-2, f"{what} must be a contiguous vector of {size}")
+def _rows(t: torch.Tensor, what: str, dtype, device: int, shape):
+    """the address and the row stride of a tensor of this type and shape [rows, width] on the context's device"""
+    if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():  # nothing more to ask: 0.3 us less a tensor
+        return t.data_ptr(), shape[1]
+    return _address(t, what, dtype, device), _row_stride(t, what, shape)
+
+
+def _vector(t: torch.Tensor, what: str, dtype, device: int, shape) -> int:
+    """the address of a contiguous vector of this type and shape [size] on the context's device"""
+    if t.shape != shape or not t.is_contiguous():
+        raise MfError(-2, f"{what} must be a contiguous vector of {shape[0]}")
+    return _address(t, what, dtype, device)
 
 
 class AdapterPlan:
@@ -306,9 +315,8 @@ class AdapterGrouping:
     def encode(self, adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> AdapterPlan:
         """adapter_of_row int32 [t]"""
         ctx = self.context
-        ids = _address(adapter_of_row, "adapter_of_row", torch.int32, ctx.device.index)
-        t = adapter_of_row.numel()
-        _vector(adapter_of_row, "adapter_of_row", t)
+        device, t = ctx.device.index, adapter_of_row.numel()
+        ids = _vector(adapter_of_row, "adapter_of_row", torch.int32, device, (t,))
         if plan is None:
             plan = self.plan(t)
             if stream is not None:
@@ -316,7 +324,7 @@ class AdapterGrouping:
         elif plan.t != t or plan.num_adapters != self.num_adapters:
             raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
         words = plan.words
-        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, _address(words, "the plan", torch.int32, ctx.device.index),
+        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, _address(words, "the plan", torch.int32, device),
                                            words.numel() * 4), ctx.handle)
         return plan
 
@@ -349,8 +357,7 @@ class LowRankAdapters:
         self.pool = _capi.AdapterPool(self.num_adapters, self.rank, self.n, None, None)
         for name, v, dtype in (("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
             if v is not None:
-                _vector(v, name, self.num_adapters)
-                setattr(self.pool, name, _address(v, name, dtype, device))
+                setattr(self.pool, name, _vector(v, name, dtype, device, (self.num_adapters,)))
         if self.workspace_bytes(1) == 0:
             raise MfError(-2, f"num_adapters={self.num_adapters} rank={self.rank} n={self.n}")
 
@@ -370,16 +377,15 @@ class LowRankAdapters:
         if len(ys) != len(self._fixed):
             raise MfError(-2, f"{len(ys)} results for {len(self._fixed)} projections")
         t = adapter_of_row.numel()
-        ids = _address(adapter_of_row, "adapter_of_row", torch.int32, device)
-        _vector(adapter_of_row, "adapter_of_row", t)
-        x_ptr = _address(x, "x", torch.bfloat16, device)
-        x_stride = _row_stride(x, "x", (t, self.n))
+        ids = _vector(adapter_of_row, "adapter_of_row", torch.int32, device, (t,))
+        x_ptr, x_stride = _rows(x, "x", torch.bfloat16, device, (t, self.n))
         dtype = ys[0].dtype
         if dtype is not torch.bfloat16 and dtype is not torch.float32:
             raise ValueError(f"the results must be bfloat16 or float32, not {dtype}")
         targets = []
         for (a, b, m), y in zip(self._fixed, ys):
-            targets += (a, b, _address(y, "y", dtype, device), m, _row_stride(y, "y", (t, m)))
+            y_ptr, y_stride = _rows(y, "y", dtype, device, (t, m))
+            targets += (a, b, y_ptr, m, y_stride)
         words = None
         if plan is not None:
             if plan.t != t or plan.num_adapters != self.num_adapters:
@@ -418,19 +424,18 @@ class BlockNorm:
         if len(shape) != 2:
             raise MfError(-2, "hidden must be [t, d]")
         t, d = shape
-        h_ptr, h_stride = _address(hidden, "hidden", bf16, device), _row_stride(hidden, "hidden", shape)
+        channels = (d,)
+        h_ptr, h_stride = _rows(hidden, "hidden", bf16, device, shape)
         d_ptr = d_stride = f32 = o_ptr = o_stride = g_ptr = g_stride = pre = post = 0
         if delta is not None:
             f32 = 1 if delta.dtype is torch.float32 else 0
-            d_ptr, d_stride = _address(delta, "delta", torch.float32 if f32 else bf16, device), _row_stride(delta, "delta", shape)
+            d_ptr, d_stride = _rows(delta, "delta", torch.float32 if f32 else bf16, device, shape)
         if out is not None:
-            o_ptr, o_stride = _address(out, "out", bf16, device), _row_stride(out, "out", shape)
+            o_ptr, o_stride = _rows(out, "out", bf16, device, shape)
         if pre_weight is not None:
-            _vector(pre_weight, "pre_weight", d)
-            pre = _address(pre_weight, "pre_weight", bf16, device)
+            pre = _vector(pre_weight, "pre_weight", bf16, device, channels)
         if post_weight is not None:
-            _vector(post_weight, "post_weight", d)
-            post = _address(post_weight, "post_weight", bf16, device)
+            post = _vector(post_weight, "post_weight", bf16, device, channels)
         if gate is not None:
             g_ptr = _address(gate, "gate", bf16, device)
             if gate_kind == GATE_ROW:
@@ -442,7 +447,7 @@ class BlockNorm:
             elif gate_kind == GATE_ELEMENT:
                 g_stride = _row_stride(gate, "gate", shape)
             else:
-                _vector(gate, "gate", d)
+                _vector(gate, "gate", bf16, device, channels)
         args = self._pack(h_ptr, d_ptr, g_ptr, post, pre, o_ptr, d, t, h_stride, d_stride, g_stride, o_stride, f32, gate_kind,
                           eps if post_eps is None else post_eps, eps, residual_scale, branch_scale, weight_bias)
         check(_capi.lib().mf_block_norm(ctx.handle, _on(ctx, stream), args), ctx.handle)
