@@ -71,6 +71,8 @@ __device__ __forceinline__ uint2 block_exclusive(uint2 v, uint2* part) {
 // rows, where one workgroup's turns still cost less than a second launch.  Four bytes a row are read and written: what it takes is latency (ids,
 // ballots, two scans, scattered stores): 200 rows 2.7 us, 16384 rows 3.7 + 6.7 us.  Calls of the simple form (a thread an adapter that
 // reads all rows) took 27 and 1829 us.
+constexpr uint32_t kOwnTiles = 4;
+
 template <int IT, bool COUNT>
 __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __restrict__ ids, uint32_t t, uint32_t n, AdapterPlan plan) {
   __shared__ uint16_t counts[16 * (MF_MAX_ADAPTERS + 1)];  // [wave][key]; then where a wave's rows of a key start among the run's
@@ -119,9 +121,14 @@ __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __re
       starts[k] = at.x + before;
       if (k % gridDim.x == blockIdx.x) {
         plan.offsets[k] = at.x;
-        for (uint32_t i = 0; i < total.y; ++i)
-          plan.tiles[at.y + i] = make_uint2(k | min(total.x - i * plan.tile_rows, plan.tile_rows) << 16, at.x + i * plan.tile_rows);
+        for (uint32_t i = 0; i < min(total.y, kOwnTiles); ++i) plan.tiles[at.y + i] = plan.tile(k, at.x, total.x, i);
       }
+    }
+    // an adapter with many rows: its wave deals out its tiles (16384 rows of one adapter 13.9 -> 6.2 us)
+    for (uint64_t many = __ballot(k < n && k % gridDim.x == blockIdx.x && total.y > kOwnTiles); many; many &= many - 1) {
+      const int of = __builtin_ctzll(many);
+      const uint32_t key = __shfl(k, of), x = __shfl(at.x, of), y = __shfl(at.y, of), rows = __shfl(total.x, of), tiles = __shfl(total.y, of);
+      for (uint32_t i = kOwnTiles + (threadIdx.x & 63); i < tiles; i += 64) plan.tiles[y + i] = plan.tile(key, x, rows, i);
     }
     if (k == n - 1) {  // behind all adapters: the rows without one.  What of them lies in the runs in front is what the adapters leave.
       const uint32_t with = at.x + total.x;
@@ -761,6 +768,7 @@ hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, u
   };
   if (it == 1) go(std::integral_constant<int, 1>{});
   else if (it == 4) go(std::integral_constant<int, 4>{});
+  else if (it == 8) go(std::integral_constant<int, 8>{});
   else go(std::integral_constant<int, 16>{});
   return hipGetLastError();
 }

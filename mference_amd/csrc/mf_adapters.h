@@ -16,6 +16,10 @@ struct AdapterPlan {
   uint32_t* runs;     // [runs][n + 1]: rows of every key in each run, where there are several
   uint32_t tile_rows, most_tiles;
 
+  // tile i of an adapter whose rows start at `at` in the list
+  __device__ uint2 tile(uint32_t adapter, uint32_t at, uint32_t count, uint32_t i) const {
+    return make_uint2(adapter | min(count - i * tile_rows, tile_rows) << 16, at + i * tile_rows);
+  }
   // rows a tile: what a wave of the products holds at once.  Where a batch has few rows an adapter the wide tiles would be
   // mostly empty.
   static uint32_t rows_of_tile(uint32_t t, uint32_t n) { return t / 32 >= n ? 64 : 16; }

@@ -524,3 +524,11 @@ def test_buffers_of_a_call_on_another_stream(gpu):
         torch.full((low.workspace_bytes(t),), 255, dtype=torch.uint8, device="cuda")
         side.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("t", [700, 4096, 9000, 70001])
+@pytest.mark.parametrize("adapters", [1, 5, 700])
+@pytest.mark.parametrize("order", ["one", "runs"])
+def test_an_adapter_of_many_tiles(gpu, t, adapters, order):
+    """one adapter's rows fill more tiles of the plan than a lane writes by itself: every row once, by the plan and without it"""
+    Case(t, 64, (9,), adapters, 8, seed=t).check(gpu, make_ids(order, t, adapters, 0.05, seed=adapters), True)
