@@ -742,7 +742,7 @@ typedef struct {
  * MLP), the gate and the scales.  fp32 between the roundings named; as in mf_residual_rmsnorm the second norm is of the narrowed
  * stream.  The two calls add the squares of a row in different orders.  out may share no memory with hidden, delta or gate, hidden
  * none with delta or gate, neither with a weight (MF_ERR_INVALID_ARGUMENT).  The squares of a row are added in fp32: magnitudes
- * from about 2^63 on overflow to a norm of 0.  Any d >= 1; t = 0 does nothing; t <= MF_MAX_ROWS.  Faster where all
+ * from about 2^63 on overflow to a norm of 0.  Any d of 1 .. 2^28; t = 0 does nothing; t <= MF_MAX_ROWS.  Faster where all
  * tensors are 16-byte aligned and d and the strides are multiples of 8. */
 mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args* args);
 

@@ -1069,7 +1069,7 @@ mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool*
 mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args* args) {
   if (!ctx || !args) return MF_ERR_INVALID_ARGUMENT;
   mf_block_norm_args a = *args;
-  if (a.d == 0) return MF_ERR_DIMENSION_MISMATCH;
+  if (a.d == 0 || a.d > 1u << 28) return MF_ERR_DIMENSION_MISMATCH;  // (a thread's place in the row stays within 32 bits)
   if (a.t > MF_MAX_ROWS || a.gate_kind < MF_GATE_NONE || a.gate_kind > MF_GATE_CHANNEL) return MF_ERR_INVALID_ARGUMENT;
   if (a.t == 0) return MF_OK;
   // a gate or a norm behind the block needs the block's output; the norm in front of the next one needs a place for its result

@@ -181,6 +181,13 @@ def test_block_norm_refuses(ctx, over, status):
     assert norm(ctx, norm_args(**over)[0]) == status
 
 
+@pytest.mark.parametrize("d", [(1 << 28) + 1, (1 << 32) - 8, (1 << 32) - 1])
+def test_block_norm_refuses_rows_that_are_too_long(ctx, d):
+    a, _ = norm_args()
+    a.d = d
+    assert norm(ctx, a) == DIMENSION
+
+
 def test_block_norm_refuses_unaligned_and_shared(ctx):
     for name in ("hidden", "delta", "pre_weight", "out"):
         a, _ = norm_args()
