@@ -412,8 +412,10 @@ __device__ __forceinline__ uint4 keep_bf16(uint4 v, uint32_t n) {
 }
 
 // A workgroup's share of the results of one adapter's rows: its waves take 64 results in turn, the y and B of the next ones requested
-// before the present ones are worked on.
-template <int RT, bool F32, int WAVES>
+// before the present ones are worked on.  DEEP: B of the next 32 ranks in their place, and y no earlier than its results' first B; that is for
+// fp32 results of 32 rows, whose y takes most registers, and ranks past 32 (2000 rows, two times 4096, rank 48 43 -> 36 us, 64 45 -> 41, 128 62 -> 57;
+// bf16 results 55 -> 57, fp32 ones of 16 rows 11.2 -> 12.3, of rank 16 251 -> 290).
+template <int RT, bool F32, int WAVES, bool DEEP>
 struct Expand {
   static constexpr int kTerms = F32 ? 3 : 2, kPer = F32 ? 4 : 8, kChunks = 16 / kPer;  // results to 16 bytes; such pieces a lane holds of a row
   using Elem = std::conditional_t<F32, float, uint16_t>;
@@ -462,7 +464,7 @@ struct Expand {
       yp[r] = static_cast<Elem*>(tg.y) + static_cast<size_t>(__shfl(my_row, mine[r] ? at : lead)) * tg.y_stride;
     }
     if (block < end) {
-      load_y(block, yv);
+      if constexpr (!DEEP) load_y(block, yv);
       load_b(block, 0, bv);
     }
   }
@@ -470,8 +472,11 @@ struct Expand {
   __device__ __forceinline__ void run(uint32_t block, uint32_t end, uint32_t rank, const uint4* operand) {
     const uint32_t lane = threadIdx.x & 63, kb = (rank + 31) / 32;
     for (; block < end; block += WAVES) {
-      uint4 next_y[RT][kChunks], next_b[4];
-      if (block + WAVES < end) {
+      [[maybe_unused]] uint4 next_y[RT][kChunks];
+      uint4 next_b[4];
+      if constexpr (DEEP) {
+        load_y(block, yv);
+      } else if (block + WAVES < end) {
         load_y(block + WAVES, next_y);
         load_b(block + WAVES, 0, next_b);
       }
@@ -482,7 +487,12 @@ struct Expand {
         for (int j = 0; j < 4; ++j) acc[r][j] = f32x4_t{0, 0, 0, 0};
       for (uint32_t b = 0; b < kb; ++b) {
         const uint32_t k = b * 32 + q * 8, have = k < rank ? min(rank - k, 8u) : 0;
-        if (b) load_b(block, b * 32, bv);
+        if constexpr (DEEP) {
+          const bool more = b + 1 < kb;
+          if (more || block + WAVES < end) load_b(more ? block : block + WAVES, more ? b * 32 + 32 : 0, next_b);
+        } else {
+          if (b) load_b(block, b * 32, bv);
+        }
         if (rank % 32) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) bv[j] = have < 8 ? keep_bf16(bv[j], have) : bv[j];
@@ -495,6 +505,10 @@ struct Expand {
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[r][j] = mfma16(bv[j], term, acc[r][j]);
           }
+        if constexpr (DEEP) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bv[j] = next_b[j];
+        }
       }
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -523,12 +537,14 @@ struct Expand {
           }
         }
       }
+      if constexpr (!DEEP) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) yv[r][c] = next_y[r][c];
+          for (int c = 0; c < kChunks; ++c) yv[r][c] = next_y[r][c];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bv[j] = next_b[j];
+        for (int j = 0; j < 4; ++j) bv[j] = next_b[j];
+      }
     }
   }
 };
@@ -561,11 +577,12 @@ struct Share {
 // third launch that did would cost more.  Long batches are bound by y, which is read and written once: 4096 rows, rank 16, two times 17408,
 // 137 us, 345 MB read and 285 written = 4.6 TB/s, where a copy reaches 4.8.  Short ones are bound by a chain of requests (rows and
 // adapters 1.1 us, parts of v 2.9, products and y 1.8): 777 rows, rank 64, two times 2048, 10.9 us; eight rows, 5120 in fp32, 6.5 us.  Tried: eight
-// waves (no gain), y past the caches (no gain), whole lines of y in 8-byte pieces (199 us where it took 146), B of the next 32 ranks requested a
-// turn ahead (43 registers more; at rank 64 52 -> 55 us, 36 -> 40).
+// waves (no gain), y past the caches (no gain), whole lines of y in 8-byte pieces (199 us where it took 146), a wave's results one behind the
+// other (rows that start inside a line 108 -> 126 us).  Such rows cost: two times 13992 (16-byte places) 108 us where whole lines would take 85,
+// 13999 (2-byte places) 152.
 constexpr uint32_t kExpandWaves = 4;
 
-template <int RT, bool F32>
+template <int RT, bool F32, bool DEEP>
 __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const AdapterArgs a) {
   extern __shared__ uint4 operand[];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -575,7 +592,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
   uint32_t adapter, lanes, lead;
   for (uint32_t turn = 0; meeting.next(adapter, lanes, lead); ++turn) {
     if (turn % gridDim.z != blockIdx.z) continue;
-    Expand<RT, F32, kExpandWaves> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
+    Expand<RT, F32, kExpandWaves, DEEP> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
     const uint32_t rank = live_rank(a, adapter);
     __syncthreads();  // (the operands of the adapter before have been read)
     for (uint32_t slot = threadIdx.x; slot < (rank + 31) / 32 * RT * 64; slot += kExpandWaves * 64) {
@@ -604,7 +621,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = static_cast<uint32_t>(e) < have ? v[e] : 0.0f;
-      store_terms<RT, Expand<RT, F32, kExpandWaves>::kTerms>(operand, slot, v);
+      store_terms<RT, Expand<RT, F32, kExpandWaves, DEEP>::kTerms>(operand, slot, v);
     }
     __syncthreads();
     if (rank) expand.run(share.first + wave, share.end, rank, operand);
@@ -639,7 +656,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const Ada
     if (turn % gridDim.z != blockIdx.z) continue;
     S stage;
     stage.rows_of_x(a, meeting.row, lanes, lead);
-    Expand<1, F32, kWaves> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
+    Expand<1, F32, kWaves, false> expand(a, tg, adapter, meeting.row, lanes, lead, share.first + wave, share.end);
 #pragma unroll
     for (int c = 0; c < CF; ++c) stage.rows_of_a(c, tg.a + static_cast<size_t>(adapter) * a.rank * a.n, a.n, c * 16, a.rank);  // not waiting for its own rank
     if (turn) __syncthreads();  // (the parts of the adapter before have been read)
@@ -673,7 +690,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const Ada
 constexpr uint32_t kMostSplits = 16, kShrinkGroups = 512;
 uint32_t shrink_splits(uint32_t t, uint32_t n, uint32_t blocks) {
   const bool all = t > 256 && blocks <= 2;
-  return std::max(1u, std::min({kShrinkGroups * (all ? 2 : 1) / ((t + 15) / 16), n / 64 / kWaves, t <= 256 ? kMostSplits : all ? 8u : 4u}));
+  // two units a wave where there is a workgroup a CU without any parts (2578 rows of 1600, rank 128, two targets: three parts 26.5 us, one 18.8)
+  const uint32_t least = t > 256 && (t + 31) / 32 * ((blocks + 1) / 2) >= 256 ? 2 : 1;
+  return std::max(1u, std::min({kShrinkGroups * (all ? 2 : 1) / ((t + 15) / 16), n / 64 / (kWaves * least), t <= 256 ? kMostSplits : all ? 8u : 4u}));
 }
 
 // deals the results of all targets to workgroups, `least` blocks of 64 or more each, and so many that there are no more than `most`
@@ -710,7 +729,14 @@ hipError_t launch_expand(hipStream_t s, AdapterArgs& a, uint32_t tiles, uint32_t
   constexpr uint32_t kBlock = RT * (F32 ? 3 : 2) * 1024;  // of 32 ranks
   static_assert(MF_MAX_ADAPTER_RANK / 32 * kBlock <= 48 * 1024, "what a launch may ask for without further ado");
   const uint32_t lds = (a.rank + 31) / 32 * kBlock;
-  adapter_expand_kernel<RT, F32><<<dim3(a.first_run[a.num_targets], tiles, turns), dim3(kExpandWaves * 64), lds, s>>>(a);
+  const dim3 grid(a.first_run[a.num_targets], tiles, turns), block(kExpandWaves * 64);
+  if constexpr (RT == 2 && F32) {
+    if (a.rank > 32) {
+      adapter_expand_kernel<RT, F32, true><<<grid, block, lds, s>>>(a);
+      return hipGetLastError();
+    }
+  }
+  adapter_expand_kernel<RT, F32, false><<<grid, block, lds, s>>>(a);
   return hipGetLastError();
 }
 
