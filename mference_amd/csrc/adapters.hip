@@ -636,8 +636,13 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
 // waves' sums 1.0, results 0.8; the rest starts and ends the launch).  Four rows of 5120, rank 32, two times 17408: 10.4 us, of which 4.2 are
 // the loop, which draws 410 KB of x and A through a CU's L1, 40 bytes a clock of 64.  200 mixed rows of 2816, rank 24, two
 // times 2112: 11.5 us, 25 MB from memory.  Sixteen waves, and more units in flight, were no gain.
+//
+// Two workgroups a CU need 128 registers a lane: bf16 results and ranks up to 16 fit them with two units in flight instead of four (2169 rows,
+// rank 8, two times 809, 21.2 -> 17.5 us; 3000 rows, rank 16, 27.4 -> 22.8; one row 5.6 -> 5.5).  The others would spill: fp32 8.9 -> 10.8 us
+// on 700 rows, two blocks of ranks 11.9 -> 16.0 on 200.
+template <int CF, bool F32> constexpr bool kTwoACu = CF == 1 && !F32;
 template <int CF, bool F32>
-__global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const AdapterArgs a) {
+__global__ __launch_bounds__(kWaves * 64, (kTwoACu<CF, F32> ? 4 : 2)) void adapter_fused_kernel(const AdapterArgs a) {
   constexpr int kTerms = F32 ? 3 : 2;
   using S = Stage<1, CF>;
   __shared__ uint4 lds[kWaves * S::kBytes / 16 + kTerms * 64];
@@ -660,7 +665,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void adapter_fused_kernel(const Ada
 #pragma unroll
     for (int c = 0; c < CF; ++c) stage.rows_of_a(c, tg.a + static_cast<size_t>(adapter) * a.rank * a.n, a.n, c * 16, a.rank);  // not waiting for its own rank
     if (turn) __syncthreads();  // (the parts of the adapter before have been read)
-    stage.template multiply<kWaves, kUnitsAhead<1, CF>>(0, a.n / 64, place, reinterpret_cast<f32x4_t*>(place));
+    stage.template multiply<kWaves, (kTwoACu<CF, F32> ? 2 : kUnitsAhead<1, CF>)>(0, a.n / 64, place, reinterpret_cast<f32x4_t*>(place));
     const uint32_t rank = live_rank(a, adapter);
     const float scale = a.scales ? a.scales[adapter] : 1.0f;
     __syncthreads();
