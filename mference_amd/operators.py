@@ -297,6 +297,12 @@ class AdapterPlan:
         self.rows = words[:t]                               # int32 [t]: row numbers, stably sorted, rows without an adapter last
         self.offsets = words[t:t + num_adapters + 1]        # int32: where every adapter's rows start; then the rows without one
 
+    def _address_for(self, t: int, num_adapters: int, device: int) -> int:
+        """the address of its words, for a call of t rows and a pool of num_adapters on this device"""
+        if self.t != t or self.num_adapters != num_adapters:
+            raise MfError(-2, f"the plan is one of {self.t} rows and {self.num_adapters} adapters")
+        return _address(self.words, "the plan", torch.int32, device)
+
 
 class AdapterGrouping:
     """mf_adapter_group: the rows of a batch by adapter, on the device, once for all projections of a step (what
@@ -321,11 +327,8 @@ class AdapterGrouping:
             plan = self.plan(t)
             if stream is not None:
                 _used_on(ctx, plan.words, stream)
-        elif plan.t != t or plan.num_adapters != self.num_adapters:
-            raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
-        words = plan.words
-        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, _address(words, "the plan", torch.int32, device),
-                                           words.numel() * 4), ctx.handle)
+        words = plan._address_for(t, self.num_adapters, device)
+        check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, words, plan.words.numel() * 4), ctx.handle)
         return plan
 
 
@@ -386,11 +389,7 @@ class LowRankAdapters:
         for (a, b, m), y in zip(self._fixed, ys):
             y_ptr, y_stride = _rows(y, "y", dtype, device, (t, m))
             targets += (a, b, y_ptr, m, y_stride)
-        words = None
-        if plan is not None:
-            if plan.t != t or plan.num_adapters != self.num_adapters:
-                raise MfError(-2, f"the plan is one of {plan.t} rows and {plan.num_adapters} adapters")
-            words = _address(plan.words, "the plan", torch.int32, device)
+        words = None if plan is None else plan._address_for(t, self.num_adapters, device)
         if t == 0:
             return
         if workspace is None:
@@ -478,7 +477,8 @@ class SharedExpertInt4:
                        adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> None:
         """The MLP with an adapter beside each of its three projections (the same adapter of a row in all of them): the
         projections by themselves (mf_qmm), LowRankAdapters on their results, silu(gate) * up in between.  No counterpart in
-        the reference.  x bf16 [t, d], y bf16 [t, d]; buffers come from torch's allocator."""
+        the reference.  x bf16 [t, d], y bf16 [t, d]; both pools hold the same number of adapters; buffers come from torch's
+        allocator.  What does not fit together is refused in front of the first launch, y as it was."""
         if not (gate.rows == up.rows and gate.n == up.n and down.rows == gate.n and down.n == gate.rows):
             raise MfError(-2, f"gate=({gate.rows},{gate.n}) up=({up.rows},{up.n}) down=({down.rows},{down.n})")
         t, d, f = x.shape[0], gate.n, gate.rows
@@ -487,8 +487,15 @@ class SharedExpertInt4:
         for adapters, n, ms in ((gate_up_adapters, d, [f, f]), (down_adapters, f, [d])):  # in front of the first launch
             if adapters.n != n or adapters.ms != ms:
                 raise MfError(-2, f"adapters of {adapters.n} to {adapters.ms} beside projections of {n} to {ms}")
+            if adapters.context.device != self.context.device:
+                raise ValueError("the adapters lie on another device than the context")
+        if gate_up_adapters.num_adapters != down_adapters.num_adapters:  # a row's adapter is the same one in all three projections
+            raise MfError(-2, f"{gate_up_adapters.num_adapters} adapters for gate and up, {down_adapters.num_adapters} for down")
         device = self.context.device.index
         _address(x, "x", torch.bfloat16, device), _address(y, "y", torch.bfloat16, device)
+        _vector(adapter_of_row, "adapter_of_row", torch.int32, device, (t,))
+        if plan is not None:
+            plan._address_for(t, down_adapters.num_adapters, device)
         if t == 0:
             return
         if t * f >= 1 << 31:
@@ -500,13 +507,15 @@ class SharedExpertInt4:
             qmm, elementwise = MPPPrefillInt4QMM(self.context), Elementwise(self.context)
             need = max(qmm.workspace_bytes(t, f, d), qmm.workspace_bytes(t, d, f), 256)
             workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-            for w, out in ((gate, g), (up, u)):
-                if qmm.encode(w, x, out, t, f, d, workspace=workspace, stream=on) == "unavailable":
-                    raise MfError(-1, "a projection refused its operands")
+            lib, handle, ws, s = _capi.lib(), self.context.handle, workspace.data_ptr(), on.cuda_stream
+            projections = [(w.c(), w.bits, src.data_ptr(), out.data_ptr(), t, w.rows, w.n) for w, src, out in ((gate, x, g), (up, x, u), (down, act, y))]
+            if any(lib.mf_qmm_path(*p, ws, need) < 0 for p in projections):
+                raise MfError(-1, "a projection refuses its operands")
+            for p in projections[:2]:
+                check(lib.mf_qmm(handle, s, *p, 0, ws, need), handle)
             gate_up_adapters.encode(x, adapter_of_row, (g, u), plan=plan, stream=on)
             elementwise.encode_silu_mul(g, u, act, t * f, stream=on)
-            if qmm.encode(down, act, y, t, d, f, workspace=workspace, stream=on) == "unavailable":
-                raise MfError(-1, "a projection refused its operands")
+            check(lib.mf_qmm(handle, s, *projections[2], 0, ws, need), handle)
             down_adapters.encode(act, adapter_of_row, y, plan=plan, stream=on)
 
     @staticmethod
