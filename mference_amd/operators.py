@@ -241,9 +241,20 @@ def _on(context: MetalContext, stream) -> int:
     return stream.cuda_stream if isinstance(stream, torch.cuda.Stream) else int(stream)
 
 
-def _used_on(context: MetalContext, t: torch.Tensor, stream) -> None:
-    """tells torch's allocator that a tensor of the current stream is used on the one that a call was given"""
-    t.record_stream(stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(int(stream), context.device))
+def _stream_object(context: MetalContext, stream) -> torch.cuda.Stream:
+    if isinstance(stream, torch.cuda.Stream):
+        return stream
+    handle = int(stream)
+    return torch.cuda.ExternalStream(handle, context.device) if handle else torch.cuda.default_stream(context.device)
+
+
+def _taken_on(context: MetalContext, stream, take):
+    """take(), a buffer from torch's allocator, as memory of the stream that a call was given: a block that was freed on the current
+    stream may still be in use there"""
+    if stream is None or _on(context, stream) == _on(context, None):
+        return take()
+    with torch.cuda.stream(_stream_object(context, stream)):
+        return take()
 
 
 def _address(t: torch.Tensor, what: str, dtype, device: int) -> int:
@@ -324,9 +335,9 @@ class AdapterGrouping:
         device, t = ctx.device.index, adapter_of_row.numel()
         ids = _vector(adapter_of_row, "adapter_of_row", torch.int32, device, (t,))
         if plan is None:
-            plan = self.plan(t)
-            if stream is not None:
-                _used_on(ctx, plan.words, stream)
+            plan = _taken_on(ctx, stream, lambda: self.plan(t))
+            if stream is not None:  # the caller may go on with it on the current stream
+                plan.words.record_stream(torch.cuda.current_stream(ctx.device))
         words = plan._address_for(t, self.num_adapters, device)
         check(_capi.lib().mf_adapter_group(ctx.handle, _on(ctx, stream), ids, t, self.num_adapters, words, plan.words.numel() * 4), ctx.handle)
         return plan
@@ -393,9 +404,7 @@ class LowRankAdapters:
         if t == 0:
             return
         if workspace is None:
-            workspace = torch.empty(self.workspace_bytes(t), dtype=torch.uint8, device=ctx.device)
-            if stream is not None:
-                _used_on(ctx, workspace, stream)
+            workspace = _taken_on(ctx, stream, lambda: torch.empty(self.workspace_bytes(t), dtype=torch.uint8, device=ctx.device))
         elif not workspace.is_contiguous():
             raise MfError(-1, "the workspace must be contiguous")
         elif workspace.get_device() != device:
