@@ -242,6 +242,7 @@ def _on(context: MetalContext, stream) -> int:
 
 
 def _stream_object(context: MetalContext, stream) -> torch.cuda.Stream:
+    """torch's object for a stream that a call was given (an ExternalStream of handle 0 would be one of torch's own streams)"""
     if isinstance(stream, torch.cuda.Stream):
         return stream
     handle = int(stream)
@@ -509,8 +510,7 @@ class SharedExpertInt4:
             return
         if t * f >= 1 << 31:
             raise MfError(-1, f"t={t} rows of f={f} are more than one call takes")
-        on = stream if isinstance(stream, torch.cuda.Stream) else \
-            torch.cuda.current_stream(self.context.device) if stream is None else torch.cuda.ExternalStream(int(stream), self.context.device)
+        on = torch.cuda.current_stream(self.context.device) if stream is None else _stream_object(self.context, stream)
         with torch.cuda.stream(on):  # so that the allocator knows the stream of the buffers
             g, u, act = (torch.empty((t, f), dtype=torch.bfloat16, device=x.device) for _ in range(3))
             qmm, elementwise = MPPPrefillInt4QMM(self.context), Elementwise(self.context)

@@ -35,11 +35,11 @@ def call(monkeypatch):
     w = lambda rows, n: SimpleNamespace(rows=rows, n=n)  # noqa: E731
     pool = lambda n, ms, adapters=N, device=0: SimpleNamespace(n=n, ms=ms, num_adapters=adapters, context=SimpleNamespace(device=torch.device("cuda", device)))  # noqa: E731
     args = dict(x=torch.zeros(T, D, dtype=torch.bfloat16), y=torch.zeros(T, D, dtype=torch.bfloat16), gate_up=pool(D, [F, F]), down=pool(F, [D]),
-                ids=torch.zeros(T, dtype=torch.int32), plan=None)
+                ids=torch.zeros(T, dtype=torch.int32), plan=None, stream=None)
 
     def run(**over):
         a = {**args, **over}
-        return ops.SharedExpertInt4(ctx).encode_adapted(a["x"], w(F, D), w(F, D), w(D, F), a["y"], a["gate_up"], a["down"], a["ids"], plan=a["plan"])
+        return ops.SharedExpertInt4(ctx).encode_adapted(a["x"], w(F, D), w(F, D), w(D, F), a["y"], a["gate_up"], a["down"], a["ids"], plan=a["plan"], stream=a["stream"])
 
     run.pool = pool
     return run
@@ -114,3 +114,25 @@ def test_projections_that_refuse_their_operands(monkeypatch, bits):
     assert not launches
     run((4, 4, 4))
     assert launches == ["mf_qmm", "mf_qmm", "adapters", "silu_mul", "mf_qmm", "adapters"]
+
+
+def test_the_null_streams_handle(monkeypatch, call):
+    """torch.cuda.ExternalStream(0) is no stream of handle 0 but one of torch's own: stream=0 has to be the device's default stream"""
+    default, entered = SimpleNamespace(cuda_stream=0), []
+
+    def no_handle(handle, device=None):
+        raise AssertionError("a stream object of a handle of 0")
+
+    class Entered(Exception):
+        pass
+
+    def stream(s):
+        entered.append(s)
+        raise Entered
+
+    monkeypatch.setattr(ops.torch.cuda, "ExternalStream", no_handle)
+    monkeypatch.setattr(ops.torch.cuda, "default_stream", lambda device=None: default)
+    monkeypatch.setattr(ops.torch.cuda, "stream", stream)
+    with pytest.raises(Entered):
+        call(stream=0)
+    assert entered == [default]
