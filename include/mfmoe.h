@@ -121,7 +121,8 @@ typedef struct {
 mf_status mf_ctx_create(int device, mf_ctx** out);
 void mf_ctx_destroy(mf_ctx* ctx);
 const char* mf_status_string(mf_status s);
-/* text of the last failing HIP call on this context ("" if none) */
+/* text of the last failing HIP call on this context ("" if none), whichever thread made it: a copy that stays until the calling
+ * thread asks again */
 const char* mf_last_hip_error(const mf_ctx* ctx);
 int mf_abi_version(void);
 

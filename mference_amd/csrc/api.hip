@@ -1,5 +1,6 @@
 // The C ABI (include/mfmoe.h): argument validation, workspace ownership and
 // kernel dispatch.  Bad arguments return a negative status and launch nothing.
+#include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
 
@@ -11,6 +12,16 @@
 #include "mf_internal.h"
 #include "mf_qmm.h"
 
+void mf::set_hip_error(mf_ctx* ctx, const char* format, ...) {
+  va_list args;
+  va_start(args, format);
+  {
+    const std::lock_guard<std::mutex> lock(ctx->error_lock);
+    vsnprintf(ctx->hip_error, sizeof ctx->hip_error, format, args);
+  }
+  va_end(args);
+}
+
 namespace {
 
 constexpr int kAbiVersion = 3;  // 2: mf_moe_config.gate_group_size; 3: low-rank adapters, block norms
@@ -18,7 +29,7 @@ constexpr int kAbiVersion = 3;  // 2: mf_moe_config.gate_group_size; 3: low-rank
 constexpr uint32_t kRouterRows = 256;
 
 mf_status fail_hip(mf_ctx* ctx, hipError_t e, const char* what) {
-  if (ctx) snprintf(ctx->hip_error, sizeof ctx->hip_error, "%s: %s", what, hipGetErrorString(e));
+  if (ctx) mf::set_hip_error(ctx, "%s: %s", what, hipGetErrorString(e));
   return e == hipErrorOutOfMemory ? MF_ERR_OUT_OF_MEMORY : MF_ERR_LAUNCH;
 }
 
@@ -99,7 +110,13 @@ mf_status mf_ctx_create(int device, mf_ctx** out) {
 
 void mf_ctx_destroy(mf_ctx* ctx) { delete ctx; }
 
-const char* mf_last_hip_error(const mf_ctx* ctx) { return ctx ? ctx->hip_error : ""; }
+const char* mf_last_hip_error(const mf_ctx* ctx) {
+  static thread_local char text[sizeof ctx->hip_error];  // a copy: another thread's call may fail while this one reads
+  if (!ctx) return "";
+  const std::lock_guard<std::mutex> lock(ctx->error_lock);
+  memcpy(text, ctx->hip_error, sizeof text);
+  return text;
+}
 
 /* ----------------------------------------------------------------- format */
 
@@ -725,8 +742,7 @@ mf_status mf_moe_status(mf_moe* h, mf_stream stream) {
   MF_HIP(h->ctx, hipMemcpyAsync(&word, h->ws.status, sizeof word, hipMemcpyDeviceToHost, s));
   MF_HIP(h->ctx, hipStreamSynchronize(s));
   if (word != 0) {
-    snprintf(h->ctx->hip_error, sizeof h->ctx->hip_error,
-             "fused decode layer: a bounded wait on exchanged data gave up (status word %u)", word);
+    mf::set_hip_error(h->ctx, "fused decode layer: a bounded wait on exchanged data gave up (status word %u)", word);
     return MF_ERR_LAUNCH;
   }
   return MF_OK;

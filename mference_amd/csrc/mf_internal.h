@@ -6,12 +6,14 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <mutex>
 
 #include "../../include/mfmoe.h"
 
 struct mf_ctx {
   int device = 0;
   int num_cu = 0;
+  mutable std::mutex error_lock;  // calls that hold no state may fail on several threads at once
   char hip_error[256] = {0};
 };
 
@@ -50,6 +52,9 @@ struct mf_moe {
 };
 
 namespace mf {
+
+// the text that mf_last_hip_error gives from now on (api.hip)
+__attribute__((format(printf, 2, 3))) void set_hip_error(mf_ctx* ctx, const char* format, ...);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }

@@ -9,7 +9,6 @@
 // pointer, never the array's name.  All calls on one GPU share the array: calls that overlap on
 // one GPU (two streams, two host threads) race on it.  Nothing in it has to start at zero -- the
 // gate/up launch writes every element the down launch reads -- so nothing is cleared.
-#include <stdio.h>
 
 #include <atomic>
 
@@ -59,16 +58,14 @@ extern "C" mf_status mf_shared_expert_static(mf_ctx* ctx, mf_stream stream, cons
   }
   if (!mf::aligned2(x) || !mf::aligned2(y)) return MF_ERR_INVALID_ARGUMENT;
   if (static_cast<size_t>(t) * f > MF_STATIC_ACT_ELEMS) {
-    snprintf(ctx->hip_error, sizeof ctx->hip_error,
-             "mf_shared_expert_static: t*f = %zu activations exceed the built-in scratch of %u",
-             static_cast<size_t>(t) * f, static_cast<unsigned>(MF_STATIC_ACT_ELEMS));
+    mf::set_hip_error(ctx, "mf_shared_expert_static: t*f = %zu activations exceed the built-in scratch of %u",
+                      static_cast<size_t>(t) * f, static_cast<unsigned>(MF_STATIC_ACT_ELEMS));
     return MF_ERR_SCRATCH_TOO_SMALL;
   }
   void* const scratch_ptr =
       ctx->device >= 0 && ctx->device < kMaxDevices ? g_scratch_ptr[ctx->device].load(std::memory_order_acquire) : nullptr;
   if (!scratch_ptr) {
-    snprintf(ctx->hip_error, sizeof ctx->hip_error,
-             "mf_shared_expert_static: the scratch array's address is unknown on device %d", ctx->device);
+    mf::set_hip_error(ctx, "mf_shared_expert_static: the scratch array's address is unknown on device %d", ctx->device);
     return MF_ERR_LAUNCH;
   }
   auto* act = static_cast<uint16_t*>(scratch_ptr);
@@ -76,7 +73,7 @@ extern "C" mf_status mf_shared_expert_static(mf_ctx* ctx, mf_stream stream, cons
   hipError_t e = mf::launch_gate_up_act(s, gate, up, bits, x, act, f, d, t);
   if (e == hipSuccess) e = mf::launch_gemv(s, down, bits, act, y, d, f, t, false);
   if (e != hipSuccess) {
-    snprintf(ctx->hip_error, sizeof ctx->hip_error, "mf_shared_expert_static: %s", hipGetErrorString(e));
+    mf::set_hip_error(ctx, "mf_shared_expert_static: %s", hipGetErrorString(e));
     return MF_ERR_LAUNCH;
   }
   return MF_OK;
