@@ -700,7 +700,7 @@ mf_status mf_adapter_group(mf_ctx* ctx, mf_stream stream, const int32_t* adapter
  * sum over n is cut differently), never between two equal calls.
  * workspace: mf_adapter_workspace_bytes bytes, 16-byte aligned (they serve every smaller t too).  x and the ys are faster when
  * 16-byte aligned with strides that are multiples of 8.  No y may share memory with x or with another y, column ranges of one
- * buffer excepted (MF_ERR_INVALID_ARGUMENT).  t = 0 does nothing; t <= MF_MAX_ROWS.  An infinity or a NaN of x stays with its
+ * buffer excepted; and no y, nor the workspace, with anything else of the call (MF_ERR_INVALID_ARGUMENT).  t = 0 does nothing; t <= MF_MAX_ROWS.  An infinity or a NaN of x stays with its
  * row; one in an adapter's live weights makes the results it meets infinite or NaN.  Rows of an adapter of rank 0 keep their
  * bits too.  plan and workspace belong to the call until it has run: calls that may overlap, captured graphs among them, have
  * workspaces of their own (a plan is only read, and may be shared).  Forward only: the library has no gradients. */

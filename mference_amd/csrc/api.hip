@@ -1002,6 +1002,14 @@ bool rows_meet(const Rows& a, const Rows& b, uint64_t t) {
   return from_a < a.width || from_a + b.width > a.stride;
 }
 
+// Whether t rows can share a byte with a block of memory: one that lies among them has to keep to the columns that are not theirs.
+bool rows_meet_block(const Rows& rows, uint64_t t, const void* p, uint64_t bytes) {
+  if (!p || !bytes) return false;
+  const auto pa = reinterpret_cast<uintptr_t>(rows.p), pb = reinterpret_cast<uintptr_t>(p);
+  if (pa + (t - 1) * rows.stride + rows.width <= pb || pb + bytes <= pa) return false;
+  return rows_meet(rows, {p, rows.stride, bytes}, t);
+}
+
 bool adapter_pool_ok(const mf_adapter_pool* p) {
   return p && p->num_adapters >= 1 && p->num_adapters <= MF_MAX_ADAPTERS && p->rank >= 8 && p->rank <= MF_MAX_ADAPTER_RANK &&
          p->rank % 8 == 0 && p->n > 0 && p->n <= 1u << 22 && p->n % MF_GROUP_SIZE == 0;
@@ -1050,6 +1058,14 @@ mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool*
   const uint32_t size = y_f32 ? 4 : 2;
   Rows ys[MF_MAX_ADAPTER_TARGETS];
   const Rows xs = {x, 2ull * x_stride, 2ull * pool->n};
+  const size_t need = mf::adapter_workspace_bytes(num_targets, pool->rank, pool->n, t);
+  const Rows ws = {workspace, need, need};
+  // what the call reads beside x: the tables of the pool, the rows' adapters, the plan; the weights join them below
+  struct {
+    const void* p;
+    uint64_t bytes;
+  } read[4 + 2 * MF_MAX_ADAPTER_TARGETS] = {{pool->ranks, 4ull * pool->num_adapters}, {pool->scales, 4ull * pool->num_adapters}, {adapter_of_row, 4ull * t},
+                                            {plan, plan ? mf::AdapterPlan::words(t, pool->num_adapters) * sizeof(uint32_t) : 0}};
   mf::AdapterArgs a{};
   for (uint32_t k = 0; k < num_targets; ++k) {
     const mf_adapter_target& g = targets[k];
@@ -1060,9 +1076,19 @@ mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool*
     if (rows_meet(ys[k], xs, t)) return MF_ERR_INVALID_ARGUMENT;
     for (uint32_t j = 0; j < k; ++j)
       if (rows_meet(ys[j], ys[k], t)) return MF_ERR_INVALID_ARGUMENT;
+    const uint64_t weights = 2ull * pool->num_adapters * pool->rank;  // bytes, times the rows of a or b
+    read[4 + 2 * k] = {g.a, weights * pool->n}, read[5 + 2 * k] = {g.b, weights * g.m};
     a.target[k] = {g.a, g.b, g.y, g.m, g.y_stride};
   }
-  if (workspace_bytes < mf::adapter_workspace_bytes(num_targets, pool->rank, pool->n, t)) return MF_ERR_SCRATCH_TOO_SMALL;
+  if (workspace_bytes < need) return MF_ERR_SCRATCH_TOO_SMALL;
+  if (rows_meet_block(xs, t, workspace, need)) return MF_ERR_INVALID_ARGUMENT;
+  for (uint32_t k = 0; k < num_targets; ++k)
+    if (rows_meet_block(ys[k], t, workspace, need)) return MF_ERR_INVALID_ARGUMENT;
+  for (const auto& r : read) {
+    if (rows_meet_block(ws, 1, r.p, r.bytes)) return MF_ERR_INVALID_ARGUMENT;
+    for (uint32_t k = 0; k < num_targets; ++k)
+      if (rows_meet_block(ys[k], t, r.p, r.bytes)) return MF_ERR_INVALID_ARGUMENT;
+  }
   a.ranks = pool->ranks;
   a.scales = pool->scales;
   a.x = x;
