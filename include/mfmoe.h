@@ -665,7 +665,8 @@ typedef struct {
   uint32_t num_adapters;  /* 1 .. MF_MAX_ADAPTERS */
   uint32_t rank;          /* a multiple of 8, 8 .. MF_MAX_ADAPTER_RANK */
   uint32_t n;             /* length of a row of x, a multiple of 64, 64 .. 2^22 */
-  const uint32_t* ranks;  /* device [num_adapters], values 0 .. rank (larger ones count as rank); NULL: all `rank` */
+  const uint32_t* ranks;  /* device [num_adapters], values 0 .. rank (larger ones count as rank; from 2^31 on, negative as
+                           * int32, as 0); NULL: all `rank` */
   const float* scales;    /* device [num_adapters], c_a; NULL: all 1 */
 } mf_adapter_pool;
 

@@ -156,7 +156,10 @@ __global__ __launch_bounds__(1024) void adapter_group_kernel(const int32_t* __re
 
 // ------------------------------------------------------------------ which rows meet which adapter
 
-__device__ __forceinline__ uint32_t live_rank(const AdapterArgs& a, uint32_t adapter) { return a.ranks ? min(a.ranks[adapter], a.rank) : a.rank; }
+// (a number below zero, for callers whose tables are signed, is no rank)
+__device__ __forceinline__ uint32_t live_rank(const AdapterArgs& a, uint32_t adapter) {
+  return a.ranks ? static_cast<uint32_t>(max(0, min(static_cast<int>(a.ranks[adapter]), static_cast<int>(a.rank)))) : a.rank;
+}
 
 // ROWS rows of the batch, a lane each (ROWS <= 32; the lanes behind hold none), and the adapters that they meet.  With a plan they are
 // (a part of) one of its tiles, of one adapter; without one they are consecutive rows, whose adapters are taken one after the other in

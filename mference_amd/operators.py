@@ -347,7 +347,8 @@ class AdapterGrouping:
 class LowRankAdapters:
     """mf_adapter_apply: the low-rank corrections of many requests, added to the results of projections that read the same x
     (DequantInt4GEMV, MPPPrefillInt4QMM, SharedExpertInt4 leave them).  a[s] bf16 [num_adapters, rank, n] and
-    b[s] bf16 [num_adapters, m_s, rank] for every projection s; scales float32 and ranks int32 [num_adapters]."""
+    b[s] bf16 [num_adapters, m_s, rank] for every projection s; scales float32 and ranks int32 [num_adapters]
+    (below 0: 0; past rank: rank)."""
 
     def __init__(self, context: MetalContext, a: Sequence[torch.Tensor], b: Sequence[torch.Tensor],
                  scales: Optional[torch.Tensor] = None, ranks: Optional[torch.Tensor] = None):
