@@ -20,6 +20,7 @@ STATIC_ACT_ELEMS = MAX_TOKENS * 32768  # MF_STATIC_ACT_ELEMS
 BITS_TERNARY, BITS_2, BITS_4, BITS_8 = 1, 2, 4, 8
 ROUTER_TOPK_SOFTMAX, ROUTER_FULL_SOFTMAX = 0, 1
 
+MAX_ROWS = 1 << 20         # MF_MAX_ROWS
 MAX_ADAPTERS = 1024        # MF_MAX_ADAPTERS
 MAX_ADAPTER_RANK = 256     # MF_MAX_ADAPTER_RANK
 MAX_ADAPTER_TARGETS = 4    # MF_MAX_ADAPTER_TARGETS

@@ -19,8 +19,8 @@ import torch
 
 from . import _capi
 from ._capi import (BITS_2, BITS_4, BITS_8, BITS_TERNARY, GATE_CHANNEL, GATE_ELEMENT, GATE_NONE, GATE_ROW, GROUP_SIZE,
-                    MAX_ADAPTER_RANK, MAX_ADAPTER_TARGETS, MAX_ADAPTERS, MAX_TOKENS, ROUTER_FULL_SOFTMAX,
-                    ROUTER_TOPK_SOFTMAX, ExpertOffsets, MfError, check)
+                    MAX_ADAPTER_RANK, MAX_ADAPTER_TARGETS, MAX_ADAPTERS, MAX_ROWS, MAX_TOKENS,
+                    ROUTER_FULL_SOFTMAX, ROUTER_TOPK_SOFTMAX, ExpertOffsets, MfError, check)
 
 __all__ = [
     "MetalContext", "QuantizedTensor", "Quantization", "DequantInt4GEMV", "DequantInt4GEMVMultiX",
@@ -269,6 +269,9 @@ def _address(t: torch.Tensor, what: str, dtype, device: int) -> int:
     return t.data_ptr()
 
 
+_U32 = (1 << 32) - 1  # the largest number the library's arguments hold
+
+
 def _row_stride(t: torch.Tensor, what: str, shape) -> int:
     """elements from row to row of a tensor of this shape [rows, width] whose rows are contiguous"""
     if t.shape != shape:
@@ -281,6 +284,8 @@ def _row_stride(t: torch.Tensor, what: str, shape) -> int:
     stride = t.stride(0)
     if stride < width:
         raise MfError(-2, f"the rows of {what} overlap")
+    if stride > _U32:
+        raise MfError(-2, f"the rows of {what} are {stride} elements apart")
     return stride
 
 
@@ -302,7 +307,7 @@ class AdapterPlan:
     """What AdapterGrouping.encode fills: the rows of a batch in the order of their adapters (mf_adapter_group)."""
 
     def __init__(self, t: int, num_adapters: int, words: torch.Tensor):
-        need = int(_capi.lib().mf_adapter_plan_bytes(t, num_adapters)) if t >= 0 and num_adapters > 0 else 0
+        need = int(_capi.lib().mf_adapter_plan_bytes(t, num_adapters)) if 0 <= t <= MAX_ROWS and 0 < num_adapters <= MAX_ADAPTERS else 0
         if need == 0 or words.dtype is not torch.int32 or words.dim() != 1 or not words.is_contiguous() or words.numel() * 4 < need:
             raise MfError(-1, f"t={t}, num_adapters={num_adapters}: {need // 4} contiguous int32 words")
         self.t, self.num_adapters, self.words = t, num_adapters, words
@@ -327,7 +332,7 @@ class AdapterGrouping:
 
     def plan(self, t: int) -> AdapterPlan:
         """room for the plan of t rows"""
-        need = int(_capi.lib().mf_adapter_plan_bytes(t, self.num_adapters)) if t >= 0 else 0
+        need = int(_capi.lib().mf_adapter_plan_bytes(t, self.num_adapters)) if 0 <= t <= MAX_ROWS else 0
         return AdapterPlan(t, self.num_adapters, torch.empty(need // 4, dtype=torch.int32, device=self.context.device if need else "cpu"))
 
     def encode(self, adapter_of_row: torch.Tensor, plan: Optional[AdapterPlan] = None, stream=None) -> AdapterPlan:
@@ -374,12 +379,12 @@ class LowRankAdapters:
         for name, v, dtype in (("ranks", ranks, torch.int32), ("scales", scales, torch.float32)):
             if v is not None:
                 setattr(self.pool, name, _vector(v, name, dtype, device, (self.num_adapters,)))
-        if self.workspace_bytes(1) == 0:
-            raise MfError(-2, f"num_adapters={self.num_adapters} rank={self.rank} n={self.n}")
+        if max(self.num_adapters, self.rank, self.n) > _U32 or max(self.ms) > 1 << 28 or self.workspace_bytes(1) == 0:
+            raise MfError(-2, f"num_adapters={self.num_adapters} rank={self.rank} n={self.n} m={self.ms}")
 
     def workspace_bytes(self, t: int) -> int:
         """bytes that a call of t rows, or fewer, asks for"""
-        return int(_capi.lib().mf_adapter_workspace_bytes(C.byref(self.pool), len(self._fixed), t))
+        return int(_capi.lib().mf_adapter_workspace_bytes(C.byref(self.pool), len(self._fixed), t)) if 0 <= t <= MAX_ROWS else 0
 
     def encode(self, x: torch.Tensor, adapter_of_row: torch.Tensor, ys, plan: Optional[AdapterPlan] = None,
                workspace: Optional[torch.Tensor] = None, stream=None) -> None:
@@ -405,6 +410,8 @@ class LowRankAdapters:
         words = None if plan is None else plan._address_for(t, self.num_adapters, device)
         if t == 0:
             return
+        if t > MAX_ROWS:
+            raise MfError(-1, f"t={t} rows are more than one call takes")
         if workspace is None:
             workspace = _taken_on(ctx, stream, lambda: torch.empty(self.workspace_bytes(t), dtype=torch.uint8, device=ctx.device))
         elif not workspace.is_contiguous():
@@ -434,6 +441,8 @@ class BlockNorm:
         if len(shape) != 2:
             raise MfError(-2, "hidden must be [t, d]")
         t, d = shape
+        if t > MAX_ROWS or d > _U32:
+            raise MfError(-1 if t > MAX_ROWS else -2, f"t={t} rows of d={d} are more than one call takes")
         channels = (d,)
         h_ptr, h_stride = _rows(hidden, "hidden", bf16, device, shape)
         d_ptr = d_stride = f32 = o_ptr = o_stride = g_ptr = g_stride = pre = post = 0
@@ -454,6 +463,8 @@ class BlockNorm:
                 g_stride = gate.stride(0) if t > 1 else 1
                 if g_stride == 0 and t > 1:  # 0 means "not given" to the library
                     raise MfError(-2, "a gate of one logit a row cannot be an expanded one")
+                if g_stride > _U32:
+                    raise MfError(-2, f"the logits of the gate are {g_stride} elements apart")
             elif gate_kind == GATE_ELEMENT:
                 g_stride = _row_stride(gate, "gate", shape)
             else:
