@@ -730,7 +730,8 @@ typedef struct {
   int delta_f32;
   mf_gate_kind gate_kind;
   float post_eps, pre_eps;
-  float residual_scale, branch_scale; /* usually 1 */
+  float residual_scale, branch_scale; /* usually 1; without delta there is nothing to scale: any other residual_scale is refused
+                                       * (but the 0 of a cleared structure) */
   float weight_bias;                  /* added to both norms' weights: 1 where a model stores them as differences from one */
 } mf_block_norm_args;
 

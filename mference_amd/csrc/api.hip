@@ -1118,7 +1118,8 @@ mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args*
   if ((a.gate_kind != MF_GATE_NONE) != (a.gate != nullptr) || (!a.delta && (a.gate || a.post_weight)) ||
       (a.pre_weight != nullptr) != (a.out != nullptr) || (!a.delta && !a.out))
     return MF_ERR_INVALID_ARGUMENT;
-  if (!a.hidden) return MF_ERR_INVALID_ARGUMENT;
+  // the stream is only read without a block's output, and its scale would be lost (0: a cleared structure)
+  if (!a.hidden || (!a.delta && a.residual_scale != 1.0f && a.residual_scale != 0.0f)) return MF_ERR_INVALID_ARGUMENT;
   if (!a.hidden_stride) a.hidden_stride = a.d;
   if (!a.delta_stride) a.delta_stride = a.d;
   if (!a.out_stride) a.out_stride = a.d;

@@ -449,6 +449,8 @@ class BlockNorm:
         if delta is not None:
             f32 = 1 if delta.dtype is torch.float32 else 0
             d_ptr, d_stride = _rows(delta, "delta", torch.float32 if f32 else bf16, device, shape)
+        elif residual_scale != 1.0:
+            raise MfError(-1, f"residual_scale={residual_scale} without a block output: the stream is only read")
         if out is not None:
             o_ptr, o_stride = _rows(out, "out", bf16, device, shape)
         if pre_weight is not None:
