@@ -37,7 +37,7 @@ struct RowRanks {
         const uint64_t with = __ballot(set);
         same &= set ? with : ~with;
       }
-      const uint32_t in_front = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(same >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(same), 0));
+      const uint32_t in_front = lanes_in_front(same);
       if (valid) {
         const uint32_t before = counts[key[k]];
         rank[k] = before + in_front;

@@ -47,6 +47,16 @@ __device__ __forceinline__ uint16_t f_to_bf16(float x) {
 __device__ __forceinline__ uint16_t narrow_bf16(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
 __device__ __forceinline__ float round_bf16(float x) { return bf16_to_f(f_to_bf16(x)); }
 
+// Set bits of a mask of lanes in front of this lane, and in front of place `at` (0 .. 63).  Both take the mask as two words: a 64-bit shift by a
+// register reads a second one behind it, and where the amount lay in the last register of a wave some lanes got a wrong mask.
+__device__ __forceinline__ uint32_t lanes_in_front(uint64_t mask) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
+__device__ __forceinline__ uint32_t bits_in_front(uint64_t mask, uint32_t at) {
+  const uint32_t lo = static_cast<uint32_t>(mask), hi = static_cast<uint32_t>(mask >> 32), below = (1u << (at & 31)) - 1;
+  return at < 32 ? __popc(lo & below) : __popc(lo) + __popc(hi & below);
+}
+
 // ------------------------------------------------------------------- exp
 
 // Deterministic exp: the same sequence of IEEE operations as the CPU oracle,

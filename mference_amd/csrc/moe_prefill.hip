@@ -596,7 +596,7 @@ __global__ __launch_bounds__(256) void group_emit_kernel(const uint32_t* __restr
       const uint32_t e0 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(e), leader));
       const unsigned long long same = __ballot(open && e == e0);
       if (open && e == e0) {
-        rank = __popcll(same & ((1ull << lane) - 1ull));
+        rank = lanes_in_front(same);
         open = false;
       }
       if (lane == static_cast<uint32_t>(leader)) s_wave[wv][e0] = __popcll(same);
@@ -671,7 +671,7 @@ __device__ __forceinline__ void group_serial(const uint32_t* __restrict__ idx, c
       const unsigned long long same = __ballot(open && e == e0);
       const uint32_t base = s_hist[wv][e0];
       if (open && e == e0) {
-        pos = base + __popcll(same & ((1ull << lane) - 1ull));
+        pos = base + lanes_in_front(same);
         open = false;
       }
       if (lane == static_cast<uint32_t>(leader)) s_hist[wv][e0] = base + __popcll(same);
@@ -923,7 +923,7 @@ __global__ __launch_bounds__(MF_MAX_EXPERTS) void group_place_kernel(const uint3
     r.expert = ex;
     r.rank = threadIdx.x - i * K;
     r.weight_bits = wbits;
-    sorted[s_base[ex] + __popcll(s_mine[ex] & ((1ull << i) - 1ull))] = r;
+    sorted[s_base[ex] + bits_in_front(s_mine[ex], i)] = r;
   }
 }
 
