@@ -802,7 +802,6 @@ hipError_t launch_adapter_group(hipStream_t s, const int32_t* ids, uint32_t t, u
   };
   if (it == 1) go(std::integral_constant<int, 1>{});
   else if (it == 4) go(std::integral_constant<int, 4>{});
-  else if (it == 8) go(std::integral_constant<int, 8>{});
   else go(std::integral_constant<int, 16>{});
   return hipGetLastError();
 }

@@ -49,3 +49,14 @@ def test_no_64_bit_shift_by_a_vector_register(tmp_path):
                 found.append(f"{kernel} {line.split('//')[0].strip()}")
         assert listing.wait() == 0
     assert not found, found
+
+
+@pytest.mark.skipif(not os.path.exists(TOOLS + "llvm-readelf"), reason="no reader of code objects")
+def test_row_grouping_has_the_instances_that_are_launched(tmp_path):
+    """rows a lane takes in turn: 1, 4 or 16 (AdapterPlan::turns_of), counting runs or placing rows"""
+    names = set()
+    for path in code_objects(tmp_path):
+        symbols = subprocess.run([TOOLS + "llvm-readelf", "--symbols", "--wide", str(path)], capture_output=True, text=True, check=True).stdout
+        names |= set(re.findall(r"adapter_group_kernelILi(\d+)ELb(\d)E\w+(?!\w|\.kd)", symbols))
+    # a batch of one run (up to 4096 rows) has 1 or 4 turns and is not counted; longer ones have 1, 4 or 16 and are
+    assert names == {(turns, count) for turns in ("1", "4", "16") for count in ("0", "1")}
