@@ -701,10 +701,11 @@ mf_status mf_adapter_group(mf_ctx* ctx, mf_stream stream, const int32_t* adapter
  * sum over n is cut differently), never between two equal calls.
  * workspace: mf_adapter_workspace_bytes bytes, 16-byte aligned (they serve every smaller t too).  x and the ys are faster when
  * 16-byte aligned with strides that are multiples of 8.  No y may share memory with x or with another y, column ranges of one
- * buffer excepted; and no y, nor the workspace, with anything else of the call (MF_ERR_INVALID_ARGUMENT).  t = 0 does nothing; t <= MF_MAX_ROWS.  An infinity or a NaN of x stays with its
- * row; one in an adapter's live weights makes the results it meets infinite or NaN.  Rows of an adapter of rank 0 keep their
- * bits too.  plan and workspace belong to the call until it has run: calls that may overlap, captured graphs among them, have
- * workspaces of their own (a plan is only read, and may be shared).  Forward only: the library has no gradients. */
+ * buffer excepted; and no y, nor the workspace, with anything else of the call (MF_ERR_INVALID_ARGUMENT).  t = 0 does nothing;
+ * t <= MF_MAX_ROWS.  An infinity or a NaN of x stays with its row; one in an adapter's live weights makes the results it meets
+ * infinite or NaN.  Rows of an adapter of rank 0 keep their bits too.  plan and workspace belong to the call until it has run:
+ * calls that may overlap, captured graphs among them, have workspaces of their own (a plan is only read, and may be shared).
+ * Forward only: the library has no gradients. */
 size_t mf_adapter_workspace_bytes(const mf_adapter_pool* pool, uint32_t num_targets, uint32_t t);
 mf_status mf_adapter_apply(mf_ctx* ctx, mf_stream stream, const mf_adapter_pool* pool, const mf_adapter_target* targets,
                            uint32_t num_targets, const uint16_t* x, uint32_t x_stride, const int32_t* adapter_of_row, uint32_t t,
@@ -744,9 +745,9 @@ typedef struct {
  * mf_residual_rmsnorm joins them, with the norm behind the block (the layers that have one: one norm on either side of attention and
  * MLP), the gate and the scales.  fp32 between the roundings named; as in mf_residual_rmsnorm the second norm is of the narrowed
  * stream.  The two calls add the squares of a row in different orders.  out may share no memory with hidden, delta or gate, hidden
- * none with delta or gate, neither with a weight (MF_ERR_INVALID_ARGUMENT).  The squares of a row are added in fp32: magnitudes
- * from about 2^63 on overflow to a norm of 0.  Any d of 1 .. 2^28; t = 0 does nothing; t <= MF_MAX_ROWS.  Faster where all
- * tensors are 16-byte aligned and d and the strides are multiples of 8. */
+ * none with delta or gate, neither with a weight (MF_ERR_INVALID_ARGUMENT).  The squares of a row are added in fp32: a row whose
+ * root mean square is 2^64 / sqrt(d) or more (2^58 for d = 4096) overflows to a norm of 0.  Any d of 1 .. 2^28; t = 0 does
+ * nothing; t <= MF_MAX_ROWS.  Faster where all tensors are 16-byte aligned and d and the strides are multiples of 8. */
 mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args* args);
 
 #ifdef __cplusplus
