@@ -69,7 +69,7 @@ __device__ __forceinline__ uint2 block_exclusive(uint2 v, uint2* part) {
 // those counts of all runs (a thread a key), knows from them where every key's rows start and where its own go, and writes its rows;
 // the lists of adapters and tiles are dealt out over the workgroups.  A batch of one run needs no counting launch in front: up to 4096
 // rows, where one workgroup's turns still cost less than a second launch.  Four bytes a row are read and written: what it takes is latency (ids,
-// ballots, two scans, scattered stores): 200 rows 2.7 us, 16384 rows 3.7 + 6.7 us.  Calls of the simple form (a thread an adapter that
+// ballots, two scans, scattered stores): 200 rows 2.8 us, 16384 rows 3.7 + 6.8 us.  Calls of the simple form (a thread an adapter that
 // reads all rows) took 27 and 1829 us.
 constexpr uint32_t kOwnTiles = 4;
 
@@ -331,7 +331,7 @@ template <int RT, int CF> constexpr int kUnitsAhead = 6 - RT - CF;
 
 // The first of two launches: v to memory, in parts over n.  It reads x once for every RT * 16 rows and two blocks of ranks, and those
 // rows of A; matrix instructions are a few percent of its time.  Bound by the loads' latency: a wave has two to four
-// units in flight and often no more than three turns.  777 rows of 4096, rank 64, two targets: 11.1 us, 14.5 MB from memory; 4096 rows of
+// units in flight and often no more than three turns.  777 rows of 4096, rank 64, two targets: 12.4 us, 14.5 MB from memory; 4096 rows of
 // 5120, rank 16, two targets: 18.9 us, 45.6 MB = 2.4 TB/s; eight rows of 17408, rank 16: 5.6 us.
 // The simple form of both launches (a dot product a wave, a result a thread) took 932 and 4263 us for the two prompts.
 template <int RT, int CF>
@@ -578,8 +578,8 @@ struct Share {
 
 // The second of two launches.  A workgroup takes RT * 16 rows and a run of a target's results, and adds up the parts of v itself: a
 // third launch that did would cost more.  Long batches are bound by y, which is read and written once: 4096 rows, rank 16, two times 17408,
-// 137 us, 345 MB read and 285 written = 4.6 TB/s, where a copy reaches 4.8.  Short ones are bound by a chain of requests (rows and
-// adapters 1.1 us, parts of v 2.9, products and y 1.8): 777 rows, rank 64, two times 2048, 10.9 us; eight rows, 5120 in fp32, 6.5 us.  Tried: eight
+// 138 us, 345 MB read and 285 written = 4.6 TB/s, where a copy reaches 4.8.  Short ones are bound by a chain of requests (rows and
+// adapters 1.1 us, parts of v 2.9, products and y 1.8): 777 rows, rank 64, two times 2048, 11.3 us; eight rows, 5120 in fp32, 6.6 us.  Tried: eight
 // waves (no gain), y past the caches (no gain), whole lines of y in 8-byte pieces (199 us where it took 146), a wave's results one behind the
 // other (rows that start inside a line 108 -> 126 us).  Such rows cost: two times 13992 (16-byte places) 108 us where whole lines would take 85,
 // 13999 (2-byte places) 152.
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void adapter_expand_kernel(const
 //
 // Every workgroup makes the v of its rows and its target for itself, over the whole of n, and goes on to its results: nothing goes
 // through memory in between, and there is no second launch.  Workgroups that share rows make the same v, on compute units that
-// would have nothing else to do.  One row of 2048, rank 16, two times 512: 5.6 us (ids 0.8, addresses 0.7, the loop over n 1.3, the
+// would have nothing else to do.  One row of 2048, rank 16, two times 512: 5.5 us (ids 0.8, addresses 0.7, the loop over n 1.3, the
 // waves' sums 1.0, results 0.8; the rest starts and ends the launch).  Four rows of 5120, rank 32, two times 17408: 10.4 us, of which 4.2 are
 // the loop, which draws 410 KB of x and A through a CU's L1, 40 bytes a clock of 64.  200 mixed rows of 2816, rank 24, two
 // times 2112: 11.5 us, 25 MB from memory.  Sixteen waves, and more units in flight, were no gain.
@@ -756,8 +756,10 @@ struct Tiling {
     // Consecutive rows of a short batch: the adapters of a tile side by side.  Us a pass, all of one tile's after one another / side by
     // side: 80 rows of several requests, one launch of rank 16, 2048 to two times 2048, 13.4 / 7.0, of one request 6.8 / 6.9, but 1000 rows
     // of one request 9.6 / 11.4; the second of two launches of rank 64, two times 4096, 80 rows 15.4 / 9.4 (one request 7.9 / 8.1), 777 rows, two
-    // times 2048, 13.5 / 11.0 (9.5 / 9.8), 2000 rows 32.4 / 34.1; the first, whose workgroups are many, 1000 rows of 8192, 12.7 / 11.1, 200 rows
-    // of 5120 10.2 / 13.4, 1402 rows 12.0 / 13.6.
+    // times 2048, 13.5 / 11.0 (9.5 / 9.8), 2000 rows 32.4 / 34.1.  The first of two launches has workgroups for its parts of n and groups of ranks
+    // too: 1000 rows of 8192 (32 tiles of 32 rows) 12.7 / 11.1, 1402 rows 12.0 / 13.6, 200 rows of 5120 (13 tiles of 16) 10.2 / 13.4; 257 to 512 rows (9
+    // to 16 tiles of 32) go either way and take one: 300 rows of 4096, rank 64, 9.6 / 8.4, 512 rows of 17408, rank 16, 14.1 / 9.4, of 4096, rank 64, 10.2 / 9.2,
+    // rank 128 13.2 / 15.5.
     const auto at_once = [&](uint32_t most) { return planned ? 1 : std::min({a.t, a.num_adapters, most}); };
     turns = at_once(tiles <= 4 ? 16 : tiles <= 16 ? 4 : 1);
     shrink_turns = at_once(tiles <= 4 ? 16 : tiles > 16 && tiles <= 32 ? 2 : 1);

@@ -69,9 +69,9 @@ __device__ __forceinline__ void store8(uint16_t* p, uint32_t have, const uint4& 
 
 // A workgroup a row, the row in registers: NV pieces of eight elements a thread, all that the row takes part in requested at once,
 // in front of the first sum, and kept as it lies in memory until it is used; two sums over the workgroup; every byte read and
-// written once.  Long batches run at the rate of a copy: 8192 rows of 5120, all operands bf16, 70 us, 168 MB read and 168 written = 4.8 TB/s.  Short
-// ones are the latency of a request, two sums and a launch: one row of 2048 2.7 us, eight of 2816 4.2, 777 of 4096 with an fp32 block output and a gate
-// an element 11.5 us (25.7 + 12.7 MB).
+// written once.  Long batches run at the rate of a copy: 8192 rows of 5120, all operands bf16, 71 us, 168 MB read and 168 written = 4.8 TB/s.  Short
+// ones are the latency of a request, two sums and a launch: one row of 2048 2.7 us, eight of 2816 4.4, 777 of 4096 with an fp32 block output and a gate
+// an element 11.4 us (25.7 + 12.7 MB).
 // Calls of the simple form (three passes over the row) took 8.2, 8.8, 28 and 217 us, in the order of one, eight, 777 and 8192 rows.
 template <int NV, bool F32>
 __global__ __launch_bounds__(1024) void block_norm_kernel(const mf_block_norm_args a) {
@@ -151,7 +151,9 @@ __global__ __launch_bounds__(1024) void block_norm_kernel(const mf_block_norm_ar
   }
 }
 
-// rows that registers do not hold: three passes of the workgroup over its row
+// Rows that registers do not hold: three passes of the workgroup over its row, the later ones mostly from the caches.  Both norms, all operands bf16, us a
+// pass: 512 rows of 32768 33.4, 2048 of 20000 78.8 (4.0 and 4.2 TB/s of the bytes that one pass would move; 2048 rows of 16384, in registers, 57.0 = 4.7),
+// one row of 32768 11.0.
 template <bool F32>
 __global__ __launch_bounds__(1024) void block_norm_long_kernel(const mf_block_norm_args a) {
   __shared__ float part[2][16];
