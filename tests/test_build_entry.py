@@ -49,6 +49,14 @@ def test_build_with_a_program_whose_source_is_absent(tree):
     assert os.path.exists(cpp / "mirror_test") and not os.path.exists(cpp / "adapters_test")
 
 
+def test_build_with_a_program_that_only_makes_own_rules_know(tree):
+    """a source without a rule in the Makefile: make would compile it by a rule of its own, which lacks the include paths"""
+    cpp = _makefile(tree, "mirror_test")
+    (cpp / "adapters_test.cpp").write_text('#include "mfmoe.hpp"\nint main() {}\n')
+    entry.build()
+    assert os.path.exists(cpp / "mirror_test") and not os.path.exists(cpp / "adapters_test")
+
+
 def test_build_without_tests(tree):
     entry.build()
 
