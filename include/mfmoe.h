@@ -750,6 +750,107 @@ typedef struct {
  * nothing; t <= MF_MAX_ROWS.  Faster where all tensors are 16-byte aligned and d and the strides are multiples of 8. */
 mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args* args);
 
+/* ------------------------------------------------- layers kept in 16 bits */
+
+/* Mixed-precision conversions keep some layers in 16 bits: the projections around attention, an image encoder, the first and last
+ * layers, the experts of a model that is compared against.  The calls below are those layers' products, what stands between the
+ * projections and attention, and their experts, beside the routers and norms above.  Forward only. */
+
+/* What is applied to a product, in fp32.  z / (1 + e^-z); 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))); 0.5 z (1 + erf(z / sqrt 2)). */
+typedef enum { MF_ACT_NONE = 0, MF_ACT_SILU = 1, MF_ACT_GELU_TANH = 2, MF_ACT_GELU = 3 } mf_activation;
+
+typedef struct {
+  const uint16_t* x;     /* bf16 [t, n] */
+  const uint16_t* w;     /* bf16 [m, n]; gated: [2 m, n], the gate's rows first */
+  const uint16_t* bias;  /* bf16 [m], gated: [2 m]; NULL: none */
+  const void* residual;  /* [t, m], of y's type; NULL: none; may be y itself (same address and stride) */
+  void* y;               /* [t, m]: bf16, or fp32 when y_f32 != 0 */
+  uint32_t t, m, n;
+  uint32_t x_stride, w_stride, residual_stride, y_stride; /* elements from row to row; 0: the row's width */
+  int y_f32;
+  int gated;
+  mf_activation activation;
+} mf_project_args;
+
+/* y = narrow(residual + act(x W^T + bias)), gated: narrow(residual + act(x G^T + bias_g) * (x U^T + bias_u)), W = [G; U].
+ * The projection that DequantInt4GEMV and MPPPrefillInt4QMM are for quantized weights (Kernels/Quant/DequantInt4GEMV.swift:57-103,
+ * Kernels/TensorCore/MPPPrefillInt4QMM.swift:34-78), with what follows it in the same launch; no counterpart in the reference.
+ * Sums, bias, activation and residual in fp32, one rounding at the end.  Any t of 0 .. MF_MAX_ROWS (0 does nothing), m of 1 .. 2^24, n of
+ * 1 .. 2^22, any strides that are no shorter than their row.  Faster where x and w are 16-byte aligned with n and the strides multiples
+ * of 8.  workspace: mf_project_workspace_bytes(m, n, t, gated) bytes, 16-byte aligned (0: none is needed, it may be NULL); they serve
+ * every smaller t of the same m and n too.  It belongs to the call until that has run.  y may share no memory with anything that the call
+ * reads but residual as said above, nor with the workspace (MF_ERR_INVALID_ARGUMENT).  A row's last bits may differ between batches of
+ * other sizes (the sum over n is cut by the batch), never between two equal calls.  An infinity or a NaN of x stays with its row, one of
+ * w or bias with its column. */
+size_t mf_project_workspace_bytes(uint32_t m, uint32_t n, uint32_t t, int gated);
+mf_status mf_project(mf_ctx* ctx, mf_stream stream, const mf_project_args* args, void* workspace, size_t workspace_bytes);
+
+/* Heads of rows: head h of row i starts at element i * row_stride + h * head_stride.  Either order of the two axes in memory will do
+ * (heads side by side in a row, or a head's rows side by side), in a buffer of its own or in part of one. */
+typedef struct {
+  const uint16_t* x;       /* bf16; NULL with heads = 0: none of this kind */
+  uint16_t* out;           /* bf16; x itself with the same strides: in place */
+  const uint16_t* weight;  /* bf16 [head_dim]; NULL: no norm */
+  uint32_t heads;
+  uint32_t row_stride, head_stride, out_row_stride, out_head_stride; /* row strides 0: heads * head stride; head strides 0: head_dim */
+} mf_head_rows;
+
+typedef struct {
+  mf_head_rows q, k;
+  const int32_t* positions;     /* [axes, t], axis a of row i at a * position_stride + i; NULL: no rotation */
+  const float* inv_freq;        /* [rotary_dim / 2]: the angle of a pair for each step of its position */
+  const uint8_t* axis_of_pair;  /* [rotary_dim / 2], values 0 .. axes - 1 (others: the pair is not turned); NULL: axis 0 for all */
+  uint32_t t, head_dim, rotary_dim, axes, position_stride; /* position_stride 0: t */
+  int interleaved;              /* pair p is elements (2 p, 2 p + 1); else (p, p + rotary_dim / 2) */
+  float eps, weight_bias;       /* weight_bias is added to both weights: 1 where a model stores them as differences from one */
+  float rotation_scale;         /* times cosine and sine (scaled context windows); usually 1 */
+} mf_head_norms_args;
+
+/* What stands between the projections and attention, one launch and one pass over the heads: for every head of q and k
+ *   z = h * rsqrt(mean(h^2) + eps) * (weight + weight_bias)          (h itself without a weight)
+ *   pair p of its first rotary_dim elements (a, b) -> (a c - b s, b c + a s),  c, s = rotation_scale * cos, sin of
+ *       positions[axis_of_pair[p], row] * inv_freq[p]
+ * narrowed once.  RMSNorm.encodeBF16W (Kernels/Primitives/RMSNorm.swift:52-64) for heads, and the rotation behind it; no counterpart in
+ * the reference's operators of this library.  Positions of several axes (time, height, width) turn the pairs that axis_of_pair gives
+ * them.  The angle is reduced in fp64, so that far positions keep theirs; everything else is fp32.  head_dim 1 .. 1024, rotary_dim even,
+ * 0 .. head_dim (0 without positions), axes 1 .. 8, heads 0 .. 65535, t 0 .. MF_MAX_ROWS.  What is written may share no memory with anything
+ * else of the call but a head's own input in place (MF_ERR_INVALID_ARGUMENT).  Faster where head_dim and rotary_dim are multiples of 16
+ * and all addresses and strides are of 16 bytes. */
+mf_status mf_head_norms(mf_ctx* ctx, mf_stream stream, const mf_head_norms_args* args);
+
+#define MF_BF16_EXPERTS_ROWS 64
+
+/* A layer of experts kept in 16 bits. */
+typedef struct {
+  const uint16_t* gate_up;         /* bf16 [num_experts, 2 f, d], the gate's rows first, 16-byte aligned */
+  const uint16_t* down;            /* bf16 [num_experts, d, f], 16-byte aligned */
+  const uint16_t* gate_up_bias;    /* bf16 [num_experts, 2 f]; NULL: none */
+  const uint16_t* down_bias;       /* bf16 [num_experts, d]; NULL: none */
+  const uint16_t* shared_gate_up;  /* bf16 [2 shared_f, d], 16-byte aligned; used when shared_f > 0 */
+  const uint16_t* shared_down;     /* bf16 [d, shared_f], 16-byte aligned */
+  const uint16_t* shared_gate;     /* bf16 [d]: the shared expert's result times sigmoid(shared_gate . x); NULL: as it is */
+  uint32_t num_experts;            /* 1 .. MF_MAX_EXPERTS */
+  uint32_t top_k;                  /* 1 .. MF_MAX_TOPK */
+  uint32_t d, f, shared_f;         /* multiples of 8, 8 .. 2^20 (shared_f: 0: no shared expert) */
+  mf_activation activation;
+} mf_bf16_expert_pool;
+
+/* The layer for a few tokens, in two launches that read each live expert once: for token i with experts idx[i, k] and weights w[i, k]
+ * (from any of the routers above)
+ *   y = narrow(residual + sum over k of w * (down_e a + down_bias_e) + sigmoid(shared_gate . x) * shared_down a_s)
+ *   a = act(gate_e x + bias) * (up_e x + bias')
+ * What mf_moe_decode_layer is for quantized experts (RealForwardRunner.swift:2811-3218), the routing given; no counterpart in the
+ * reference.  Products in fp32; the activations meet the second product as two bf16 terms (2^-16 of them is lost), the sums over f, k
+ * and the shared expert and the residual are fp32, one rounding at the end.  An index >= num_experts contributes nothing, an expert named
+ * twice contributes twice.  t 0 .. MF_BF16_EXPERTS_ROWS (0 does nothing; longer batches go in parts).  residual may be y itself (same
+ * address and stride); y otherwise shares no memory with what the call reads (MF_ERR_INVALID_ARGUMENT).  The sums are cut by t and the
+ * sizes: a token's last bits may differ beside other tokens, never between two equal calls.  workspace: 16-byte aligned,
+ * mf_bf16_experts_workspace_bytes bytes (they serve every smaller t); it belongs to the call until that has run. */
+size_t mf_bf16_experts_workspace_bytes(const mf_bf16_expert_pool* pool, uint32_t t);
+mf_status mf_bf16_experts(mf_ctx* ctx, mf_stream stream, const mf_bf16_expert_pool* pool, const uint16_t* x, uint32_t x_stride,
+                          const uint32_t* idx, const float* w, const uint16_t* residual, uint32_t residual_stride, uint32_t t,
+                          uint16_t* y, uint32_t y_stride, void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,8 @@ MAX_ADAPTERS = 1024        # MF_MAX_ADAPTERS
 MAX_ADAPTER_RANK = 256     # MF_MAX_ADAPTER_RANK
 MAX_ADAPTER_TARGETS = 4    # MF_MAX_ADAPTER_TARGETS
 GATE_NONE, GATE_ROW, GATE_ELEMENT, GATE_CHANNEL = 0, 1, 2, 3
+ACT_NONE, ACT_SILU, ACT_GELU_TANH, ACT_GELU = 0, 1, 2, 3
+BF16_EXPERTS_ROWS = 64     # MF_BF16_EXPERTS_ROWS
 
 STATUS_NAMES = {
     0: "MF_OK", -1: "MF_ERR_INVALID_ARGUMENT", -2: "MF_ERR_DIMENSION_MISMATCH",
@@ -92,6 +94,33 @@ class BlockNormArgs(C.Structure):
                 ("residual_scale", C.c_float), ("branch_scale", C.c_float), ("weight_bias", C.c_float)]
 
 
+class ProjectArgs(C.Structure):
+    """mf_project_args"""
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p),
+                ("t", C.c_uint32), ("m", C.c_uint32), ("n", C.c_uint32),
+                ("x_stride", C.c_uint32), ("w_stride", C.c_uint32), ("residual_stride", C.c_uint32), ("y_stride", C.c_uint32),
+                ("y_f32", C.c_int), ("gated", C.c_int), ("activation", C.c_int)]
+
+
+class HeadRows(C.Structure):
+    """mf_head_rows"""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("weight", C.c_void_p), ("heads", C.c_uint32),
+                ("row_stride", C.c_uint32), ("head_stride", C.c_uint32), ("out_row_stride", C.c_uint32), ("out_head_stride", C.c_uint32)]
+
+
+class HeadNormsArgs(C.Structure):
+    """mf_head_norms_args"""
+    _fields_ = [("q", HeadRows), ("k", HeadRows), ("positions", C.c_void_p), ("inv_freq", C.c_void_p), ("axis_of_pair", C.c_void_p),
+                ("t", C.c_uint32), ("head_dim", C.c_uint32), ("rotary_dim", C.c_uint32), ("axes", C.c_uint32), ("position_stride", C.c_uint32),
+                ("interleaved", C.c_int), ("eps", C.c_float), ("weight_bias", C.c_float), ("rotation_scale", C.c_float)]
+
+
+class Bf16ExpertPool(C.Structure):
+    """mf_bf16_expert_pool"""
+    _fields_ = [(n, C.c_void_p) for n in ("gate_up", "down", "gate_up_bias", "down_bias", "shared_gate_up", "shared_down", "shared_gate")] + [
+        (n, C.c_uint32) for n in ("num_experts", "top_k", "d", "f", "shared_f")] + [("activation", C.c_int)]
+
+
 # every entry point include/mfmoe.h declares: name -> (restype, argtypes)
 _P, _SZ, _U32, _I = C.c_void_p, C.c_size_t, C.c_uint32, C.c_int
 SIGNATURES = {
@@ -151,6 +180,11 @@ SIGNATURES = {
     "mf_adapter_workspace_bytes": (_SZ, [C.POINTER(AdapterPool), _U32, _U32]),
     "mf_adapter_apply": (_I, [_P, _P, C.POINTER(AdapterPool), _P, _U32, _P, _U32, _P, _U32, _I, _P, _P, _SZ]),
     "mf_block_norm": (_I, [_P, _P, _P]),
+    "mf_project_workspace_bytes": (_SZ, [_U32, _U32, _U32, _I]),
+    "mf_project": (_I, [_P, _P, _P, _P, _SZ]),
+    "mf_head_norms": (_I, [_P, _P, _P]),
+    "mf_bf16_experts_workspace_bytes": (_SZ, [C.POINTER(Bf16ExpertPool), _U32]),
+    "mf_bf16_experts": (_I, [_P, _P, C.POINTER(Bf16ExpertPool), _P, _U32, _P, _P, _P, _U32, _U32, _P, _U32, _P, _SZ]),
     "mf_group_pairs_host": (_I, [_P, _SZ, _I, _I, _I, _I, _P, _SZ, _P, _P, _P, _P,
                                  C.POINTER(_SZ), _P, C.POINTER(_SZ), _P]),
 }

@@ -5,10 +5,12 @@
 #include <string.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <new>
 #include <vector>
 
 #include "mf_adapters.h"
+#include "mf_dense16.h"
 #include "mf_internal.h"
 #include "mf_qmm.h"
 
@@ -24,7 +26,7 @@ void mf::set_hip_error(mf_ctx* ctx, const char* format, ...) {
 
 namespace {
 
-constexpr int kAbiVersion = 3;  // 2: mf_moe_config.gate_group_size; 3: low-rank adapters, block norms
+constexpr int kAbiVersion = 4;  // 2: mf_moe_config.gate_group_size; 3: low-rank adapters, block norms; 4: layers kept in 16 bits
 // rows of router logits a handle holds for mf_moe_router calls that bring no logits buffer
 constexpr uint32_t kRouterRows = 256;
 
@@ -1148,6 +1150,201 @@ mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args*
   const OnDevice on(ctx);
   MF_HIP(ctx, on.error());
   MF_HIP(ctx, mf::launch_block_norm(static_cast<hipStream_t>(stream), a));
+  return MF_OK;
+}
+
+/* ------------------------------------------------- layers kept in 16 bits */
+
+namespace {
+
+bool activation_ok(int act) { return act >= MF_ACT_NONE && act <= MF_ACT_GELU; }
+
+// Whether t rows that are written can share a byte with one of the blocks that the call reads.
+struct Block {
+  const void* p;
+  uint64_t bytes;
+};
+bool rows_meet_any(const Rows& written, uint64_t t, std::initializer_list<Block> blocks) {
+  for (const Block& b : blocks)
+    if (rows_meet_block(written, t, b.p, b.bytes)) return true;
+  return false;
+}
+
+bool projection_ok(uint32_t m, uint32_t n, uint32_t t) { return m >= 1 && m <= 1u << 24 && n >= 1 && n <= 1u << 22 && t <= MF_MAX_ROWS; }
+
+}  // namespace
+
+size_t mf_project_workspace_bytes(uint32_t m, uint32_t n, uint32_t t, int gated) {
+  return projection_ok(m, n, t) ? mf::project_workspace_bytes(m, n, t, gated != 0) : 0;
+}
+
+mf_status mf_project(mf_ctx* ctx, mf_stream stream, const mf_project_args* args, void* workspace, size_t workspace_bytes) {
+  if (!ctx || !args) return MF_ERR_INVALID_ARGUMENT;
+  mf_project_args a = *args;
+  if (a.t > MF_MAX_ROWS || !activation_ok(a.activation)) return MF_ERR_INVALID_ARGUMENT;
+  if (!projection_ok(a.m, a.n, a.t)) return MF_ERR_DIMENSION_MISMATCH;
+  if (a.t == 0) return MF_OK;
+  if (!a.x || !a.w || !a.y) return MF_ERR_INVALID_ARGUMENT;
+  if (!a.x_stride) a.x_stride = a.n;
+  if (!a.w_stride) a.w_stride = a.n;
+  if (!a.y_stride) a.y_stride = a.m;
+  if (!a.residual_stride) a.residual_stride = a.m;
+  if (a.x_stride < a.n || a.w_stride < a.n || a.y_stride < a.m || (a.residual && a.residual_stride < a.m)) return MF_ERR_DIMENSION_MISMATCH;
+  const bool f32 = a.y_f32 != 0;
+  if (!mf::aligned2(a.x) || !mf::aligned2(a.w) || !mf::aligned2(a.bias) || !(f32 ? aligned4(a.y) && aligned4(a.residual) : mf::aligned2(a.y) && mf::aligned2(a.residual)))
+    return MF_ERR_INVALID_ARGUMENT;
+  const uint64_t size = f32 ? 4 : 2, t = a.t, rows = a.gated ? 2ull * a.m : a.m;
+  const Rows y = {a.y, size * a.y_stride, size * a.m};
+  const size_t need = mf::project_workspace_bytes(a.m, a.n, a.t, a.gated != 0);
+  if (need && (!workspace || !mf::aligned16(workspace))) return MF_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < need) return MF_ERR_SCRATCH_TOO_SMALL;
+  const bool in_place = a.residual == a.y && (a.residual_stride == a.y_stride || a.t == 1);
+  const Rows x = {a.x, 2ull * a.x_stride, 2ull * a.n}, w = {a.w, 2ull * a.w_stride, 2ull * a.n};
+  const Block bias = {a.bias, a.bias ? 2 * rows : 0}, ws = {workspace, need};
+  if (rows_meet(y, x, t) || (a.residual && !in_place && rows_meet(y, {a.residual, size * a.residual_stride, size * a.m}, t))) return MF_ERR_INVALID_ARGUMENT;
+  // (w's rows are other ones than y's: column ranges of one buffer are not told apart)
+  if (rows_meet_any(y, t, {{a.w, (rows - 1) * w.stride + w.width}, bias, ws})) return MF_ERR_INVALID_ARGUMENT;
+  if (need && (rows_meet_block(x, t, workspace, need) || rows_meet_block(w, rows, workspace, need) ||
+               (a.residual && rows_meet_block({a.residual, size * a.residual_stride, size * a.m}, t, workspace, need)) ||
+               (a.bias && rows_meet_block({workspace, need, need}, 1, bias.p, bias.bytes))))
+    return MF_ERR_INVALID_ARGUMENT;
+  const OnDevice on(ctx);
+  MF_HIP(ctx, on.error());
+  MF_HIP(ctx, mf::launch_project(static_cast<hipStream_t>(stream), a, workspace));
+  return MF_OK;
+}
+
+namespace {
+
+// The bytes of t rows of heads as rows for rows_meet: rows of heads side by side, or heads of rows side by side.  False where rows or heads overlap.
+struct HeadRows {
+  Rows rows;
+  uint64_t count;
+};
+bool head_rows(const void* p, uint64_t heads, uint64_t t, uint64_t row_stride, uint64_t head_stride, uint64_t dim, HeadRows* out) {
+  const uint64_t across = (heads - 1) * head_stride + dim, along = (t - 1) * row_stride + dim;
+  if ((heads == 1 || head_stride >= dim) && (t == 1 || row_stride >= across)) {
+    *out = {{p, 2 * (t == 1 ? std::max(row_stride, across) : row_stride), 2 * across}, t};
+    return true;
+  }
+  if (row_stride >= dim && head_stride >= along) {
+    *out = {{p, 2 * head_stride, 2 * along}, heads};
+    return true;
+  }
+  return false;
+}
+bool heads_meet(const HeadRows& a, const HeadRows& b) {
+  const auto pa = reinterpret_cast<uintptr_t>(a.rows.p), pb = reinterpret_cast<uintptr_t>(b.rows.p);
+  if (pa + (a.count - 1) * a.rows.stride + a.rows.width <= pb || pb + (b.count - 1) * b.rows.stride + b.rows.width <= pa) return false;
+  return rows_meet(a.rows, b.rows, std::max(a.count, b.count));
+}
+
+}  // namespace
+
+mf_status mf_head_norms(mf_ctx* ctx, mf_stream stream, const mf_head_norms_args* args) {
+  if (!ctx || !args) return MF_ERR_INVALID_ARGUMENT;
+  mf_head_norms_args a = *args;
+  if (a.t > MF_MAX_ROWS) return MF_ERR_INVALID_ARGUMENT;
+  if (a.head_dim == 0 || a.head_dim > 1024 || a.rotary_dim > a.head_dim || a.rotary_dim % 2 || a.q.heads > 65535 || a.k.heads > 65535) return MF_ERR_DIMENSION_MISMATCH;
+  if ((a.positions != nullptr) != (a.rotary_dim != 0) || (a.positions != nullptr) != (a.inv_freq != nullptr) || (a.axis_of_pair && !a.positions))
+    return MF_ERR_INVALID_ARGUMENT;
+  if (a.positions) {
+    if (a.axes == 0 || a.axes > 8) return MF_ERR_DIMENSION_MISMATCH;
+    if (!a.position_stride) a.position_stride = a.t;
+    if (a.axes > 1 && a.position_stride < a.t) return MF_ERR_DIMENSION_MISMATCH;
+    if (!aligned4(a.positions) || !aligned4(a.inv_freq)) return MF_ERR_INVALID_ARGUMENT;
+  }
+  HeadRows in[2], out[2];
+  uint32_t kinds = 0;
+  bool in_place[2];
+  for (mf_head_rows* h : {&a.q, &a.k}) {
+    if (h->heads == 0) continue;
+    if (!h->x || !h->out || !mf::aligned2(h->x) || !mf::aligned2(h->out) || !mf::aligned2(h->weight)) return MF_ERR_INVALID_ARGUMENT;
+    if (!h->head_stride) h->head_stride = a.head_dim;
+    if (!h->out_head_stride) h->out_head_stride = a.head_dim;
+    const uint64_t row = static_cast<uint64_t>(h->heads) * h->head_stride, out_row = static_cast<uint64_t>(h->heads) * h->out_head_stride;
+    if ((!h->row_stride && row > ~0u) || (!h->out_row_stride && out_row > ~0u)) return MF_ERR_DIMENSION_MISMATCH;
+    if (!h->row_stride) h->row_stride = static_cast<uint32_t>(row);
+    if (!h->out_row_stride) h->out_row_stride = static_cast<uint32_t>(out_row);
+    if (a.t == 0) continue;
+    if (!head_rows(h->x, h->heads, a.t, h->row_stride, h->head_stride, a.head_dim, &in[kinds]) ||
+        !head_rows(h->out, h->heads, a.t, h->out_row_stride, h->out_head_stride, a.head_dim, &out[kinds]))
+      return MF_ERR_DIMENSION_MISMATCH;
+    in_place[kinds] = h->x == h->out && (a.t == 1 || h->row_stride == h->out_row_stride) && (h->heads == 1 || h->head_stride == h->out_head_stride);
+    ++kinds;
+  }
+  if (a.t == 0 || kinds == 0) return MF_OK;
+  const uint64_t pairs = a.rotary_dim / 2;
+  const std::initializer_list<Block> read = {{a.positions, a.positions ? 4 * ((a.axes - 1ull) * a.position_stride + a.t) : 0}, {a.inv_freq, 4 * pairs},
+                        {a.axis_of_pair, a.axis_of_pair ? pairs : 0}, {a.q.heads ? a.q.weight : nullptr, 2ull * a.head_dim}, {a.k.heads ? a.k.weight : nullptr, 2ull * a.head_dim}};
+  for (uint32_t i = 0; i < kinds; ++i) {
+    if (rows_meet_any(out[i].rows, out[i].count, read)) return MF_ERR_INVALID_ARGUMENT;
+    for (uint32_t j = 0; j < kinds; ++j) {
+      if (!(i == j && in_place[i]) && heads_meet(out[i], in[j])) return MF_ERR_INVALID_ARGUMENT;
+      if (i != j && heads_meet(out[i], out[j])) return MF_ERR_INVALID_ARGUMENT;
+    }
+  }
+  const OnDevice on(ctx);
+  MF_HIP(ctx, on.error());
+  MF_HIP(ctx, mf::launch_head_norms(static_cast<hipStream_t>(stream), a));
+  return MF_OK;
+}
+
+namespace {
+
+bool expert_pool_ok(const mf_bf16_expert_pool* p) {
+  const auto width = [](uint32_t v) { return v >= 8 && v <= 1u << 20 && v % 8 == 0; };
+  return p && p->num_experts >= 1 && p->num_experts <= MF_MAX_EXPERTS && p->top_k >= 1 && p->top_k <= MF_MAX_TOPK && width(p->d) && width(p->f) &&
+         (p->shared_f == 0 || width(p->shared_f));
+}
+
+}  // namespace
+
+size_t mf_bf16_experts_workspace_bytes(const mf_bf16_expert_pool* pool, uint32_t t) {
+  return expert_pool_ok(pool) && t <= MF_BF16_EXPERTS_ROWS ? mf::bf16_experts_workspace_bytes(*pool, t) : 0;
+}
+
+mf_status mf_bf16_experts(mf_ctx* ctx, mf_stream stream, const mf_bf16_expert_pool* pool, const uint16_t* x, uint32_t x_stride,
+                          const uint32_t* idx, const float* w, const uint16_t* residual, uint32_t residual_stride, uint32_t t,
+                          uint16_t* y, uint32_t y_stride, void* workspace, size_t workspace_bytes) {
+  if (!ctx || !pool) return MF_ERR_INVALID_ARGUMENT;
+  if (!expert_pool_ok(pool)) return MF_ERR_DIMENSION_MISMATCH;
+  const mf_bf16_expert_pool& p = *pool;
+  if (!activation_ok(p.activation)) return MF_ERR_INVALID_ARGUMENT;
+  if (t > MF_BF16_EXPERTS_ROWS) return MF_ERR_QUERY_COUNT;
+  if (t == 0) return MF_OK;
+  if (!p.gate_up || !p.down || (p.shared_f && (!p.shared_gate_up || !p.shared_down)) || !x || !idx || !w || !y || !workspace) return MF_ERR_INVALID_ARGUMENT;
+  if (!mf::aligned16(p.gate_up) || !mf::aligned16(p.down) || !mf::aligned2(p.gate_up_bias) || !mf::aligned2(p.down_bias) ||
+      (p.shared_f && (!mf::aligned16(p.shared_gate_up) || !mf::aligned16(p.shared_down) || !mf::aligned2(p.shared_gate))) || !mf::aligned2(x) ||
+      !aligned4(idx) || !aligned4(w) || !mf::aligned2(residual) || !mf::aligned2(y) || !mf::aligned16(workspace))
+    return MF_ERR_INVALID_ARGUMENT;
+  mf::Bf16ExpertsArgs a{};
+  a.pool = p;
+  a.x = x;
+  a.idx = idx;
+  a.w = w;
+  a.residual = residual;
+  a.y = y;
+  a.t = t;
+  a.x_stride = x_stride ? x_stride : p.d;
+  a.residual_stride = residual_stride ? residual_stride : p.d;
+  a.y_stride = y_stride ? y_stride : p.d;
+  if (a.x_stride < p.d || a.y_stride < p.d || (residual && a.residual_stride < p.d)) return MF_ERR_DIMENSION_MISMATCH;
+  const size_t need = mf::bf16_experts_workspace_bytes(p, t);
+  if (workspace_bytes < need) return MF_ERR_SCRATCH_TOO_SMALL;
+  const uint64_t width = 2ull * p.d, e = p.num_experts, d = p.d, f = p.f, fs = p.shared_f;
+  const Rows ys = {y, 2ull * a.y_stride, width}, xs = {x, 2ull * a.x_stride, width}, rs = {residual, 2ull * a.residual_stride, width}, ws = {workspace, need, need};
+  const bool in_place = residual == y && (a.residual_stride == a.y_stride || t == 1);
+  const std::initializer_list<Block> read = {{p.gate_up, 4 * e * f * d}, {p.down, 2 * e * f * d}, {p.gate_up_bias, p.gate_up_bias ? 4 * e * f : 0}, {p.down_bias, p.down_bias ? 2 * e * d : 0},
+                        {fs ? p.shared_gate_up : nullptr, 4 * fs * d}, {fs ? p.shared_down : nullptr, 2 * fs * d}, {fs ? p.shared_gate : nullptr, 2 * d},
+                        {idx, 4ull * t * p.top_k}, {w, 4ull * t * p.top_k}};
+  if (rows_meet(ys, xs, t) || (residual && !in_place && rows_meet(ys, rs, t)) || rows_meet_any(ys, t, read) || rows_meet_any(ws, 1, read) ||
+      rows_meet_block(ys, t, workspace, need) || rows_meet_block(xs, t, workspace, need) || (residual && rows_meet_block(rs, t, workspace, need)))
+    return MF_ERR_INVALID_ARGUMENT;
+  mf::bf16_experts_layout(a, workspace);
+  const OnDevice on(ctx);
+  MF_HIP(ctx, on.error());
+  MF_HIP(ctx, mf::launch_bf16_experts(static_cast<hipStream_t>(stream), a));
   return MF_OK;
 }
 

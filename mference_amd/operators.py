@@ -18,9 +18,9 @@ import numpy as np
 import torch
 
 from . import _capi
-from ._capi import (BITS_2, BITS_4, BITS_8, BITS_TERNARY, GATE_CHANNEL, GATE_ELEMENT, GATE_NONE, GATE_ROW, GROUP_SIZE,
-                    MAX_ADAPTER_RANK, MAX_ADAPTER_TARGETS, MAX_ADAPTERS, MAX_ROWS, MAX_TOKENS,
-                    ROUTER_FULL_SOFTMAX, ROUTER_TOPK_SOFTMAX, ExpertOffsets, MfError, check)
+from ._capi import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, BF16_EXPERTS_ROWS, BITS_2, BITS_4, BITS_8, BITS_TERNARY,
+                    GATE_CHANNEL, GATE_ELEMENT, GATE_NONE, GATE_ROW, GROUP_SIZE, MAX_ADAPTER_RANK, MAX_ADAPTER_TARGETS, MAX_ADAPTERS, MAX_EXPERTS,
+                    MAX_ROWS, MAX_TOKENS, MAX_TOPK, ROUTER_FULL_SOFTMAX, ROUTER_TOPK_SOFTMAX, ExpertOffsets, MfError, check)
 
 __all__ = [
     "MetalContext", "QuantizedTensor", "Quantization", "DequantInt4GEMV", "DequantInt4GEMVMultiX",
@@ -28,6 +28,7 @@ __all__ = [
     "PrefillMoEGrouping", "PrefillTokenExpertPair", "MfError", "BITS_2", "BITS_4", "BITS_TERNARY",
     "ROUTER_TOPK_SOFTMAX", "ROUTER_FULL_SOFTMAX", "bf16_tensor", "bf16_bits",
     "AdapterGrouping", "AdapterPlan", "LowRankAdapters", "BlockNorm", "GATE_NONE", "GATE_ROW", "GATE_ELEMENT", "GATE_CHANNEL",
+    "Projection", "HeadNorms", "Bf16Experts", "ACT_NONE", "ACT_SILU", "ACT_GELU_TANH", "ACT_GELU",
 ]
 
 MoEExpertOffsets = ExpertOffsets
@@ -476,6 +477,231 @@ class BlockNorm:
         check(_capi.lib().mf_block_norm(ctx.handle, _on(ctx, stream), args), ctx.handle)
 
     _pack = Struct("@6P6I2i5f4x").pack  # mf_block_norm_args
+
+
+def _workspace(context: MetalContext, workspace: Optional[torch.Tensor], need: int, stream) -> tuple:
+    """address and size of a call's workspace: the caller's, or one of the call's stream from torch's allocator (kept by the tensor returned)"""
+    if workspace is None:
+        if need == 0:
+            return None, 0, None
+        workspace = _taken_on(context, stream, lambda: torch.empty(need, dtype=torch.uint8, device=context.device))
+    elif not workspace.is_contiguous():
+        raise MfError(-1, "the workspace must be contiguous")
+    elif workspace.get_device() != context.device.index:
+        raise ValueError("the workspace lies on another device than the context")
+    return workspace.data_ptr(), workspace.nbytes, workspace
+
+
+class Projection:
+    """mf_project: y = residual + act(x W^T + bias) of a weight kept in 16 bits (what DequantInt4GEMV and MPPPrefillInt4QMM are for
+    quantized ones), or with `gated` residual + act(x G^T + bias_g) * (x U^T + bias_u), the weight holding G's rows and then U's."""
+
+    def __init__(self, context: MetalContext, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: int = ACT_NONE,
+                 gated: bool = False):
+        """weight bf16 [m, n], gated [2 m, n]; its rows are contiguous"""
+        if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] == 0 or gated and weight.shape[0] % 2:
+            raise MfError(-2, f"weight {tuple(weight.shape)}")
+        if not ACT_NONE <= activation <= ACT_GELU:
+            raise MfError(-1, f"activation={activation}")
+        rows, self.n = weight.shape
+        self.m = rows // 2 if gated else rows
+        if self.m > 1 << 24 or self.n > 1 << 22:
+            raise MfError(-2, f"m={self.m} n={self.n}")
+        self.context, self.gated, self.activation = context, bool(gated), activation
+        self.weight, self.bias = weight, bias  # kept: the addresses stay valid
+        device = context.device.index
+        self._w, self._w_stride = _rows(weight, "weight", torch.bfloat16, device, weight.shape)
+        self._bias = None if bias is None else _vector(bias, "bias", torch.bfloat16, device, (rows,))
+
+    def workspace_bytes(self, t: int) -> int:
+        """bytes that a call of t rows, or fewer, asks for"""
+        return int(_capi.lib().mf_project_workspace_bytes(self.m, self.n, t, 1 if self.gated else 0)) if 0 <= t <= MAX_ROWS else 0
+
+    def encode(self, x: torch.Tensor, y: torch.Tensor, residual: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+               stream=None) -> None:
+        """x bf16 [t, n]; y bf16 or float32 [t, m]; residual of y's type, y itself for an update in place.  Without a workspace the call
+        takes what it needs from torch's allocator."""
+        ctx, m = self.context, self.m
+        device, t = ctx.device.index, x.shape[0]
+        dtype = y.dtype
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise ValueError(f"y must be bfloat16 or float32, not {dtype}")
+        x_ptr, x_stride = _rows(x, "x", torch.bfloat16, device, (t, self.n))
+        y_ptr, y_stride = _rows(y, "y", dtype, device, (t, m))
+        r_ptr = r_stride = 0
+        if residual is not None:
+            r_ptr, r_stride = _rows(residual, "residual", dtype, device, (t, m))
+        if t == 0:
+            return
+        if t > MAX_ROWS:
+            raise MfError(-1, f"t={t} rows are more than one call takes")
+        ws, size, _kept = _workspace(ctx, workspace, 0 if workspace is not None else self.workspace_bytes(t), stream)
+        args = self._pack(x_ptr, self._w, self._bias or 0, r_ptr, y_ptr, t, m, self.n, x_stride, self._w_stride, r_stride, y_stride,
+                          1 if dtype is torch.float32 else 0, 1 if self.gated else 0, self.activation)
+        check(_capi.lib().mf_project(ctx.handle, _on(ctx, stream), args, ws, size), ctx.handle)
+
+    _pack = Struct("@5P7I3i0P").pack  # mf_project_args
+
+
+class HeadNorms:
+    """mf_head_norms: the norms of query and key heads and their rotation by positions of one or several axes, in one launch (RMSNorm is
+    the norm of whole rows)."""
+
+    def __init__(self, context: MetalContext, head_dim: int, inv_freq: Optional[torch.Tensor] = None, axis_of_pair: Optional[torch.Tensor] = None,
+                 interleaved: bool = False, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 weight_bias: float = 0.0, rotation_scale: float = 1.0):
+        """inv_freq float32 [pairs]: the first 2 * pairs elements of a head are rotated (None: nothing is); axis_of_pair uint8 [pairs]:
+        whose position turns a pair (None: the first axis; axes_of_sections makes one); interleaved: a pair is two neighbours,
+        else one element of either half; weights bf16 [head_dim] (None: no norm)."""
+        if not 1 <= head_dim <= 1024:
+            raise MfError(-2, f"head_dim={head_dim}")
+        self.context, self.head_dim, self.interleaved = context, head_dim, bool(interleaved)
+        self.inv_freq, self.axis_of_pair, self.q_weight, self.k_weight = inv_freq, axis_of_pair, q_weight, k_weight  # kept: the addresses stay valid
+        device, pairs = context.device.index, 0 if inv_freq is None else inv_freq.numel()
+        if 2 * pairs > head_dim or inv_freq is not None and pairs == 0:
+            raise MfError(-2, f"{pairs} pairs in heads of {head_dim}")
+        if axis_of_pair is not None and inv_freq is None:
+            raise MfError(-1, "axis_of_pair without inv_freq")
+        self.rotary_dim = 2 * pairs
+        self._tables = [0 if v is None else _vector(v, name, dtype, device, (n,)) for v, name, dtype, n in (
+            (q_weight, "q_weight", torch.bfloat16, head_dim), (k_weight, "k_weight", torch.bfloat16, head_dim),
+            (inv_freq, "inv_freq", torch.float32, pairs), (axis_of_pair, "axis_of_pair", torch.uint8, pairs))]
+        self._numbers = (eps, weight_bias, rotation_scale)
+
+    @staticmethod
+    def axes_of_sections(sections: Sequence[int], turns: bool = False, device="cuda") -> torch.Tensor:
+        """axis_of_pair for axes that own so many pairs each: one section behind the other, or by turns while an axis has pairs left"""
+        left, table = [int(n) for n in sections], []
+        if not 1 <= len(left) <= 8 or min(left) < 0:
+            raise MfError(-2, f"sections {left}")
+        if not turns:
+            table = [axis for axis, n in enumerate(left) for _ in range(n)]
+        while turns and any(left):
+            for axis, n in enumerate(left):
+                if n:
+                    table.append(axis)
+                    left[axis] -= 1
+        return torch.tensor(table, dtype=torch.uint8, device=device)
+
+    def _heads(self, x: torch.Tensor, what: str, device: int, t: int, heads: int):
+        """address, row stride and head stride (0: as the library takes it by itself) of a tensor [t, heads, head_dim]"""
+        if x.shape != (t, heads, self.head_dim):
+            raise MfError(-2, f"{what} is {tuple(x.shape)}, not {(t, heads, self.head_dim)}")
+        row, head, element = x.stride()
+        if self.head_dim > 1 and element != 1:
+            raise MfError(-1, f"the heads of {what} must be contiguous")
+        row, head = (row if t > 1 else 0), (head if heads > 1 else self.head_dim)
+        if t > 1 and row < 1 or head < 1:
+            raise MfError(-2, f"the rows of {what} overlap")
+        if row > _U32 or head > _U32:
+            raise MfError(-2, f"the rows of {what} are {max(row, head)} elements apart")
+        return _address(x, what, torch.bfloat16, device), row, head
+
+    def encode(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+               q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None) -> None:
+        """q bf16 [t, heads, head_dim], k [t, kv heads, head_dim], views of a wider buffer or of any order of rows and heads among them;
+        in place without q_out / k_out.  positions int32 [t], or [axes, t]."""
+        ctx = self.context
+        device = ctx.device.index
+        if q.dim() != 3 or k is not None and k.dim() != 3:
+            raise MfError(-2, "heads must be [t, heads, head_dim]")
+        if k is None and k_out is not None:
+            raise MfError(-1, "k_out without k")
+        t = q.shape[0]
+        if t > MAX_ROWS:
+            raise MfError(-1, f"t={t} rows are more than one call takes")
+        wq, wk, freq, axes_table = self._tables
+        words = []
+        for x, out, what, weight in ((q, q_out, "q", wq), (k, k_out, "k", wk)):
+            if x is None:
+                words += (0, 0, 0, 0, 0, 0, 0, 0)
+                continue
+            heads = x.shape[1]
+            if heads > 65535:
+                raise MfError(-2, f"{heads} heads")
+            ptr, row, head = self._heads(x, what, device, t, heads)
+            o_ptr, o_row, o_head = (ptr, row, head) if out is None else self._heads(out, what + "_out", device, t, heads)
+            words += (ptr, o_ptr, weight, heads, row, head, o_row, o_head)
+        if (positions is None) != (self.rotary_dim == 0):
+            raise MfError(-1, "positions and inv_freq come together")
+        at = axes = p_stride = 0
+        if positions is not None:
+            if positions.shape[-1] != t or positions.dim() not in (1, 2):
+                raise MfError(-2, f"positions {tuple(positions.shape)} for {t} rows")
+            axes = 1 if positions.dim() == 1 else positions.shape[0]
+            if not 1 <= axes <= 8:
+                raise MfError(-2, f"{axes} axes")
+            if t > 1 and positions.stride(-1) != 1:
+                raise MfError(-1, "the positions of an axis must be contiguous")
+            p_stride = positions.stride(0) if axes > 1 else t
+            if axes > 1 and not t <= p_stride <= _U32:
+                raise MfError(-2, "the positions of the axes overlap, or are too far apart")
+            at = _address(positions, "positions", torch.int32, device)
+        if t == 0:
+            return
+        args = self._pack(*words, at, freq, axes_table, t, self.head_dim, self.rotary_dim, axes, p_stride, 1 if self.interleaved else 0, *self._numbers)
+        check(_capi.lib().mf_head_norms(ctx.handle, _on(ctx, stream), args), ctx.handle)
+
+    _pack = Struct("@3P5I4x3P5I4x3P5Ii3f0P").pack  # mf_head_norms_args
+
+
+class Bf16Experts:
+    """mf_bf16_experts: a layer of experts kept in 16 bits for a few tokens, the routed ones and the shared one, in two launches (what
+    MoE.encode_decode_layer is for quantized experts; the routing comes from MoE.encode_router or one of FamilyRouters)."""
+    max_tokens = BF16_EXPERTS_ROWS
+
+    def __init__(self, context: MetalContext, gate_up: torch.Tensor, down: torch.Tensor, top_k: int, gate_up_bias: Optional[torch.Tensor] = None,
+                 down_bias: Optional[torch.Tensor] = None, shared_gate_up: Optional[torch.Tensor] = None, shared_down: Optional[torch.Tensor] = None,
+                 shared_gate: Optional[torch.Tensor] = None, activation: int = ACT_SILU):
+        """gate_up bf16 [experts, 2 f, d] (gate rows first), down [experts, d, f], biases [experts, 2 f] and [experts, d];
+        shared_gate_up [2 shared_f, d], shared_down [d, shared_f], shared_gate [d] (its sigmoid scales the shared expert)"""
+        if gate_up.dim() != 3 or down.dim() != 3 or gate_up.shape[1] % 2 or down.shape != (gate_up.shape[0], gate_up.shape[2], gate_up.shape[1] // 2):
+            raise MfError(-2, f"gate_up {tuple(gate_up.shape)}, down {tuple(down.shape)}")
+        if (shared_gate_up is None) != (shared_down is None) or shared_gate is not None and shared_down is None:
+            raise MfError(-1, "a shared expert has both of its matrices")
+        experts, f2, d = gate_up.shape
+        fs = 0 if shared_down is None else shared_down.shape[-1]
+        if not 1 <= experts <= MAX_EXPERTS or not 1 <= top_k <= MAX_TOPK or any(v % 8 or not 8 <= v <= 1 << 20 for v in (d, f2 // 2, fs or 8)):
+            raise MfError(-2, f"experts={experts} top_k={top_k} d={d} f={f2 // 2} shared_f={fs}")
+        self.context, self.num_experts, self.top_k, self.d, self.f, self.shared_f = context, experts, top_k, d, f2 // 2, fs
+        device, bf16 = context.device.index, torch.bfloat16
+        self.tensors = (gate_up, down, gate_up_bias, down_bias, shared_gate_up, shared_down, shared_gate)  # kept: the addresses stay valid
+        shapes = ((experts, f2, d), (experts, d, f2 // 2), (experts, f2), (experts, d), (2 * fs, d), (d, fs), (d,))
+        names = ("gate_up", "down", "gate_up_bias", "down_bias", "shared_gate_up", "shared_down", "shared_gate")
+        self.pool = _capi.Bf16ExpertPool(num_experts=experts, top_k=top_k, d=d, f=f2 // 2, shared_f=fs, activation=activation)
+        for name, v, shape in zip(names, self.tensors, shapes):
+            if v is not None:
+                if v.shape != shape or not v.is_contiguous():
+                    raise MfError(-2, f"{name} must be contiguous {shape}")
+                setattr(self.pool, name, _address(v, name, bf16, device))
+        if not ACT_NONE <= activation <= ACT_GELU:
+            raise MfError(-1, f"activation={activation}")
+        self._pool = C.byref(self.pool)
+
+    def workspace_bytes(self, t: int) -> int:
+        """bytes that a call of t rows, or fewer, asks for"""
+        return int(_capi.lib().mf_bf16_experts_workspace_bytes(self._pool, t)) if 0 <= t <= BF16_EXPERTS_ROWS else 0
+
+    def encode(self, x: torch.Tensor, indices: torch.Tensor, routing_weights: torch.Tensor, y: torch.Tensor,
+               residual: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
+        """x bf16 [t, d], t <= max_tokens; indices int32 and routing_weights float32 [t, top_k]; y bf16 [t, d]; residual bf16 [t, d], y
+        itself for an update in place.  Without a workspace the call takes one from torch's allocator."""
+        ctx = self.context
+        device, t = ctx.device.index, x.shape[0]
+        shape, routes = (t, self.d), (t, self.top_k)
+        x_ptr, x_stride = _rows(x, "x", torch.bfloat16, device, shape)
+        y_ptr, y_stride = _rows(y, "y", torch.bfloat16, device, shape)
+        r_ptr = r_stride = 0
+        if residual is not None:
+            r_ptr, r_stride = _rows(residual, "residual", torch.bfloat16, device, shape)
+        idx, w = _vector(indices, "indices", torch.int32, device, routes), _vector(routing_weights, "routing_weights", torch.float32, device, routes)
+        if t == 0:
+            return
+        if t > BF16_EXPERTS_ROWS:
+            raise MfError(-10, f"t={t}: at most {BF16_EXPERTS_ROWS} rows a call")
+        ws, size, _kept = _workspace(ctx, workspace, 0 if workspace is not None else self.workspace_bytes(t), stream)
+        check(_capi.lib().mf_bf16_experts(ctx.handle, _on(ctx, stream), self._pool, x_ptr, x_stride, idx, w, r_ptr, r_stride, t, y_ptr, y_stride, ws, size),
+              ctx.handle)
 
 
 class SharedExpertInt4:
