@@ -187,6 +187,63 @@ class BlockNorm {
   mf_ctx* ctx_;
 };
 
+// A projection of 16-bit weights with bias, activation (or a gated pair) and residual in the same launch.
+class Projection {
+ public:
+  // weight [m, n], gated [2 m, n]
+  Projection(const MetalContext& context, const uint16_t* weight, uint32_t m, uint32_t n, const uint16_t* bias = nullptr,
+             mf_activation activation = MF_ACT_NONE, bool gated = false)
+      : ctx_(context.raw()) {
+    fixed_.w = weight, fixed_.m = m, fixed_.n = n, fixed_.bias = bias, fixed_.activation = activation, fixed_.gated = gated ? 1 : 0;
+  }
+  size_t workspaceBytes(uint32_t t) const { return mf_project_workspace_bytes(fixed_.m, fixed_.n, t, fixed_.gated); }
+  // rows one behind the other where a stride is 0
+  void encode(mf_stream cb, const uint16_t* x, uint32_t t, void* y, bool float32 = false, const void* residual = nullptr,
+              void* workspace = nullptr, size_t workspaceBytes = 0, uint32_t xStride = 0, uint32_t yStride = 0,
+              uint32_t residualStride = 0) const {
+    mf_project_args a = fixed_;
+    a.x = x, a.t = t, a.y = y, a.y_f32 = float32 ? 1 : 0, a.residual = residual;
+    a.x_stride = xStride, a.y_stride = yStride, a.residual_stride = residualStride;
+    check(mf_project(ctx_, cb, &a, workspace, workspaceBytes), ctx_);
+  }
+
+ private:
+  mf_ctx* ctx_;
+  mf_project_args fixed_{};
+};
+
+// The norms of query and key heads and their rotation by positions of one or several axes.
+class HeadNorms {
+ public:
+  explicit HeadNorms(const MetalContext& context) : ctx_(context.raw()) {}
+  // arguments that change nothing beside what is set in them: rows of heads in place, no keys, no rotation
+  static mf_head_norms_args arguments(uint16_t* q, uint32_t heads, uint32_t t, uint32_t headDim, const uint16_t* weight, float eps) {
+    mf_head_norms_args a{};
+    a.q.x = a.q.out = q, a.q.heads = heads, a.q.weight = weight;
+    a.t = t, a.head_dim = headDim, a.eps = eps, a.rotation_scale = 1.0f;
+    return a;
+  }
+  void encode(mf_stream cb, const mf_head_norms_args& args) const { check(mf_head_norms(ctx_, cb, &args), ctx_); }
+
+ private:
+  mf_ctx* ctx_;
+};
+
+// A layer of 16-bit experts for up to MF_BF16_EXPERTS_ROWS tokens, routed by MoE or one of the family routers.
+class Bf16Experts {
+ public:
+  Bf16Experts(const MetalContext& context, const mf_bf16_expert_pool& pool) : ctx_(context.raw()), pool_(pool) {}
+  size_t workspaceBytes(uint32_t t) const { return mf_bf16_experts_workspace_bytes(&pool_, t); }
+  void encode(mf_stream cb, const uint16_t* x, const uint32_t* indices, const float* routingWeights, uint32_t t, uint16_t* y, const uint16_t* residual,
+              void* workspace, size_t workspaceBytes, uint32_t xStride = 0, uint32_t yStride = 0, uint32_t residualStride = 0) const {
+    check(mf_bf16_experts(ctx_, cb, &pool_, x, xStride, indices, routingWeights, residual, residualStride, t, y, yStride, workspace, workspaceBytes), ctx_);
+  }
+
+ private:
+  mf_ctx* ctx_;
+  mf_bf16_expert_pool pool_;
+};
+
 // The router calls of MoEDeepseekV4 (Kernels/MoE/MoEDeepseekV4.swift:92-151): learned top-k on
 // sqrt(softplus(logit)) + correction bias, and weighting of hash-routed experts.  routeScale is the
 // operator's constant as in the reference (:31-87); `logits` fp32 [tokens, numExperts] stands in for

@@ -22,8 +22,6 @@ struct Bf16ExpertsArgs {
   uint16_t* y;
   uint32_t t, x_stride, residual_stride, y_stride;
   // the workspace
-  uint32_t* plan;      // [0]: live experts; then for each of them {expert, first route, routes, 0}, from word 4 on
-  uint32_t* routes;    // [t * top_k]: route numbers by live expert
   float* shared_gate;  // [t]: logits of the shared expert's gate
   uint16_t* acts;      // [2][routes, f]: what is left of the activations' 32 bits in two bf16 terms, one plane each
   uint16_t* shared_acts;  // [2][t, shared_f]
