@@ -14,33 +14,38 @@ constexpr uint32_t kRoutes = MF_BF16_EXPERTS_ROWS * MF_MAX_TOPK;
 // names them; beyond 64 routes in the order of their numbers, by a workgroup.  Both launches find them for themselves, which costs less than handing them over.
 constexpr uint32_t kFew = 64;
 
-// calls found(number, expert, lanes of its routes) for every live expert until it returns true (e: the lane's expert, or one that is none)
+// calls found(expert, lanes of its routes) for every live expert until it returns true (e: the lane's expert, or one that is none)
 template <class Found>
 __device__ __forceinline__ void each_live(uint32_t e, uint32_t num_experts, Found found) {
   uint64_t left = __ballot(e < num_experts);
-  for (uint32_t number = 0; left; ++number) {
+  while (left) {
     const uint32_t expert = __builtin_amdgcn_readlane(e, __ffsll(static_cast<unsigned long long>(left)) - 1);
     const uint64_t mine = __ballot(e == expert);
-    if (found(number, expert, mine)) return;
+    if (found(expert, mine)) return;
     left &= ~mine;
   }
 }
 
 // ------------------------------------------------------------------ activations
 
-constexpr uint32_t kUpWaves = 4, kUpStages = 3;
+constexpr uint32_t kUpWaves = 4, kUpStages = 2;
 
-// The first launch: activations of 16 gate and 16 up rows of one live expert (blockIdx.y: which), or of the shared one, for all of its routes, eight (XI = 2: 16) at
-// a time.  The call is the rows' stream; the waves share the sum over d.
+// The first launch: activations of 16 gate and 16 up rows of one live expert, or of the shared one, for eight (XI = 2: 16) of its routes: a tile (blockIdx.y).  Work is
+// the reading of W, rows of d in 128-byte lines, so a workgroup's waves share d between them and each streams its part of the 32 rows through a ring of two stages in LDS; the
+// matrix cores' sums meet in LDS.  What bounds it is the memory: 206 MB in 46 us (8 tokens, 23 live experts of 704 x 2816 beside a shared one of 2112; 4.5 TB/s), 218 MB in 58 us where
+// popular experts have several tiles, which read their rows again (61 tokens, 26 live of 1024 x 2048), 17.8 MB in 9 us (one token), where the way to the expert's number and the
+// first lines take most of it.  Measured beside it: three stages 49, 69 and 10.4 us, fewer workgroups fitting on a unit; waves with 16 + 16 rows of their own and all of d, 59 and 77 us;
+// an expert's tiles one after the other in a workgroup, 68 us at 61 tokens.
 template <int XI, bool ALIGNED>
 __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16ExpertsArgs a) {
   constexpr int kLoads = 4 + XI, kRing = kUpStages * kLoads * 64;
+  constexpr uint32_t kTile = 8 * XI;
   __shared__ uint4 rings[kUpWaves * kRing];
-  __shared__ uint32_t bits[MF_MAX_EXPERTS / 32], list[kRoutes], counts[2];
+  __shared__ uint32_t hist[MF_MAX_EXPERTS], list[kRoutes], sums[kRoutes / 64], found[3];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
-  const uint32_t most = a.most_live(), routes = a.route_count(), d = a.pool.d;
+  const uint32_t most = a.most_tiles(kTile), routes = a.route_count(), d = a.pool.d, shared_tiles = a.pool.shared_f ? (a.t + kTile - 1) / kTile : 0;
   float* part = reinterpret_cast<float*>(rings);
-  if (blockIdx.y > most) {  // the shared expert's gate, a token a workgroup
+  if (blockIdx.y >= most + shared_tiles) {  // the shared expert's gate, a token a workgroup
     for (uint32_t i = blockIdx.x; i < a.t; i += gridDim.x) {
       const uint16_t* x = a.x + static_cast<size_t>(i) * a.x_stride;
       float v = 0.0f;
@@ -53,65 +58,99 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
     }
     return;
   }
-  const bool shared = blockIdx.y == most;
-  const uint32_t f = shared ? a.pool.shared_f : a.pool.f, j0 = blockIdx.x * 16;
+  const bool shared = blockIdx.y >= most;
+  const uint32_t f = shared ? a.pool.shared_f : a.pool.f;
+  const uint32_t j0 = blockIdx.x * 16;
   if (j0 >= f) return;
-  uint32_t expert = ~0u, count = a.t;
+  uint32_t expert = ~0u, count = a.t, base = (blockIdx.y - most) * kTile;
   if (shared) {
     if (tid < a.t) list[tid] = tid;
     expert = 0;
   } else if (routes <= kFew) {
     const uint32_t e = lane < routes ? a.idx[lane] : ~0u;
-    each_live(e, a.pool.num_experts, [&](uint32_t number, uint32_t live, uint64_t mine) {
-      if (number < blockIdx.y) return false;
-      expert = live;
+    uint32_t tile = 0;
+    each_live(e, a.pool.num_experts, [&](uint32_t live, uint64_t mine) {
       count = __popcll(mine);
+      base = (blockIdx.y - tile) * kTile;
+      tile += (count + kTile - 1) / kTile;
+      if (tile <= blockIdx.y) return false;
+      expert = live;
       if (wave == 0 && e == live) list[lanes_in_front(mine)] = lane;
       return true;
     });
     if (expert == ~0u) return;
   } else {
-    if (tid < MF_MAX_EXPERTS / 32) bits[tid] = 0;
-    if (tid == 0) counts[0] = 0;
+    constexpr uint32_t kThreads = 64 * kUpWaves, kEach = MF_MAX_EXPERTS / kThreads, kTurns = kRoutes / kThreads;
+    static_assert(kEach * kThreads == MF_MAX_EXPERTS && kTurns * kThreads == kRoutes, "the threads share out experts and routes");
+    for (uint32_t k = tid; k < MF_MAX_EXPERTS; k += kThreads) hist[k] = 0;
+    if (tid == 0) found[0] = ~0u;
     __syncthreads();
-    uint32_t e[kRoutes / (64 * kUpWaves)];
+    uint32_t e[kTurns];
 #pragma unroll
-    for (uint32_t k = 0; k < kRoutes / (64 * kUpWaves); ++k) {
-      const uint32_t route = k * 64 * kUpWaves + tid;
+    for (uint32_t k = 0; k < kTurns; ++k) {
+      const uint32_t route = k * kThreads + tid;
       e[k] = route < routes ? a.idx[route] : ~0u;
-      if (e[k] < a.pool.num_experts) atomicOr(&bits[e[k] / 32], 1u << (e[k] & 31));
+      if (e[k] < a.pool.num_experts) atomicAdd(&hist[e[k]], 1u);
     }
     __syncthreads();
-    uint32_t live = 0;
-    for (uint32_t w = 0; w < MF_MAX_EXPERTS / 32; ++w) {
-      uint32_t word = bits[w];
-      const uint32_t here = __popc(word);
-      if (blockIdx.y >= live && blockIdx.y < live + here) {
-        for (uint32_t skip = blockIdx.y - live; skip; --skip) word &= word - 1;
-        expert = w * 32 + __ffs(static_cast<int>(word)) - 1;
-      }
-      live += here;
-    }
-    if (expert == ~0u) return;
-    // (the order of an expert's routes changes no result: each is a column of its own)
+    uint32_t tiles = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < kRoutes / (64 * kUpWaves); ++k)
-      if (e[k] == expert) list[atomicAdd(&counts[0], 1u)] = k * 64 * kUpWaves + tid;
+    for (uint32_t k = 0; k < kEach; ++k) tiles += (hist[tid * kEach + k] + kTile - 1) / kTile;
+    uint32_t tile = tiles;
+#pragma unroll
+    for (uint32_t s = 1; s < 64; s *= 2) {
+      const uint32_t v = __shfl_up(tile, s);
+      if (lane >= s) tile += v;
+    }
+    if (lane == 63) sums[wave] = tile;
     __syncthreads();
-    count = counts[0];
+    tile -= tiles;
+    for (uint32_t w = 0; w < wave; ++w) tile += sums[w];
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t here = hist[tid * kEach + k], own = (here + kTile - 1) / kTile;
+      if (blockIdx.y >= tile && blockIdx.y < tile + own) found[0] = tid * kEach + k, found[1] = here, found[2] = (blockIdx.y - tile) * kTile;
+      tile += own;
+    }
+    __syncthreads();
+    expert = found[0];
+    if (expert == ~0u) return;
+    count = found[1];
+    base = found[2];
+    // an expert's routes in the order of their numbers: its tiles are other workgroups' too
+#pragma unroll
+    for (uint32_t k = 0; k < kTurns; ++k) {
+      const uint64_t mine = __ballot(e[k] == expert);
+      if (lane == 0) sums[k * kUpWaves + wave] = __popcll(mine);
+    }
+    __syncthreads();
+    uint32_t at = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kTurns; ++k) {
+      const uint64_t mine = __ballot(e[k] == expert);
+      uint32_t first = at;
+      for (uint32_t w = 0; w < kUpWaves; ++w) {
+        if (w < wave) first += sums[k * kUpWaves + w];
+        at += sums[k * kUpWaves + w];
+      }
+      if (e[k] == expert) list[first + lanes_in_front(mine)] = k * kThreads + tid;
+    }
   }
   __syncthreads();
   expert = __builtin_amdgcn_readfirstlane(expert);
   count = __builtin_amdgcn_readfirstlane(count);
+  base = __builtin_amdgcn_readfirstlane(base);
   const uint32_t share = ((d + 63) / 64 + kUpWaves - 1) / kUpWaves, from = min(wave * share * 64, d), to = min(from + share * 64, d), begin = to > from ? from : 0;
-  const uint16_t* w = (shared ? a.pool.shared_gate_up : a.pool.gate_up + static_cast<size_t>(expert) * 2 * f * d) + static_cast<size_t>(j0) * d + begin;
+  const uint16_t* matrix = (shared ? a.pool.shared_gate_up : a.pool.gate_up + static_cast<size_t>(expert) * 2 * f * d) + begin;
   const uint16_t* bias = shared || !a.pool.gate_up_bias ? nullptr : a.pool.gate_up_bias + static_cast<size_t>(expert) * 2 * f;
   uint16_t* acts = shared ? a.shared_acts : a.acts;
   const size_t plane = static_cast<size_t>(shared ? a.t : routes) * f;
-  for (uint32_t base = 0; base < count; base += 8 * XI) {
-    RowAt<ALIGNED> at[kLoads];
+  // eight or 16 routes through 16 + 16 rows
+  const auto rows_of = [&](auto columns) {
+    constexpr int kX = decltype(columns)::value, kN = 4 + kX;
+    RowAt<ALIGNED> at[kN];
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
+    for (int q = 0; q < kN; ++q) {
       const uint32_t row = q % 2 * 8 + lane / 8;
       if (q < 4) {
         at[q] = (static_cast<RowAt<ALIGNED>>(min(row, f - 1 - j0)) * d + lane_piece(lane)) * 2;
@@ -120,14 +159,15 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
         at[q] = (static_cast<RowAt<ALIGNED>>(token) * a.x_stride + lane_piece(lane)) * 2;
       }
     }
+    const uint16_t* w = matrix + static_cast<size_t>(j0) * d;
     f32x4_t zg = {}, zu = {};
-    stream_rows<true, ALIGNED, kUpStages, XI>(w, w + static_cast<size_t>(f) * d, a.x + begin, at, to - from, rings + wave * kRing, zg, zu);
+    stream_rows<true, ALIGNED, kUpStages, kX>(w, w + static_cast<size_t>(f) * d, a.x + begin, at, to - from, rings + wave * kRing, zg, zu);
     __syncthreads();
     *reinterpret_cast<f32x4_t*>(part + wave * 512 + r * 16 + g * 4) = zg;
     *reinterpret_cast<f32x4_t*>(part + wave * 512 + 256 + r * 16 + g * 4) = zu;
     __syncthreads();
     const uint32_t column = tid / 16, j = j0 + tid % 16;
-    if (column < 8 * XI && base + column < count && j < f) {
+    if (column < 8 * kX && base + column < count && j < f) {
       float gate = 0.0f, up = 0.0f;
 #pragma unroll
       for (uint32_t v = 0; v < kUpWaves; ++v) gate += part[v * 512 + tid], up += part[v * 512 + 256 + tid];
@@ -138,32 +178,49 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
       acts[to_at] = high;
       acts[plane + to_at] = narrow_bf16(__builtin_isfinite(bf16_to_f(high)) ? act - bf16_to_f(high) : 0.0f);
     }
-    __syncthreads();
-  }
+  };
+  if (XI == 2 && count - base > 8) rows_of(std::integral_constant<int, 2>{});
+  else rows_of(std::integral_constant<int, 1>{});
 }
 
 // ------------------------------------------------------------------ results
 
-constexpr uint32_t kDownWaves = 8;
+// How the second launch is cut: rows of a workgroup; the sums over f in parts that a workgroup's waves share, or, where there are several groups, one for each group
+// (their sums of a token meet in a third launch).
+struct DownCut {
+  uint32_t rows, routed_blocks, shared_blocks, parts, groups;  // (blocks: of 64 of f, in a part)
+};
 
-// The second launch: ROWS results of every token.  The work is cut into items, the rows of one expert's down matrix times up to 8 XI of its routes over a part of f, dealt to the
-// waves; a wave's items are one stream through its ring.  Every route's sum goes to LDS, and the weighted sums over a token's routes are made there in the
-// order of their ranks, the parts of a sum in theirs.
-template <int ROWS, int XI, int STAGES>
-__global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf16ExpertsArgs a, uint32_t part_blocks, uint32_t parts) {
-  constexpr uint32_t kW = ROWS / 8, kLoads = kW + 2 * XI, kStage = kLoads * 64, kTile = 8 * XI;
+// The result of token i's row j from what the routed experts gave it.
+__device__ __forceinline__ void finish_token(const Bf16ExpertsArgs& a, uint32_t i, uint32_t j, float v) {
+  if (a.residual) v += bf16_to_f(a.residual[static_cast<size_t>(i) * a.residual_stride + j]);
+  a.y[static_cast<size_t>(i) * a.y_stride + j] = narrow_bf16(v);
+}
+
+// The second launch: up to ROWS results of every token.  The work is cut into items, the rows of one expert's down matrix times up to 8 XI of its routes over a part of f,
+// dealt to a workgroup's waves; a wave's items are one stream through its ring in LDS, whose requests run over an item's end into the next.  Every route's sum goes to LDS, and the
+// weighted sums over a token's routes are made there in the order of their ranks, the parts of a sum in theirs: no atomics, so calls repeat to the bit.
+// The activations come as two bf16 terms (32 bits narrowed to 16 would cost the layer half a step more than the result's own rounding).  What bounds it: 103 MB in 29 us
+// (8 tokens, d 2816: 256 workgroups of 11 rows; 176 of 16 took 47), 109 MB in 46 us (61 tokens), where LDS holds all routes' sums and rings of two stages, too few bytes on their
+// way for more than 3.8 TB/s with the rows that several tiles read; 9.4 MB in 10 us (one token), latency: idx, then the rows, then the sums.
+template <int ROWS, int XI, int STAGES, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16ExpertsArgs a, const DownCut cut) {
+  constexpr uint32_t kW = ROWS / 8, kLoads = kW + 2 * XI, kStage = kLoads * 64, kTile = 8 * XI, kM = (ROWS + 15) / 16, kThreads = 64 * WAVES;
   extern __shared__ uint4 whole_lds[];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
-  const uint32_t d = a.pool.d, routes = a.route_count(), shared_rows = a.pool.shared_f ? a.t : 0, rows = routes + shared_rows, j0 = blockIdx.x * ROWS;
-  float* sums = reinterpret_cast<float*>(whole_lds + kDownWaves * STAGES * kStage);          // [parts][rows][ROWS]
-  uint32_t* list = reinterpret_cast<uint32_t*>(sums + static_cast<size_t>(parts) * rows * ROWS);  // [routes]: by tile
-  uint2* tiles = reinterpret_cast<uint2*>(list + (routes + 1) / 2 * 2);                      // expert | routes << 16, first; at most `routes` of them
-  __shared__ uint32_t tile_count, hist[MF_MAX_EXPERTS], wave_sums[2][kDownWaves];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4, group = blockIdx.y;
+  const uint32_t d = a.pool.d, routes = a.route_count(), shared_rows = a.pool.shared_f ? a.t : 0, rows = routes + shared_rows, j0 = blockIdx.x * cut.rows, own_rows = min(cut.rows, d - j0);
+  float* sums = reinterpret_cast<float*>(whole_lds + WAVES * STAGES * kStage);                      // [parts][rows][ROWS]
+  uint32_t* list = reinterpret_cast<uint32_t*>(sums + static_cast<size_t>(cut.parts) * rows * ROWS);  // [routes]: by tile
+  uint2* tiles = reinterpret_cast<uint2*>(list + (routes + 1) / 2 * 2);                             // expert | routes << 16, first; at most `routes` of them
+  uint2* named = tiles + routes;                                                                    // [routes]: expert, weight
+  uint2* table = named + routes;                                                                    // a group's items: expert | routes << 16 | part << 24, first
+  __shared__ uint32_t tile_count, hist[MF_MAX_EXPERTS], wave_sums[2][WAVES];
+  for (uint32_t k = tid; k < routes; k += kThreads) named[k] = make_uint2(a.idx[k], __float_as_uint(a.w[k]));
   if (routes <= kFew) {
     if (wave == 0) {
       const uint32_t e = lane < routes ? a.idx[lane] : ~0u;
       uint32_t first = 0, n = 0;
-      each_live(e, a.pool.num_experts, [&](uint32_t, uint32_t live, uint64_t mine) {
+      each_live(e, a.pool.num_experts, [&](uint32_t live, uint64_t mine) {
         const uint32_t count = __popcll(mine);
         if (e == live) list[first + lanes_in_front(mine)] = lane;
         for (uint32_t k = 0; k < count; k += kTile, ++n)
@@ -174,15 +231,24 @@ __global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf1
       if (lane == 0) tile_count = n;
     }
   } else {
-    // a thread an expert and a route
-    static_assert(64 * kDownWaves >= MF_MAX_EXPERTS && 64 * kDownWaves >= kRoutes, "a thread each");
-    const uint32_t e = tid < routes ? a.idx[tid] : ~0u;
-    hist[tid] = 0;
+    // a thread two neighbouring experts (or one)
+    constexpr uint32_t kEach = MF_MAX_EXPERTS / kThreads;
+    static_assert(kEach * kThreads == MF_MAX_EXPERTS, "the threads share out the experts");
+    for (uint32_t k = tid; k < MF_MAX_EXPERTS; k += kThreads) hist[k] = 0;
     __syncthreads();
-    if (e < a.pool.num_experts) atomicAdd(&hist[e], 1u);
+    for (uint32_t k = tid; k < routes; k += kThreads) {
+      const uint32_t e = a.idx[k];
+      if (e < a.pool.num_experts) atomicAdd(&hist[e], 1u);
+    }
     __syncthreads();
-    const uint32_t count = hist[tid], mine = (count + kTile - 1) / kTile;
-    uint32_t first = count, tile = mine;
+    uint32_t count[kEach], all = 0, all_tiles = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      count[k] = hist[tid * kEach + k];
+      all += count[k];
+      all_tiles += (count[k] + kTile - 1) / kTile;
+    }
+    uint32_t first = all, tile = all_tiles;
 #pragma unroll
     for (uint32_t s = 1; s < 64; s *= 2) {
       const uint32_t c = __shfl_up(first, s), t = __shfl_up(tile, s);
@@ -190,51 +256,56 @@ __global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf1
     }
     if (lane == 63) wave_sums[0][wave] = first, wave_sums[1][wave] = tile;
     __syncthreads();
-    first -= count;
-    tile -= mine;
+    first -= all;
+    tile -= all_tiles;
     for (uint32_t w = 0; w < wave; ++w) first += wave_sums[0][w], tile += wave_sums[1][w];
-    for (uint32_t k = 0; k < mine; ++k) tiles[tile + k] = make_uint2(tid | min(count - k * kTile, kTile) << 16, first + k * kTile);
-    if (tid == 64 * kDownWaves - 1) tile_count = tile + mine;
-    hist[tid] = first;  // (from here on: where the next route of the expert goes; their order changes no result)
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+      const uint32_t e = tid * kEach + k;
+      for (uint32_t c = 0; c < count[k]; c += kTile) tiles[tile++] = make_uint2(e | min(count[k] - c, kTile) << 16, first + c);
+      hist[e] = first;  // (from here on: where the next route of the expert goes; their order changes no result)
+      first += count[k];
+    }
+    if (tid == kThreads - 1) tile_count = tile;
     __syncthreads();
-    if (e < a.pool.num_experts) list[atomicAdd(&hist[e], 1u)] = tid;
+    for (uint32_t k = tid; k < routes; k += kThreads) {
+      const uint32_t e = a.idx[k];
+      if (e < a.pool.num_experts) list[atomicAdd(&hist[e], 1u)] = k;
+    }
   }
   __syncthreads();
-  // items: the shared expert's first (its f may be the longest), then the tiles of routes
-  const uint32_t shared_tiles = (shared_rows + kTile - 1) / kTile, shared_blocks = (a.pool.shared_f + 63) / 64, routed_blocks = (a.pool.f + 63) / 64;
-  const uint32_t shared_parts = (shared_blocks + part_blocks - 1) / part_blocks, routed_parts = (routed_blocks + part_blocks - 1) / part_blocks;
-  const uint32_t shared_items = shared_tiles * shared_parts, items = shared_items + __builtin_amdgcn_readfirstlane(tile_count) * routed_parts;
+  // items: the shared expert's first (its f may be the longest), then the tiles of routes; a tile's parts side by side
+  const bool one = cut.groups == 1;
+  const auto parts_of = [&](uint32_t f, uint32_t blocks) { return one ? (f + blocks * 64 - 1) / (blocks * 64) : group * blocks * 64 < f ? 1u : 0u; };
+  const uint32_t shared_parts = parts_of(a.pool.shared_f, cut.shared_blocks), routed_parts = parts_of(a.pool.f, cut.routed_blocks);
+  const uint32_t shared_items = (shared_rows + kTile - 1) / kTile * shared_parts, items = shared_items + __builtin_amdgcn_readfirstlane(tile_count) * routed_parts;
   struct Item {
     const uint16_t *w, *act, *low;  // down rows; the activations' two terms
-    uint32_t f, first, blocks, count, from, part;
+    uint32_t f, first, blocks, count, left, part;
     bool shared;
   };
+  for (uint32_t n = tid; n < items; n += kThreads) {
+    const bool shared = n < shared_items;
+    const uint32_t in = shared ? n : n - shared_items, per = shared ? shared_parts : routed_parts, part = in % per, first = in / per * kTile;
+    const uint2 it = shared ? make_uint2(min(shared_rows - first, kTile) << 16, first) : tiles[in / per];
+    table[n] = make_uint2(it.x | part << 24, it.y);
+  }
+  __syncthreads();
   const auto item_of = [&](uint32_t n) {
+    const uint2 e = table[n];
+    const uint32_t who = __builtin_amdgcn_readfirstlane(e.x), expert = who & 0xFFFF;
     Item it;
+    it.first = __builtin_amdgcn_readfirstlane(e.y);
+    it.count = who >> 16 & 0xFF;
+    it.part = who >> 24;
     it.shared = n < shared_items;
-    const uint32_t in = it.shared ? n : n - shared_items, per = it.shared ? shared_parts : routed_parts, tile = in / per;
-    it.part = in % per;
     it.f = it.shared ? a.pool.shared_f : a.pool.f;
-    it.from = it.part * part_blocks * 64;
-    it.blocks = (min(it.f - it.from, part_blocks * 64) + 63) / 64;
-    if (it.shared) {
-      it.first = tile * kTile;
-      it.count = min(a.t - it.first, kTile);
-      it.w = a.pool.shared_down;
-      it.act = a.shared_acts;
-      it.low = it.act + static_cast<size_t>(a.t) * it.f;
-    } else {
-      const uint2 t = tiles[tile];
-      const uint32_t who = __builtin_amdgcn_readfirstlane(t.x);
-      it.first = __builtin_amdgcn_readfirstlane(t.y);
-      it.count = who >> 16;
-      it.w = a.pool.down + static_cast<size_t>(who & 0xFFFF) * d * it.f;
-      it.act = a.acts;
-      it.low = it.act + static_cast<size_t>(routes) * it.f;
-    }
-    it.w = uniform(it.w + static_cast<size_t>(j0) * it.f + it.from);
-    it.act = uniform(it.act + it.from);
-    it.low = uniform(it.low + it.from);
+    const uint32_t blocks = it.shared ? cut.shared_blocks : cut.routed_blocks, from = (one ? it.part : group) * blocks * 64;
+    it.left = it.f - from;
+    it.blocks = (min(it.left, blocks * 64) + 63) / 64;
+    it.w = (it.shared ? a.pool.shared_down : a.pool.down) + (static_cast<size_t>(expert) * d + j0) * it.f + from;
+    it.act = (it.shared ? a.shared_acts : a.acts) + from;
+    it.low = it.act + static_cast<size_t>(it.shared ? a.t : routes) * it.f;
     return it;
   };
   const auto route_of = [&](const Item& it, uint32_t column) {
@@ -243,28 +314,28 @@ __global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf1
   };
   // the requests' place in the stream runs ahead of the products'
   const uint32_t ring = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(whole_lds))) + wave * STAGES * kStage * 16, piece = lane_piece(lane);
-  uint32_t ask_item = wave, ask_block = 0, at[kW + XI];
+  uint32_t ask_item = wave, ask_block = 0, w_at[kW], act_at[XI];
   Item ask{};
   const auto ask_next = [&] {
     ask = item_of(ask_item);
 #pragma unroll
-    for (uint32_t q = 0; q < kW; ++q) at[q] = (min(q * 8 + lane / 8, d - 1 - j0) * ask.f + piece) * 2;
+    for (uint32_t q = 0; q < kW; ++q) w_at[q] = (min(q * 8 + lane / 8, own_rows - 1) * ask.f + piece) * 2;
 #pragma unroll
-    for (uint32_t q = 0; q < XI; ++q) at[kW + q] = (route_of(ask, q * 8 + lane / 8) * ask.f + piece) * 2;
+    for (uint32_t q = 0; q < XI; ++q) act_at[q] = (route_of(ask, q * 8 + lane / 8) * ask.f + piece) * 2;
   };
   const auto request = [&](uint32_t stage) {
-    const uint32_t k = ask_block * 64, left = ask.f - ask.from - k;  // (of the row: 64 and more but in its last block)
+    const uint32_t k = __builtin_amdgcn_readfirstlane(ask_block * 64), left = ask.left - k;  // (of the row: 64 and more but in its last block)
     const uint32_t back = piece >= left ? piece * 2 : 0, to = ring + stage * kStage * 16;
 #pragma unroll
-    for (uint32_t q = 0; q < kW; ++q) load_to_lds_from(ask.w + k, at[q] - back, to + q * 1024);
+    for (uint32_t q = 0; q < kW; ++q) load_to_lds_from(uniform(ask.w + k), w_at[q] - back, to + q * 1024);
 #pragma unroll
     for (uint32_t q = 0; q < XI; ++q) {
-      load_to_lds_from(ask.act + k, at[kW + q] - back, to + (kW + q) * 1024);
-      load_to_lds_from(ask.low + k, at[kW + q] - back, to + (kW + XI + q) * 1024);
+      load_to_lds_from(uniform(ask.act + k), act_at[q] - back, to + (kW + q) * 1024);
+      load_to_lds_from(uniform(ask.low + k), act_at[q] - back, to + (kW + XI + q) * 1024);
     }
     if (++ask_block < ask.blocks) return;
-    if (ask_item + kDownWaves < items) {
-      ask_item += kDownWaves;
+    if (ask_item + WAVES < items) {
+      ask_item += WAVES;
       ask_block = 0;
       ask_next();
     } else {
@@ -272,49 +343,56 @@ __global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf1
     }
   };
   if (wave < items) {
-    const uint32_t mine = ROWS == 16 ? place_of(r, g) : place_of(r & 7, g), mine_x = XI == 2 ? place_of(r, g) : place_of(r & 7, g);
+    const uint32_t mine = ROWS >= 16 ? place_of(r, g) : place_of(r & 7, g), mine_x = XI == 2 ? place_of(r, g) : place_of(r & 7, g);
     ask_next();
 #pragma unroll
     for (uint32_t s = 0; s < STAGES; ++s) request(s);
     uint32_t item = wave, block = 0;
     Item now = item_of(item);
-    f32x4_t sum = {};
+    f32x4_t sum[kM] = {};
     for (bool more = true; more;) {
 #pragma unroll
       for (uint32_t s = 0; s < STAGES; ++s) {
         if (!more) break;
         const uint4* stage = whole_lds + wave * STAGES * kStage + s * kStage;
         wait_loads<(STAGES - 1) * kLoads>();
-        uint4 fw[2], fh[2], fl[2];
+        uint4 fw[kM][2], fh[2], fl[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          fw[h] = stage[mine ^ h * 4];
+#pragma unroll
+          for (uint32_t m = 0; m < kM; ++m) fw[m][h] = stage[m * 128 + (mine ^ h * 4)];
           fh[h] = stage[kW * 64 + (mine_x ^ h * 4)];
           fl[h] = stage[(kW + XI) * 64 + (mine_x ^ h * 4)];
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read
         request(s);
-        const uint32_t left = now.f - now.from - block * 64;
+        const uint32_t left = now.left - block * 64;
         if (left < 64) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t keep = (h * 4 + g) * 8 < left ? ~0u : 0u;
-            fw[h] = masked(fw[h], keep);
+#pragma unroll
+            for (uint32_t m = 0; m < kM; ++m) fw[m][h] = masked(fw[m][h], keep);
             fh[h] = masked(fh[h], keep);
             fl[h] = masked(fl[h], keep);
           }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          sum = mfma16(fw[h], fh[h], sum);
-          sum = mfma16(fw[h], fl[h], sum);
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (uint32_t m = 0; m < kM; ++m) {
+            sum[m] = mfma16(fw[m][h], fh[h], sum[m]);
+            sum[m] = mfma16(fw[m][h], fl[h], sum[m]);
+          }
         if (++block < now.blocks) continue;
-        if (r < now.count && g * 4 < ROWS)
-          *reinterpret_cast<f32x4_t*>(sums + (static_cast<size_t>(now.part) * rows + (now.shared ? routes : 0) + route_of(now, r)) * ROWS + g * 4) = sum;
-        sum = f32x4_t{};
+        float* out = sums + (static_cast<size_t>(now.part) * rows + (now.shared ? routes : 0) + route_of(now, r)) * ROWS + g * 4;
+#pragma unroll
+        for (uint32_t m = 0; m < kM; ++m) {
+          if (r < now.count && g * 4 < ROWS) *reinterpret_cast<f32x4_t*>(out + m * 16) = sum[m];
+          sum[m] = f32x4_t{};
+        }
         block = 0;
-        item += kDownWaves;
+        item += WAVES;
         more = item < items;
         if (more) now = item_of(item);
       }
@@ -322,17 +400,26 @@ __global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf1
     wait_loads<0>();
   }
   __syncthreads();
-  for (uint32_t o = tid; o < a.t * ROWS; o += 64 * kDownWaves) {
+  for (uint32_t o = tid; o < a.t * ROWS; o += kThreads) {
     const uint32_t i = o / ROWS, row = o % ROWS, j = j0 + row;
-    if (j >= d) continue;
-    float v = a.residual ? bf16_to_f(a.residual[static_cast<size_t>(i) * a.residual_stride + j]) : 0.0f;
-    for (uint32_t k = 0; k < a.pool.top_k; ++k) {
-      const uint32_t route = i * a.pool.top_k + k, e = a.idx[route];
-      if (e >= a.pool.num_experts) continue;
-      float z = 0.0f;
-      for (uint32_t p = 0; p < routed_parts; ++p) z += sums[(static_cast<size_t>(p) * rows + route) * ROWS + row];
-      if (a.pool.down_bias) z += bf16_to_f(a.pool.down_bias[static_cast<size_t>(e) * d + j]);
-      v += a.w[route] * z;
+    if (row >= own_rows) continue;
+    float v = 0.0f;
+    for (uint32_t k0 = 0; k0 < a.pool.top_k; k0 += 4) {
+      uint2 who[4];
+      float bias[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {  // (loads of four at a time)
+        who[k] = named[i * a.pool.top_k + min(k0 + k, a.pool.top_k - 1)];
+        if (k0 + k >= a.pool.top_k || who[k].x >= a.pool.num_experts) who[k].x = ~0u;
+        bias[k] = a.pool.down_bias && group == 0 && who[k].x != ~0u ? bf16_to_f(a.pool.down_bias[static_cast<size_t>(who[k].x) * d + j]) : 0.0f;
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        if (who[k].x == ~0u) continue;
+        float z = 0.0f;
+        for (uint32_t p = 0; p < routed_parts; ++p) z += sums[(static_cast<size_t>(p) * rows + i * a.pool.top_k + k0 + k) * ROWS + row];
+        v += __uint_as_float(who[k].y) * (z + bias[k]);
+      }
     }
     if (shared_rows) {
       float z = 0.0f;
@@ -340,22 +427,54 @@ __global__ __launch_bounds__(64 * kDownWaves) void experts_down_kernel(const Bf1
       if (a.pool.shared_gate) z *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a.shared_gate[i] * -1.4426950408889634f));
       v += z;
     }
-    a.y[static_cast<size_t>(i) * a.y_stride + j] = narrow_bf16(v);
+    if (cut.groups > 1) a.group_sums[(static_cast<size_t>(group) * a.t + i) * d + j] = v;
+    else finish_token(a, i, j, v);
   }
 }
 
-template <int ROWS, int XI, int STAGES>
-hipError_t launch_down(hipStream_t s, const Bf16ExpertsArgs& a) {
+// The third launch, where there are several groups: their sums of a token in their order.
+__global__ __launch_bounds__(256) void experts_join_kernel(const Bf16ExpertsArgs a, uint32_t groups) {
+  const uint32_t at = blockIdx.x * 256 + threadIdx.x, d = a.pool.d;
+  if (at >= a.t * d) return;
+  float v = 0.0f;
+  for (uint32_t k = 0; k < groups; ++k) v += a.group_sums[static_cast<size_t>(k) * a.t * d + at];
+  finish_token(a, at / d, at % d, v);
+}
+
+constexpr uint32_t kMostGroups = 4;
+
+// Rows of a workgroup, at most `most`, that give every unit the same number of workgroups.  (Fewer than four would read little but activations.)
+uint32_t rows_of_workgroup(uint32_t d, uint32_t groups, uint32_t most, uint32_t cus) {
+  const uint32_t rounds = (d * groups + cus * most - 1) / (cus * most);
+  return std::min(std::max((d * groups + cus * rounds - 1) / (cus * rounds), 4u), most);
+}
+
+template <int ROWS, int XI, int STAGES, int WAVES>
+hipError_t launch_down(hipStream_t s, const Bf16ExpertsArgs& a, uint32_t own_rows, uint32_t groups) {
   const mf_bf16_expert_pool& p = a.pool;
   const uint32_t routes = a.route_count(), rows = routes + (p.shared_f ? a.t : 0), longest = (std::max(p.f, p.shared_f) + 63) / 64;
   // parts of the sum over f, so that every wave has something to do when few experts are live
   uint32_t parts = 1;
-  while (parts < 4 && a.most_live() * parts < 3 * kDownWaves && parts * 2 * rows * ROWS <= 4096 && longest > parts) parts *= 2;
-  const uint32_t part_blocks = (longest + parts - 1) / parts;
-  const size_t lds = kDownWaves * STAGES * (ROWS / 8 + 2 * XI) * 1024 + static_cast<size_t>(parts) * rows * ROWS * 4 + (routes + 1) / 2 * 8 + routes * 8;
-  const hipError_t e = allow_lds<experts_down_kernel<ROWS, XI, STAGES>>(lds, 156 * 1024);
+  while (groups == 1 && parts < 4 && a.most_live() * parts < 2 * WAVES && parts * 2 * rows * ROWS <= 4096 && longest > parts) parts *= 2;
+  const uint32_t blocks = (longest + parts - 1) / parts;
+  const auto share = [&](uint32_t f) { return ((f + 63) / 64 + groups - 1) / groups; };
+  const DownCut cut = groups == 1 ? DownCut{own_rows, blocks, blocks, parts, 1} : DownCut{own_rows, share(p.f), share(p.shared_f), 1, groups};
+  const size_t items = static_cast<size_t>(routes + (p.shared_f ? (a.t + 8 * XI - 1) / (8 * XI) : 0)) * parts;
+  const size_t lds = WAVES * STAGES * (ROWS / 8 + 2 * XI) * 1024 + static_cast<size_t>(parts) * rows * ROWS * 4 + (routes + 1) / 2 * 8 + routes * 16 + items * 8;
+  const hipError_t e = allow_lds<experts_down_kernel<ROWS, XI, STAGES, WAVES>>(lds, 154 * 1024);
   if (e != hipSuccess) return e;
-  experts_down_kernel<ROWS, XI, STAGES><<<dim3((p.d + ROWS - 1) / ROWS), 64 * kDownWaves, lds, s>>>(a, part_blocks, parts);
+  experts_down_kernel<ROWS, XI, STAGES, WAVES><<<dim3((p.d + own_rows - 1) / own_rows, groups), 64 * WAVES, lds, s>>>(a, cut);
+  if (groups > 1) experts_join_kernel<<<dim3((a.t * p.d + 255) / 256), 256, 0, s>>>(a, groups);
+  return hipGetLastError();
+}
+
+template <int XI>
+hipError_t launch_up(hipStream_t s, const Bf16ExpertsArgs& a) {
+  const mf_bf16_expert_pool& p = a.pool;
+  const uint32_t shared = p.shared_f ? (a.t + 8 * XI - 1) / (8 * XI) + (p.shared_gate ? 1 : 0) : 0;
+  const dim3 grid((std::max(p.f, p.shared_f) + 15) / 16, a.most_tiles(8 * XI) + shared);
+  if (aligned16(a.x) && a.x_stride % 8 == 0 && a.x_stride < 1u << 24) experts_up_kernel<XI, true><<<grid, 64 * kUpWaves, 0, s>>>(a);  // (offsets of 32 bits)
+  else experts_up_kernel<XI, false><<<grid, 64 * kUpWaves, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -370,6 +489,8 @@ void bf16_experts_layout(Bf16ExpertsArgs& a, void* workspace) {
   a.acts = reinterpret_cast<uint16_t*>(p);
   p += 4 * static_cast<size_t>(a.route_count()) * a.pool.f;  // (f is a multiple of 8)
   a.shared_acts = reinterpret_cast<uint16_t*>(p);
+  p += 4 * static_cast<size_t>(a.t) * a.pool.shared_f;
+  a.group_sums = reinterpret_cast<float*>(p);
 }
 
 size_t bf16_experts_workspace_bytes(const mf_bf16_expert_pool& pool, uint32_t t) {
@@ -377,25 +498,23 @@ size_t bf16_experts_workspace_bytes(const mf_bf16_expert_pool& pool, uint32_t t)
   a.pool = pool;
   a.t = t;
   bf16_experts_layout(a, nullptr);
-  return reinterpret_cast<uintptr_t>(a.shared_acts) + 4 * static_cast<size_t>(t) * pool.shared_f;
+  return reinterpret_cast<uintptr_t>(a.group_sums) + (t > 8 ? 4 * static_cast<size_t>(kMostGroups) * t * pool.d : 0);
 }
 
 hipError_t launch_bf16_experts(hipStream_t s, const Bf16ExpertsArgs& a) {
   const mf_bf16_expert_pool& p = a.pool;
-  const uint32_t widest = std::max(p.f, p.shared_f);
-  const dim3 grid((widest + 15) / 16, a.most_live() + (p.shared_f ? p.shared_gate ? 2 : 1 : 0));
-  const bool aligned = aligned16(a.x) && a.x_stride % 8 == 0 && a.x_stride < 1u << 24;  // (offsets of 32 bits)
+  const hipError_t e = a.t <= 8 ? launch_up<1>(s, a) : launch_up<2>(s, a);
+  if (e != hipSuccess) return e;
+  const uint32_t cus = device_cu_count();
   if (a.t <= 8) {
-    if (aligned) experts_up_kernel<1, true><<<grid, 64 * kUpWaves, 0, s>>>(a);
-    else experts_up_kernel<1, false><<<grid, 64 * kUpWaves, 0, s>>>(a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    return p.d / 16 < device_cu_count() ? launch_down<8, 1, 4>(s, a) : launch_down<16, 1, 4>(s, a);
+    const uint32_t rows = rows_of_workgroup(p.d, 1, 16, cus);
+    return rows <= 8 ? launch_down<8, 1, 4, 8>(s, a, rows, 1) : launch_down<16, 1, 4, 8>(s, a, rows, 1);
   }
-  if (aligned) experts_up_kernel<2, true><<<grid, 64 * kUpWaves, 0, s>>>(a);
-  else experts_up_kernel<2, false><<<grid, 64 * kUpWaves, 0, s>>>(a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? launch_down<16, 2, 2>(s, a) : e;
+  // Groups, until every unit has a workgroup of 20 rows or more: 16 tokens, 12 live experts of 1024 x 2048: 32 us in one, 17.8 + 4.8 in four; 61 tokens, 26 live of them: 60 in two
+  // groups of 16 rows, 46 + 4.8 in four of 32; 32 tokens, 27 live of 704 x 2816: 41 in two of 22 rows, 55 in four, 60 in one.
+  uint32_t groups = 1;
+  while (groups < kMostGroups && p.d * groups < cus * 20) groups *= 2;
+  return launch_down<32, 2, 2, 4>(s, a, rows_of_workgroup(p.d, groups, 32, cus), groups);
 }
 
 }  // namespace mf
