@@ -196,10 +196,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const T
   };
   const uint32_t r = lane & 15, g = lane >> 4, mine = r * 8 + (g ^ (r & 7));
   f32x4_t sum[NT][MT] = {};
-  if constexpr (NT * MT >= 64) {  // sums that need the accumulation registers: the compiler takes them only where a kernel names one
-    float none = 0.0f;
-    asm volatile("; %0" : "+a"(none));
-  }
   uint4 fx[2][MT], fw[2][NT];
   const auto read_one = [&](int k, int half, uint32_t stage) {
     const uint4* p = lds + stage * (kStage / 16) + (mine ^ half * 4);
@@ -417,16 +413,20 @@ size_t project_workspace_bytes(uint32_t m, uint32_t n, uint32_t t, bool gated) {
 
 namespace {
 
-// The shapes of tiles, and what they cost: us for a block of 64 values of n where each CU has one tile (or several in turn), where the chip has more than two rounds of them (the caches
-// then hold less of what they share), and in front of and behind the blocks.  Measured over 1 .. 4096 tokens and seven pairs of sizes; the choice is within 10 % of the
-// best shape in most of them.
+// The shapes of tiles, and what they cost: us for a block of 64 values of n where every CU has the tiles that fit it at once (one, or two of 128 x 128 in two stages), where the chip has
+// more than two tiles a CU (the caches then hold less of what they share), and in front of and behind the blocks.  Measured over 1 .. 4096 tokens and seven pairs of
+// sizes; the choice is within 10 % of the best shape in most of them.  A third stage is worth more than the second workgroup that it costs while there are no tiles for one:
+// 128 x 128 at 512 tokens, 5120 -> 5120: 40.0 us in three stages, 56.5 in two; at 1024 tokens 80 and 63.
 struct Shape {
   uint32_t tokens, rows;
   float block, block_many, fixed;
+  uint32_t a_cu;
   bool unaligned;  // has a form for rows that are no whole 16 bytes
 };
-constexpr Shape kShapes[] = {{32, 32, 0.09f, 0.1f, 3.7f, true},    {32, 64, 0.133f, 0.15f, 4.0f, false},   {64, 64, 0.178f, 0.2f, 4.3f, true},     {64, 128, 0.267f, 0.33f, 5.0f, false},
-                             {128, 128, 0.36f, 0.55f, 7.0f, true}, {256, 128, 0.8f, 0.92f, 9.0f, false}, {256, 192, 1.35f, 1.42f, 10.0f, false}, {256, 256, 1.5f, 1.62f, 13.0f, false}};
+constexpr Shape kShapes[] = {{32, 32, 0.09f, 0.1f, 3.7f, 1, true},      {32, 64, 0.133f, 0.15f, 4.0f, 1, false},     {64, 64, 0.178f, 0.2f, 4.3f, 1, true},
+                             {64, 128, 0.267f, 0.33f, 5.0f, 1, false},  {128, 128, 0.65f, 0.97f, 9.5f, 2, true},     {128, 128, 0.385f, 0.5f, 7.7f, 1, false},
+                             {128, 192, 0.53f, 0.79f, 10.0f, 1, false}, {256, 128, 0.8f, 0.92f, 9.0f, 1, false},     {256, 192, 1.35f, 1.42f, 10.0f, 1, false},
+                             {256, 256, 1.5f, 1.62f, 13.0f, 1, false}};
 
 template <bool GATED, bool ALIGNED>
 hipError_t launch_shape(hipStream_t s, TileArgs& t, float* workspace) {
@@ -439,14 +439,14 @@ hipError_t launch_shape(hipStream_t s, TileArgs& t, float* workspace) {
   int best = 0;
   uint32_t blocks = (a.n + 63) / 64, parts = 1;
   float least = 3.4e38f;
-  for (int k = 0; k < 8; ++k) {
+  for (int k = 0; k < 10; ++k) {
     const Shape& h = kShapes[k];
     if (!ALIGNED && !h.unaligned) continue;
     const uint64_t tiles = static_cast<uint64_t>((a.t + h.tokens - 1) / h.tokens) * ((rows + h.rows - 1) / h.rows);
     for (uint32_t p = 1; p <= (workspace ? kMostParts : 1); p *= 2) {
-      const uint64_t bytes = 4ull * p * a.t * rows, rounds = (tiles * p + cus - 1) / cus;
+      const uint64_t bytes = 4ull * p * a.t * rows, rounds = (tiles * p + cus * h.a_cu - 1) / (cus * h.a_cu);
       if (p > 1 && (tiles * p > cus || blocks / p < 4 || bytes > kMostPartBytes)) break;
-      float us = h.fixed + static_cast<float>(rounds * ((blocks + p - 1) / p)) * (rounds > 2 ? h.block_many : h.block);
+      float us = h.fixed + static_cast<float>(rounds * ((blocks + p - 1) / p)) * (tiles * p > 2 * cus ? h.block_many : h.block);
       if (p > 1) us += 3.5f + static_cast<float>(bytes) / 2e6f;  // the launch that adds the parts, and their way to memory and back
       if (us < least) least = us, best = k, parts = p;
     }
@@ -463,9 +463,11 @@ hipError_t launch_shape(hipStream_t s, TileArgs& t, float* workspace) {
     switch (best) {
       case 1: return launch_tiles<32, 64, 2, 2, 2, 4, GATED, true>(s, t);
       case 3: return launch_tiles<64, 128, 2, 4, 1, 3, GATED, true>(s, t);
-      case 5: return launch_tiles<256, 128, 4, 2, 1, 3, GATED, true>(s, t);
-      case 6: return launch_tiles<256, 192, 4, 2, 1, 2, GATED, true>(s, t);
-      case 7: return launch_tiles<256, 256, 2, 4, 1, 2, GATED, true>(s, t);
+      case 5: return launch_tiles<128, 128, 2, 4, 1, 3, GATED, true>(s, t);
+      case 6: return launch_tiles<128, 192, 4, 2, 1, 3, GATED, true>(s, t);
+      case 7: return launch_tiles<256, 128, 4, 2, 1, 3, GATED, true>(s, t);
+      case 8: return launch_tiles<256, 192, 4, 2, 1, 2, GATED, true>(s, t);
+      case 9: return launch_tiles<256, 256, 2, 4, 1, 2, GATED, true>(s, t);
     }
   }
   return hipErrorUnknown;
