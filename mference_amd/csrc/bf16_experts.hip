@@ -28,14 +28,14 @@ __device__ __forceinline__ void each_live(uint32_t e, uint32_t num_experts, Foun
 
 // ------------------------------------------------------------------ activations
 
-constexpr uint32_t kUpWaves = 4, kUpStages = 2;
+constexpr uint32_t kUpWaves = 2, kUpStages = 2;
 
-// The first launch: activations of 16 gate and 16 up rows of one live expert, or of the shared one, for eight (XI = 2: 16) of its routes: a tile (blockIdx.y).  Work is
-// the reading of W, rows of d in 128-byte lines, so a workgroup's waves share d between them and each streams its part of the 32 rows through a ring of two stages in LDS; the
-// matrix cores' sums meet in LDS.  What bounds it is the memory: 206 MB in 46 us (8 tokens, 23 live experts of 704 x 2816 beside a shared one of 2112; 4.5 TB/s), 218 MB in 58 us where
-// popular experts have several tiles, which read their rows again (61 tokens, 26 live of 1024 x 2048), 17.8 MB in 9 us (one token), where the way to the expert's number and the
-// first lines take most of it.  Measured beside it: three stages 49, 69 and 10.4 us, fewer workgroups fitting on a unit; waves with 16 + 16 rows of their own and all of d, 59 and 77 us;
-// an expert's tiles one after the other in a workgroup, 68 us at 61 tokens.
+// The first launch: activations of 16 gate and 16 up rows of one live expert, or of the shared one, for eight (XI = 2: 16) of its routes: a tile (blockIdx.y).  Its work is
+// the reading of W, rows of d in lines of 128 bytes: a workgroup's two waves share d and each streams its part of the 32 rows through a ring of two stages in LDS; the matrix
+// cores' sums meet in LDS.  What bounds it is the memory: 206 MB in 42 us (8 tokens, 23 live experts of 704 x 2816 beside a shared one of 2112: 4.9 TB/s, the rate of a large copy);
+// 218 MB in 55 us where popular experts have several tiles, which read their rows again (61 tokens, 26 live of 1024 x 2048); 37.7 MB in 9 us (one token, 8 of 512 x 2048 beside a
+// shared one), of which the way to the expert's number and the first lines is the larger part.  Measured beside it, at the first two: four waves 46 and 58 us; three stages
+// 46 and 63, fewer workgroups fitting on a unit; waves with 16 + 16 rows of their own and all of d, 59 and 77; an expert's tiles one after the other in a workgroup, 68 at 61 tokens.
 template <int XI, bool ALIGNED>
 __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16ExpertsArgs a) {
   constexpr int kLoads = 4 + XI, kRing = kUpStages * kLoads * 64;
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
       v = wave_sum(v);
       if (lane == 0) part[wave] = v;
       __syncthreads();
-      if (tid == 0) a.shared_gate[i] = part[0] + part[1] + part[2] + part[3];
+      if (tid == 0) a.shared_gate[i] = part[0] + part[1];
       __syncthreads();
     }
     return;
@@ -166,11 +166,12 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
     *reinterpret_cast<f32x4_t*>(part + wave * 512 + r * 16 + g * 4) = zg;
     *reinterpret_cast<f32x4_t*>(part + wave * 512 + 256 + r * 16 + g * 4) = zu;
     __syncthreads();
-    const uint32_t column = tid / 16, j = j0 + tid % 16;
-    if (column < 8 * kX && base + column < count && j < f) {
+    for (uint32_t o = tid; o < 128 * kX; o += 64 * kUpWaves) {
+      const uint32_t column = o / 16, j = j0 + o % 16;
+      if (base + column >= count || j >= f) continue;
       float gate = 0.0f, up = 0.0f;
 #pragma unroll
-      for (uint32_t v = 0; v < kUpWaves; ++v) gate += part[v * 512 + tid], up += part[v * 512 + 256 + tid];
+      for (uint32_t v = 0; v < kUpWaves; ++v) gate += part[v * 512 + o], up += part[v * 512 + 256 + o];
       if (bias) gate += bf16_to_f(bias[j]), up += bf16_to_f(bias[f + j]);
       const float act = activate(gate, a.pool.activation) * up;
       const size_t to_at = static_cast<size_t>(list[base + column]) * f + j;
@@ -202,7 +203,7 @@ __device__ __forceinline__ void finish_token(const Bf16ExpertsArgs& a, uint32_t 
 // weighted sums over a token's routes are made there in the order of their ranks, the parts of a sum in theirs: no atomics, so calls repeat to the bit.
 // The activations come as two bf16 terms (32 bits narrowed to 16 would cost the layer half a step more than the result's own rounding).  What bounds it: 103 MB in 29 us
 // (8 tokens, d 2816: 256 workgroups of 11 rows; 176 of 16 took 47), 109 MB in 46 us (61 tokens), where LDS holds all routes' sums and rings of two stages, too few bytes on their
-// way for more than 3.8 TB/s with the rows that several tiles read; 9.4 MB in 10 us (one token), latency: idx, then the rows, then the sums.
+// way for more than 3.8 TB/s with the rows that several tiles read; 18.9 MB in 10 us (one token), the way from idx to the rows to the sums; 16 waves 11 us.
 template <int ROWS, int XI, int STAGES, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16ExpertsArgs a, const DownCut cut) {
   constexpr uint32_t kW = ROWS / 8, kLoads = kW + 2 * XI, kStage = kLoads * 64, kTile = 8 * XI, kM = (ROWS + 15) / 16, kThreads = 64 * WAVES;
@@ -216,7 +217,7 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
   uint2* table = named + routes;                                                                    // a group's items: expert | routes << 16 | part << 24, first
   __shared__ uint32_t tile_count, hist[MF_MAX_EXPERTS], wave_sums[2][WAVES];
   for (uint32_t k = tid; k < routes; k += kThreads) named[k] = make_uint2(a.idx[k], __float_as_uint(a.w[k]));
-  if (routes <= kFew) {
+  if (XI == 1 || routes <= kFew) {  // (eight tokens have no more)
     if (wave == 0) {
       const uint32_t e = lane < routes ? a.idx[lane] : ~0u;
       uint32_t first = 0, n = 0;
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
       });
       if (lane == 0) tile_count = n;
     }
-  } else {
+  } else if constexpr (XI > 1) {
     // a thread two neighbouring experts (or one)
     constexpr uint32_t kEach = MF_MAX_EXPERTS / kThreads;
     static_assert(kEach * kThreads == MF_MAX_EXPERTS, "the threads share out the experts");
