@@ -186,37 +186,32 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
 
 // ------------------------------------------------------------------ results
 
-// How the second launch is cut: rows of a workgroup; the sums over f in parts that a workgroup's waves share, or, where there are several groups, one for each group
-// (their sums of a token meet in a third launch).
+// How the second launch is cut: rows of a workgroup, and parts of the sums over f, which a workgroup's waves share up to eight tokens and workgroups of their own take beyond.
 struct DownCut {
-  uint32_t rows, routed_blocks, shared_blocks, parts, groups;  // (blocks: of 64 of f, in a part)
+  uint32_t rows, routed_blocks, shared_blocks, parts;  // (blocks: of 64 of f, in a part)
 };
 
-// The result of token i's row j from what the routed experts gave it.
-__device__ __forceinline__ void finish_token(const Bf16ExpertsArgs& a, uint32_t i, uint32_t j, float v) {
-  if (a.residual) v += bf16_to_f(a.residual[static_cast<size_t>(i) * a.residual_stride + j]);
-  a.y[static_cast<size_t>(i) * a.y_stride + j] = narrow_bf16(v);
-}
-
 // The second launch: up to ROWS results of every token.  The work is cut into items, the rows of one expert's down matrix times up to 8 XI of its routes over a part of f,
-// dealt to a workgroup's waves; a wave's items are one stream through its ring in LDS, whose requests run over an item's end into the next.  Every route's sum goes to LDS, and the
-// weighted sums over a token's routes are made there in the order of their ranks, the parts of a sum in theirs: no atomics, so calls repeat to the bit.
-// The activations come as two bf16 terms (32 bits narrowed to 16 would cost the layer half a step more than the result's own rounding).  What bounds it: 103 MB in 29 us
-// (8 tokens, d 2816: 256 workgroups of 11 rows; 176 of 16 took 47), 109 MB in 46 us (61 tokens), where LDS holds all routes' sums and rings of two stages, too few bytes on their
-// way for more than 3.8 TB/s with the rows that several tiles read; 18.9 MB in 10 us (one token), the way from idx to the rows to the sums; 16 waves 11 us.
+// dealt to a workgroup's waves; a wave's items are one stream through its ring in LDS, whose requests run over an item's end into the next.  Up to eight tokens every route's sum
+// goes to LDS and the weighted sums over a token's routes are made there, in the order of their ranks, the parts of a sum in theirs; beyond, the sums go to memory and a third launch adds
+// them up in that order: no atomics either way, so calls repeat to the bit.  The activations come as two bf16 terms (32 bits narrowed to 16 would cost the layer half a step more than
+// the result's own rounding).  What bounds it: 103 MB in 28 us (8 tokens, d 2816: 256 workgroups of 11 rows; 176 of 16 took 47); 109 MB in 34 us (61 tokens; with all routes' sums in
+// LDS there was room for rings of two stages, not four, and it took 46), 4 TB/s with the rows that several tiles read; 18.9 MB in 10 us (one token), the way from idx to the
+// rows to the sums; 16 waves 11 us.
 template <int ROWS, int XI, int STAGES, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16ExpertsArgs a, const DownCut cut) {
+  constexpr bool kJoin = XI > 1;  // beyond eight tokens the third launch adds up
   constexpr uint32_t kW = ROWS / 8, kLoads = kW + 2 * XI, kStage = kLoads * 64, kTile = 8 * XI, kM = (ROWS + 15) / 16, kThreads = 64 * WAVES;
   extern __shared__ uint4 whole_lds[];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4, group = blockIdx.y;
   const uint32_t d = a.pool.d, routes = a.route_count(), shared_rows = a.pool.shared_f ? a.t : 0, rows = routes + shared_rows, j0 = blockIdx.x * cut.rows, own_rows = min(cut.rows, d - j0);
   float* sums = reinterpret_cast<float*>(whole_lds + WAVES * STAGES * kStage);                      // [parts][rows][ROWS]
-  uint32_t* list = reinterpret_cast<uint32_t*>(sums + static_cast<size_t>(cut.parts) * rows * ROWS);  // [routes]: by tile
+  uint32_t* list = reinterpret_cast<uint32_t*>(sums + (kJoin ? 0 : static_cast<size_t>(cut.parts) * rows * ROWS));  // [routes]: by tile
   uint2* tiles = reinterpret_cast<uint2*>(list + (routes + 1) / 2 * 2);                             // expert | routes << 16, first; at most `routes` of them
   uint2* named = tiles + routes;                                                                    // [routes]: expert, weight
-  uint2* table = named + routes;                                                                    // a group's items: expert | routes << 16 | part << 24, first
+  uint2* table = named + (kJoin ? 0 : routes);                                                                    // a group's items: expert | routes << 16 | part << 24, first
   __shared__ uint32_t tile_count, hist[MF_MAX_EXPERTS], wave_sums[2][WAVES];
-  for (uint32_t k = tid; k < routes; k += kThreads) named[k] = make_uint2(a.idx[k], __float_as_uint(a.w[k]));
+  for (uint32_t k = tid; !kJoin && k < routes; k += kThreads) named[k] = make_uint2(a.idx[k], __float_as_uint(a.w[k]));
   if (XI == 1 || routes <= kFew) {  // (eight tokens have no more)
     if (wave == 0) {
       const uint32_t e = lane < routes ? a.idx[lane] : ~0u;
@@ -276,8 +271,7 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
   }
   __syncthreads();
   // items: the shared expert's first (its f may be the longest), then the tiles of routes; a tile's parts side by side
-  const bool one = cut.groups == 1;
-  const auto parts_of = [&](uint32_t f, uint32_t blocks) { return one ? (f + blocks * 64 - 1) / (blocks * 64) : group * blocks * 64 < f ? 1u : 0u; };
+  const auto parts_of = [&](uint32_t f, uint32_t blocks) { return kJoin ? group * blocks * 64 < f ? 1u : 0u : (f + blocks * 64 - 1) / (blocks * 64); };
   const uint32_t shared_parts = parts_of(a.pool.shared_f, cut.shared_blocks), routed_parts = parts_of(a.pool.f, cut.routed_blocks);
   const uint32_t shared_items = (shared_rows + kTile - 1) / kTile * shared_parts, items = shared_items + __builtin_amdgcn_readfirstlane(tile_count) * routed_parts;
   struct Item {
@@ -301,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
     it.part = who >> 24;
     it.shared = n < shared_items;
     it.f = it.shared ? a.pool.shared_f : a.pool.f;
-    const uint32_t blocks = it.shared ? cut.shared_blocks : cut.routed_blocks, from = (one ? it.part : group) * blocks * 64;
+    const uint32_t blocks = it.shared ? cut.shared_blocks : cut.routed_blocks, from = (kJoin ? group : it.part) * blocks * 64;
     it.left = it.f - from;
     it.blocks = (min(it.left, blocks * 64) + 63) / 64;
     it.w = (it.shared ? a.pool.shared_down : a.pool.down) + (static_cast<size_t>(expert) * d + j0) * it.f + from;
@@ -386,10 +380,11 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
             sum[m] = mfma16(fw[m][h], fl[h], sum[m]);
           }
         if (++block < now.blocks) continue;
-        float* out = sums + (static_cast<size_t>(now.part) * rows + (now.shared ? routes : 0) + route_of(now, r)) * ROWS + g * 4;
+        const size_t row = static_cast<size_t>(kJoin ? group : now.part) * rows + (now.shared ? routes : 0) + route_of(now, r);
+        float* out = (kJoin ? a.route_sums + row * d + j0 : sums + row * ROWS) + g * 4;
 #pragma unroll
         for (uint32_t m = 0; m < kM; ++m) {
-          if (r < now.count && g * 4 < ROWS) *reinterpret_cast<f32x4_t*>(out + m * 16) = sum[m];
+          if (r < now.count && m * 16 + g * 4 < (kJoin ? own_rows : ROWS)) *reinterpret_cast<f32x4_t*>(out + m * 16) = sum[m];
           sum[m] = f32x4_t{};
         }
         block = 0;
@@ -400,6 +395,7 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
     }
     wait_loads<0>();
   }
+  if constexpr (kJoin) return;
   __syncthreads();
   for (uint32_t o = tid; o < a.t * ROWS; o += kThreads) {
     const uint32_t i = o / ROWS, row = o % ROWS, j = j0 + row;
@@ -412,7 +408,7 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
       for (uint32_t k = 0; k < 4; ++k) {  // (loads of four at a time)
         who[k] = named[i * a.pool.top_k + min(k0 + k, a.pool.top_k - 1)];
         if (k0 + k >= a.pool.top_k || who[k].x >= a.pool.num_experts) who[k].x = ~0u;
-        bias[k] = a.pool.down_bias && group == 0 && who[k].x != ~0u ? bf16_to_f(a.pool.down_bias[static_cast<size_t>(who[k].x) * d + j]) : 0.0f;
+        bias[k] = a.pool.down_bias && who[k].x != ~0u ? bf16_to_f(a.pool.down_bias[static_cast<size_t>(who[k].x) * d + j]) : 0.0f;
       }
 #pragma unroll
       for (uint32_t k = 0; k < 4; ++k) {
@@ -428,21 +424,67 @@ __global__ __launch_bounds__(64 * WAVES) void experts_down_kernel(const Bf16Expe
       if (a.pool.shared_gate) z *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a.shared_gate[i] * -1.4426950408889634f));
       v += z;
     }
-    if (cut.groups > 1) a.group_sums[(static_cast<size_t>(group) * a.t + i) * d + j] = v;
-    else finish_token(a, i, j, v);
+    if (a.residual) v += bf16_to_f(a.residual[static_cast<size_t>(i) * a.residual_stride + j]);
+    a.y[static_cast<size_t>(i) * a.y_stride + j] = narrow_bf16(v);
   }
 }
 
-// The third launch, where there are several groups: their sums of a token in their order.
-__global__ __launch_bounds__(256) void experts_join_kernel(const Bf16ExpertsArgs a, uint32_t groups) {
-  const uint32_t at = blockIdx.x * 256 + threadIdx.x, d = a.pool.d;
-  if (at >= a.t * d) return;
-  float v = 0.0f;
-  for (uint32_t k = 0; k < groups; ++k) v += a.group_sums[static_cast<size_t>(k) * a.t * d + at];
-  finish_token(a, at / d, at % d, v);
+// The third launch, beyond eight tokens: four neighbouring results of a token a thread, the weighted sums of its routes in the order of their ranks, the parts of a sum in theirs.
+template <uint32_t GROUPS>
+__global__ __launch_bounds__(64) void experts_join_kernel(const Bf16ExpertsArgs a, const DownCut cut) {
+  const uint32_t d = a.pool.d, at = blockIdx.x * 64 + threadIdx.x, i = at / (d / 4), j = at % (d / 4) * 4, routes = a.route_count(), rows = routes + (a.pool.shared_f ? a.t : 0);
+  if (i >= a.t) return;
+  const auto load = [&](f32x4_t* z, uint32_t row, uint32_t f, uint32_t blocks, bool is) {  // (a short f has fewer parts)
+#pragma unroll
+    for (uint32_t p = 0; p < GROUPS; ++p) z[p] = is && p * blocks * 64 < f ? *reinterpret_cast<const f32x4_t*>(a.route_sums + (static_cast<size_t>(p) * rows + row) * d + j) : f32x4_t{};
+  };
+  const auto whole = [](const f32x4_t* z) {
+    f32x4_t sum = z[0];
+#pragma unroll
+    for (uint32_t p = 1; p < GROUPS; ++p) sum += z[p];
+    return sum;
+  };
+  // (the loads of all ranks at once: one after the other they took 10.9 us, so 8.0: 61 tokens of 8 routes, 2048 results, four parts, 16 MB)
+  f32x4_t v = {}, z[MF_MAX_TOPK][GROUPS];
+  uint32_t e[MF_MAX_TOPK];
+  float w[MF_MAX_TOPK];
+#pragma unroll
+  for (uint32_t k = 0; k < MF_MAX_TOPK; ++k) {
+    const uint32_t route = i * a.pool.top_k + min(k, a.pool.top_k - 1);
+    e[k] = k < a.pool.top_k ? a.idx[route] : ~0u;
+    w[k] = a.w[route];
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < MF_MAX_TOPK; ++k) load(z[k], i * a.pool.top_k + k, a.pool.f, cut.routed_blocks, e[k] < a.pool.num_experts);
+#pragma unroll
+  for (uint32_t k = 0; k < MF_MAX_TOPK; ++k) {
+    if (e[k] >= a.pool.num_experts) continue;
+    f32x4_t sum = whole(z[k]);
+    if (a.pool.down_bias)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sum[c] += bf16_to_f(a.pool.down_bias[static_cast<size_t>(e[k]) * d + j + c]);
+    v += w[k] * sum;
+  }
+  if (a.pool.shared_f) {
+    load(z[0], routes + i, a.pool.shared_f, cut.shared_blocks, true);
+    f32x4_t sum = whole(z[0]);
+    if (a.pool.shared_gate) sum *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(a.shared_gate[i] * -1.4426950408889634f));
+    v += sum;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (a.residual) v[c] += bf16_to_f(a.residual[static_cast<size_t>(i) * a.residual_stride + j + c]);
+    a.y[static_cast<size_t>(i) * a.y_stride + j + c] = narrow_bf16(v[c]);
+  }
 }
 
-constexpr uint32_t kMostGroups = 4;
+// Beyond eight tokens: parts of the sums over f in workgroups of their own, until every unit has one of 20 rows or more.  16 tokens, 12 live
+// experts of 1024 x 2048: 32 us in one, 16.6 + 4.8 in four; 32 tokens, 27 live of 704 x 2816: 37 in two of 24 rows.
+uint32_t groups_of(const mf_bf16_expert_pool& p) {
+  uint32_t groups = 1;
+  while (groups < 4 && p.d * groups < device_cu_count() * 20) groups *= 2;
+  return groups;
+}
 
 // Rows of a workgroup, at most `most`, that give every unit the same number of workgroups.  (Fewer than four would read little but activations.)
 uint32_t rows_of_workgroup(uint32_t d, uint32_t groups, uint32_t most, uint32_t cus) {
@@ -454,18 +496,23 @@ template <int ROWS, int XI, int STAGES, int WAVES>
 hipError_t launch_down(hipStream_t s, const Bf16ExpertsArgs& a, uint32_t own_rows, uint32_t groups) {
   const mf_bf16_expert_pool& p = a.pool;
   const uint32_t routes = a.route_count(), rows = routes + (p.shared_f ? a.t : 0), longest = (std::max(p.f, p.shared_f) + 63) / 64;
-  // parts of the sum over f, so that every wave has something to do when few experts are live
-  uint32_t parts = 1;
-  while (groups == 1 && parts < 4 && a.most_live() * parts < 2 * WAVES && parts * 2 * rows * ROWS <= 4096 && longest > parts) parts *= 2;
-  const uint32_t blocks = (longest + parts - 1) / parts;
-  const auto share = [&](uint32_t f) { return ((f + 63) / 64 + groups - 1) / groups; };
-  const DownCut cut = groups == 1 ? DownCut{own_rows, blocks, blocks, parts, 1} : DownCut{own_rows, share(p.f), share(p.shared_f), 1, groups};
-  const size_t items = static_cast<size_t>(routes + (p.shared_f ? (a.t + 8 * XI - 1) / (8 * XI) : 0)) * parts;
-  const size_t lds = WAVES * STAGES * (ROWS / 8 + 2 * XI) * 1024 + static_cast<size_t>(parts) * rows * ROWS * 4 + (routes + 1) / 2 * 8 + routes * 16 + items * 8;
-  const hipError_t e = allow_lds<experts_down_kernel<ROWS, XI, STAGES, WAVES>>(lds, 154 * 1024);
+  DownCut cut = {own_rows, ((p.f + 63) / 64 + groups - 1) / groups, ((p.shared_f + 63) / 64 + groups - 1) / groups, 1};
+  if (XI == 1) {  // parts, so that every wave has something to do when few experts are live
+    while (cut.parts < 4 && a.most_live() * cut.parts < 2 * WAVES && cut.parts * 2 * rows * ROWS <= 4096 && longest > cut.parts) cut.parts *= 2;
+    cut.routed_blocks = cut.shared_blocks = (longest + cut.parts - 1) / cut.parts;
+  }
+  const size_t items = static_cast<size_t>(routes + (p.shared_f ? (a.t + 8 * XI - 1) / (8 * XI) : 0)) * cut.parts;
+  const size_t own = XI == 1 ? static_cast<size_t>(cut.parts) * rows * ROWS * 4 + routes * 8 : 0;
+  const size_t lds = WAVES * STAGES * (ROWS / 8 + 2 * XI) * 1024 + own + (routes + 1) / 2 * 8 + routes * 8 + items * 8;
+  hipError_t e = allow_lds<experts_down_kernel<ROWS, XI, STAGES, WAVES>>(lds, 154 * 1024);
   if (e != hipSuccess) return e;
   experts_down_kernel<ROWS, XI, STAGES, WAVES><<<dim3((p.d + own_rows - 1) / own_rows, groups), 64 * WAVES, lds, s>>>(a, cut);
-  if (groups > 1) experts_join_kernel<<<dim3((a.t * p.d + 255) / 256), 256, 0, s>>>(a, groups);
+  e = hipGetLastError();
+  if (XI == 1 || e != hipSuccess) return e;
+  const dim3 grid((a.t * (p.d / 4) + 63) / 64);
+  if (groups == 1) experts_join_kernel<1><<<grid, 64, 0, s>>>(a, cut);
+  else if (groups == 2) experts_join_kernel<2><<<grid, 64, 0, s>>>(a, cut);
+  else experts_join_kernel<4><<<grid, 64, 0, s>>>(a, cut);
   return hipGetLastError();
 }
 
@@ -491,7 +538,7 @@ void bf16_experts_layout(Bf16ExpertsArgs& a, void* workspace) {
   p += 4 * static_cast<size_t>(a.route_count()) * a.pool.f;  // (f is a multiple of 8)
   a.shared_acts = reinterpret_cast<uint16_t*>(p);
   p += 4 * static_cast<size_t>(a.t) * a.pool.shared_f;
-  a.group_sums = reinterpret_cast<float*>(p);
+  a.route_sums = reinterpret_cast<float*>(p);
 }
 
 size_t bf16_experts_workspace_bytes(const mf_bf16_expert_pool& pool, uint32_t t) {
@@ -499,7 +546,7 @@ size_t bf16_experts_workspace_bytes(const mf_bf16_expert_pool& pool, uint32_t t)
   a.pool = pool;
   a.t = t;
   bf16_experts_layout(a, nullptr);
-  return reinterpret_cast<uintptr_t>(a.group_sums) + (t > 8 ? 4 * static_cast<size_t>(kMostGroups) * t * pool.d : 0);
+  return reinterpret_cast<uintptr_t>(a.route_sums) + (t > 8 ? 4 * static_cast<size_t>(groups_of(pool)) * (a.route_count() + (pool.shared_f ? t : 0)) * pool.d : 0);
 }
 
 hipError_t launch_bf16_experts(hipStream_t s, const Bf16ExpertsArgs& a) {
@@ -511,11 +558,8 @@ hipError_t launch_bf16_experts(hipStream_t s, const Bf16ExpertsArgs& a) {
     const uint32_t rows = rows_of_workgroup(p.d, 1, 16, cus);
     return rows <= 8 ? launch_down<8, 1, 4, 8>(s, a, rows, 1) : launch_down<16, 1, 4, 8>(s, a, rows, 1);
   }
-  // Groups, until every unit has a workgroup of 20 rows or more: 16 tokens, 12 live experts of 1024 x 2048: 32 us in one, 17.8 + 4.8 in four; 61 tokens, 26 live of them: 60 in two
-  // groups of 16 rows, 46 + 4.8 in four of 32; 32 tokens, 27 live of 704 x 2816: 41 in two of 22 rows, 55 in four, 60 in one.
-  uint32_t groups = 1;
-  while (groups < kMostGroups && p.d * groups < cus * 20) groups *= 2;
-  return launch_down<32, 2, 2, 4>(s, a, rows_of_workgroup(p.d, groups, 32, cus), groups);
+  const uint32_t groups = groups_of(p);
+  return launch_down<32, 2, 4, 4>(s, a, (rows_of_workgroup(p.d, groups, 32, cus) + 3) / 4 * 4, groups);  // (four results a store)
 }
 
 }  // namespace mf

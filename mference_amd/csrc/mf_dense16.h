@@ -25,7 +25,7 @@ struct Bf16ExpertsArgs {
   float* shared_gate;  // [t]: logits of the shared expert's gate
   uint16_t* acts;      // [2][routes, f]: what is left of the activations' 32 bits in two bf16 terms, one plane each
   uint16_t* shared_acts;  // [2][t, shared_f]
-  float* group_sums;   // [groups][t, d], beyond eight tokens
+  float* route_sums;   // [parts][routes + t, d], beyond eight tokens (t: of the shared expert)
 
   __host__ __device__ uint32_t route_count() const { return t * pool.top_k; }
   __host__ __device__ uint32_t most_live() const { return pool.num_experts < route_count() ? pool.num_experts : route_count(); }
