@@ -835,7 +835,7 @@ typedef struct {
   mf_activation activation;
 } mf_bf16_expert_pool;
 
-/* The layer for a few tokens, in two launches that read each live expert once: for token i with experts idx[i, k] and weights w[i, k]
+/* The layer for a few tokens, in two launches (beyond eight tokens a third adds up the routes) that read each live expert once: for token i with experts idx[i, k] and weights w[i, k]
  * (from any of the routers above)
  *   y = narrow(residual + sum over k of w * (down_e a + down_bias_e) + sigmoid(shared_gate . x) * shared_down a_s)
  *   a = act(gate_e x + bias) * (up_e x + bias')

@@ -107,7 +107,11 @@ constexpr int largest_part(int n, int most) {
 // A workgroup TM tokens x TN rows of W (gated: TN / 2 gate rows and their up rows), WM x WN waves, sums in registers.  The operands go straight to LDS in blocks
 // of 64 values of n, a whole line of 128 bytes a row at a time, STAGES - 1 blocks ahead.  A block is two steps of the matrix cores; a wave reads a step's operands into
 // registers while the matrix cores work on the step before, so that a block costs one barrier and no wait for LDS.  The eight pieces of a row are turned by
-// the row's number, so that 16 lanes that read the same piece of 16 rows meet all banks.
+// the row's number, so that 16 lanes that read the same piece of 16 rows meet all banks.  A workgroup starts at a block of its own (`skew`), so that neighbours do not wait
+// for the same lines at once (3 %).  What bounds it: with many large tiles the matrix cores, 60 % of the units' time busy (4096 rows 5120 -> 17408, gated: 1208 us, 1.21 PFLOP/s; the
+// library's product without the gate 1200 to 1275); with one round of tiles the way to memory, 0.53 us a block of 128 x 192 where the matrix cores need 0.32 (777 rows 1280 -> 5120:
+// 22 us); with few, that and what stands in front of the first block and behind the last (200 rows 2816 -> 2113: 9.6).  Waves of four or fewer (kSpread) deal their reads and
+// requests out among the matrix instructions by hand; with eight the scheduler's groups do as well with fewer registers.
 template <int TM, int TN, int WM, int WN, int KG, int STAGES, bool GATED, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const TileArgs t) {
   constexpr bool kSpread = WM * WN <= 4;
@@ -325,7 +329,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const T
   }
 }
 
-// Results whose sums over n were made in parts: four neighbours a thread, the parts in their order.
+// Results whose sums over n were made in parts: four neighbours a thread, the parts in their order.  (20 rows 8200 -> 1100: 16.7 us in one
+// part, 10.5 in four with this launch; 100 rows 8200 -> 4100: 34.7 and 26.7.)
 template <bool GATED>
 __global__ __launch_bounds__(256) void project_parts_kernel(const TileArgs t) {
   const mf_project_args& a = t.p;
@@ -345,7 +350,9 @@ __global__ __launch_bounds__(256) void project_parts_kernel(const TileArgs t) {
 
 // ------------------------------------------------------------------ few rows
 
-// Up to 16 tokens: the call is W's stream.  A workgroup 16 rows of W (and, gated, their up rows), its waves share the sum over n.
+// Up to 16 tokens: the call is W's stream.  A workgroup 16 rows of W (and, gated, their up rows), its waves share the sum over n, each with a ring in LDS that it fills itself with whole
+// lines of 128 bytes.  Four rows 5120 -> 17408, gated: 67 us, 5.3 TB/s (operands straight from memory in the matrix cores' order touch 64 bytes of a row at a time: 2.2 TB/s; eight rows
+// an instruction without LDS: 4.7).
 template <bool GATED, bool ALIGNED, int WAVES, int STAGES, int XI>
 __global__ __launch_bounds__(64 * WAVES) void project_rows_kernel(const mf_project_args a) {
   constexpr int kW = GATED ? 4 : 2, kLoads = kW + XI;

@@ -646,7 +646,7 @@ class HeadNorms:
 
 
 class Bf16Experts:
-    """mf_bf16_experts: a layer of experts kept in 16 bits for a few tokens, the routed ones and the shared one, in two launches (what
+    """mf_bf16_experts: a layer of experts kept in 16 bits for a few tokens, the routed ones and the shared one, in two launches, three beyond eight tokens (what
     MoE.encode_decode_layer is for quantized experts; the routing comes from MoE.encode_router or one of FamilyRouters)."""
     max_tokens = BF16_EXPERTS_ROWS
 
