@@ -1195,6 +1195,7 @@ mf_status mf_project(mf_ctx* ctx, mf_stream stream, const mf_project_args* args,
     return MF_ERR_INVALID_ARGUMENT;
   const uint64_t size = f32 ? 4 : 2, t = a.t, rows = a.gated ? 2ull * a.m : a.m;
   const Rows y = {a.y, size * a.y_stride, size * a.m};
+  const OnDevice on(ctx);  // (the workspace's size is the device's, as the launch cuts the sums)
   const size_t need = mf::project_workspace_bytes(a.m, a.n, a.t, a.gated != 0);
   if (need && (!workspace || !mf::aligned16(workspace))) return MF_ERR_INVALID_ARGUMENT;
   if (workspace_bytes < need) return MF_ERR_SCRATCH_TOO_SMALL;
@@ -1208,7 +1209,6 @@ mf_status mf_project(mf_ctx* ctx, mf_stream stream, const mf_project_args* args,
                (a.residual && rows_meet_block({a.residual, size * a.residual_stride, size * a.m}, t, workspace, need)) ||
                (a.bias && rows_meet_block({workspace, need, need}, 1, bias.p, bias.bytes))))
     return MF_ERR_INVALID_ARGUMENT;
-  const OnDevice on(ctx);
   MF_HIP(ctx, on.error());
   MF_HIP(ctx, mf::launch_project(static_cast<hipStream_t>(stream), a, workspace));
   return MF_OK;
@@ -1330,6 +1330,7 @@ mf_status mf_bf16_experts(mf_ctx* ctx, mf_stream stream, const mf_bf16_expert_po
   a.residual_stride = residual_stride ? residual_stride : p.d;
   a.y_stride = y_stride ? y_stride : p.d;
   if (a.x_stride < p.d || a.y_stride < p.d || (residual && a.residual_stride < p.d)) return MF_ERR_DIMENSION_MISMATCH;
+  const OnDevice on(ctx);  // (the workspace's size is the device's, as the launch cuts the sums)
   const size_t need = mf::bf16_experts_workspace_bytes(p, t);
   if (workspace_bytes < need) return MF_ERR_SCRATCH_TOO_SMALL;
   const uint64_t width = 2ull * p.d, e = p.num_experts, d = p.d, f = p.f, fs = p.shared_f;
@@ -1342,7 +1343,6 @@ mf_status mf_bf16_experts(mf_ctx* ctx, mf_stream stream, const mf_bf16_expert_po
       rows_meet_block(ys, t, workspace, need) || rows_meet_block(xs, t, workspace, need) || (residual && rows_meet_block(rs, t, workspace, need)))
     return MF_ERR_INVALID_ARGUMENT;
   mf::bf16_experts_layout(a, workspace);
-  const OnDevice on(ctx);
   MF_HIP(ctx, on.error());
   MF_HIP(ctx, mf::launch_bf16_experts(static_cast<hipStream_t>(stream), a));
   return MF_OK;
