@@ -54,10 +54,10 @@ __device__ __forceinline__ void store4(uint16_t* p, const f32x4_t& v, uint32_t h
   }
 }
 
-// Results j .. j + 3 of row i, those of them that exist, from their sums (and, gated, from those of their up rows): one rounding, at the end.
+// Results j .. j + 3 of row i, those of them in front of `end`, from their sums (and, gated, from those of their up rows): one rounding, at the end.
 template <bool GATED>
-__device__ __forceinline__ void finish4(const mf_project_args& a, uint32_t i, uint32_t j, f32x4_t z, f32x4_t up) {
-  const uint32_t have = a.m - j;
+__device__ __forceinline__ void finish4(const mf_project_args& a, uint32_t i, uint32_t j, uint32_t end, f32x4_t z, f32x4_t up) {
+  const uint32_t have = end - j;
   if (a.bias) {
     z += load4(a.bias + j, have);
     if (GATED) up += load4(a.bias + a.m + j, have);
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const T
         store4(part, z, a.m - j);
         if (GATED) store4(part + a.m, up, a.m - j);
       } else {
-        finish4<GATED>(a, i, j, z, up);
+        finish4<GATED>(a, i, j, a.m, z, up);
       }
     }
     if (KG > 1) __syncthreads();
@@ -345,26 +345,26 @@ __global__ __launch_bounds__(256) void project_parts_kernel(const TileArgs t) {
     z += load4(part + k * plane, a.m - j);
     if (GATED) up += load4(part + k * plane + a.m, a.m - j);
   }
-  finish4<GATED>(a, i, j, z, up);
+  finish4<GATED>(a, i, j, a.m, z, up);
 }
 
 // ------------------------------------------------------------------ few rows
 
-// Up to 16 tokens: the call is W's stream.  A workgroup 16 rows of W (and, gated, their up rows), its waves share the sum over n, each with a ring in LDS that it fills itself with whole
-// lines of 128 bytes.  Four rows 5120 -> 17408, gated: 67 us, 5.3 TB/s (operands straight from memory in the matrix cores' order touch 64 bytes of a row at a time: 2.2 TB/s; eight rows
+// Up to 16 tokens: the call is W's stream.  A workgroup up to 16 rows of W (and, gated, their up rows), its waves share the sum over n, each with a ring in LDS that it fills itself with whole
+// lines of 128 bytes.  Four rows 5120 -> 17408, gated: 63.5 us, 5.6 TB/s; eight 17408 -> 5120: 32.9 us, 5.4 TB/s (operands straight from memory in the matrix cores' order touch 64 bytes of a row at a time: 2.2 TB/s; eight rows
 // an instruction without LDS: 4.7).
 template <bool GATED, bool ALIGNED, int WAVES, int STAGES, int XI>
-__global__ __launch_bounds__(64 * WAVES) void project_rows_kernel(const mf_project_args a) {
+__global__ __launch_bounds__(64 * WAVES) void project_rows_kernel(const mf_project_args a, uint32_t rows) {
   constexpr int kW = GATED ? 4 : 2, kLoads = kW + XI;
   extern __shared__ uint4 whole_lds[];
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4, j0 = blockIdx.x * 16;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4, j0 = blockIdx.x * rows, own = min(rows, a.m - j0);
   // a wave's share of n, in whole blocks
   const uint32_t share = ((a.n + 63) / 64 + WAVES - 1) / WAVES, from = min(wave * share * 64, a.n), to = min(from + share * 64, a.n), begin = to > from ? from : 0;
   RowAt<ALIGNED> at[kLoads];
 #pragma unroll
   for (int q = 0; q < kLoads; ++q) {
     const uint32_t row = q % 2 * 8 + lane / 8;
-    at[q] = ((q < kW ? static_cast<RowAt<ALIGNED>>(min(row, a.m - 1 - j0)) * a.w_stride : static_cast<RowAt<ALIGNED>>(min(row, a.t - 1)) * a.x_stride) + lane_piece(lane)) * 2;
+    at[q] = ((q < kW ? static_cast<RowAt<ALIGNED>>(min(row, own - 1)) * a.w_stride : static_cast<RowAt<ALIGNED>>(min(row, a.t - 1)) * a.x_stride) + lane_piece(lane)) * 2;
   }
   const uint16_t* w = a.w + static_cast<size_t>(j0) * a.w_stride + begin;
   f32x4_t sum = {}, up_sum = {};
@@ -376,21 +376,21 @@ __global__ __launch_bounds__(64 * WAVES) void project_rows_kernel(const mf_proje
   __syncthreads();
   if (wave) return;
   const uint32_t j = j0 + g * 4;
-  if (r >= a.t || j >= a.m) return;
+  if (r >= a.t || g * 4 >= own) return;
 #pragma unroll
   for (int v = 1; v < WAVES; ++v) {
     sum += part[v * 128 + lane];
     if (GATED) up_sum += part[v * 128 + 64 + lane];
   }
-  finish4<GATED>(a, r, j, sum, up_sum);
+  finish4<GATED>(a, r, j, j0 + own, sum, up_sum);
 }
 
 template <bool GATED, bool ALIGNED, int WAVES, int STAGES, int XI>
-hipError_t launch_rows(hipStream_t s, const mf_project_args& a) {
+hipError_t launch_rows(hipStream_t s, const mf_project_args& a, uint32_t rows) {
   constexpr int kLds = WAVES * STAGES * ((GATED ? 4 : 2) + XI) * 1024;
   const hipError_t e = allow_lds<project_rows_kernel<GATED, ALIGNED, WAVES, STAGES, XI>>(kLds, kLds);
   if (e != hipSuccess) return e;
-  project_rows_kernel<GATED, ALIGNED, WAVES, STAGES, XI><<<dim3((a.m + 15) / 16), 64 * WAVES, kLds, s>>>(a);
+  project_rows_kernel<GATED, ALIGNED, WAVES, STAGES, XI><<<dim3((a.m + rows - 1) / rows), 64 * WAVES, kLds, s>>>(a, rows);
   return hipGetLastError();
 }
 
@@ -414,7 +414,7 @@ constexpr uint64_t kMostPartBytes = 16u << 20;
 
 size_t project_workspace_bytes(uint32_t m, uint32_t n, uint32_t t, bool gated) {
   const uint64_t rows = gated ? 2ull * m : m;
-  if (t <= 8 || n < 512 || rows >= 32ull * device_cu_count()) return 0;  // (the smallest tiles have 32 rows)
+  if (t <= 16 || n < 512 || rows >= 32ull * device_cu_count()) return 0;  // (the smallest tiles have 32 rows)
   return static_cast<size_t>(std::min(kMostPartBytes, kMostParts * 4 * rows * t));
 }
 
@@ -439,10 +439,14 @@ template <bool GATED, bool ALIGNED>
 hipError_t launch_shape(hipStream_t s, TileArgs& t, float* workspace) {
   const mf_project_args& a = t.p;
   const uint32_t cus = device_cu_count(), rows = GATED ? 2 * a.m : a.m;
-  // few rows: two waves a workgroup where there are workgroups for every CU (17408 -> 5120, 4 rows: 35.6 us, four waves 39.8; 2816 -> two times 704: 5.0, 4.6); more than eight with
-  // as many go to tiles of 32 (17408 -> 5120, 12 rows: 41.8 us, here 46.1; 2816 -> two times 704: 6.0, 5.0)
-  if (a.t <= 8) return (a.m + 15) / 16 >= cus ? launch_rows<GATED, ALIGNED, 2, 4, 1>(s, a) : launch_rows<GATED, ALIGNED, 4, 3, 1>(s, a);
-  if (a.t <= 16 && (a.m + 15) / 16 < cus) return launch_rows<GATED, ALIGNED, 4, 3, 2>(s, a);
+  // Few rows: sixteen of W a workgroup while every CU has one at most, else as many as give every CU the same number of workgroups (8 rows 17408 -> 5120: 32.6 us with 10, 39.4 with 16;
+  // four 5120 -> 17408, gated: 65.9 with 14, 70.2 with 16).  Two waves where there are workgroups for every CU and one stream of W each (32.6 us, four waves 35.1), four where there are
+  // fewer (8192 -> 1024: 6.7, two 8.5) or two streams (12 rows 5120 -> 17408, gated: 69.6, two 74.9).
+  if (a.t <= 16) {
+    const uint32_t blocks = (a.m + 15) / 16, rounds = (blocks + cus - 1) / cus, few = rounds == 1 ? 16 : (a.m + cus * rounds - 1) / (cus * rounds);
+    if (GATED || blocks < cus) return a.t <= 8 ? launch_rows<GATED, ALIGNED, 4, 3, 1>(s, a, few) : launch_rows<GATED, ALIGNED, 4, 3, 2>(s, a, few);
+    return a.t <= 8 ? launch_rows<false, ALIGNED, 2, 4, 1>(s, a, few) : launch_rows<false, ALIGNED, 2, 4, 2>(s, a, few);
+  }
   int best = 0;
   uint32_t blocks = (a.n + 63) / 64, parts = 1;
   float least = 3.4e38f;

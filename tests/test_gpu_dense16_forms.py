@@ -12,8 +12,8 @@ from test_gpu_projection import make
 pytestmark = pytest.mark.gpu
 
 PROJECT = [  # t, n, m, gated: what they come to
-    (3, 264, 4100, 0), (2, 520, 4100, 1), (4, 263, 4100, 0), (6, 199, 4100, 1),  # few rows, two waves
-    (12, 264, 4100, 0), (13, 263, 4100, 1),  # as many rows as are left to tiles
+    (3, 264, 4100, 0), (2, 520, 4100, 1), (4, 263, 4100, 0), (6, 199, 4100, 1),  # few rows, nine of W a workgroup, two waves or (gated) four
+    (12, 264, 4100, 0), (13, 263, 4100, 1), (16, 263, 4100, 0), (9, 200, 9001, 0), (7, 136, 8195, 1), (8, 264, 4097, 0),  # up to 16 rows, of W 9 to 12 a workgroup
     (20, 4104, 33, 0), (20, 8199, 33, 1), (20, 5128, 33, 1), (300, 4104, 33, 0), (40, 4103, 260, 1), (513, 8200, 100, 1), (700, 8200, 130, 0),  # 32 x 32, 2 to 15 parts
     (40, 520, 4100, 0), (20, 520, 4100, 1), (20, 5128, 1100, 1), (20, 8200, 1100, 0),  # 32 x 64, 1 to 8 parts
     (100, 328, 4100, 0), (40, 327, 4100, 1), (40, 4103, 4100, 0), (700, 5128, 33, 1), (40, 8200, 1100, 1), (513, 8199, 33, 0),  # 64 x 64, 1 to 15 parts
