@@ -111,7 +111,7 @@ constexpr int largest_part(int n, int most) {
 // for the same lines at once (3 %).  What bounds it: with many large tiles the matrix cores, 60 % of the units' time busy (4096 rows 5120 -> 17408, gated: 1208 us, 1.21 PFLOP/s; the
 // library's product without the gate 1200 to 1275); with one round of tiles the way to memory, 0.53 us a block of 128 x 192 where the matrix cores need 0.32 (777 rows 1280 -> 5120:
 // 22 us); with few, that and what stands in front of the first block and behind the last (200 rows 2816 -> 2113: 9.6).  Waves of four or fewer (kSpread) deal their reads and
-// requests out among the matrix instructions by hand; with eight the scheduler's groups do as well with fewer registers.
+// requests out among the matrix instructions by hand; eight leave it to the scheduler's groups, as the order by hand would take registers that spill.
 template <int TM, int TN, int WM, int WN, int KG, int STAGES, bool GATED, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const TileArgs t) {
   constexpr bool kSpread = WM * WN <= 4;
