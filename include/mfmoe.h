@@ -756,7 +756,8 @@ mf_status mf_block_norm(mf_ctx* ctx, mf_stream stream, const mf_block_norm_args*
  * layers, the experts of a model that is compared against.  The calls below are those layers' products, what stands between the
  * projections and attention, and their experts, beside the routers and norms above.  Forward only. */
 
-/* What is applied to a product, in fp32.  z / (1 + e^-z); 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))); 0.5 z (1 + erf(z / sqrt 2)). */
+/* What is applied to a product, in fp32.  z / (1 + e^-z); 0.5 z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))); 0.5 z (1 + erf(z / sqrt 2)).
+ * Relative to its result each is good to 2^-19 for |z| <= 1 and to 2^-14 further out, where the result is 2^-119 or more; smaller ones may be 0. */
 typedef enum { MF_ACT_NONE = 0, MF_ACT_SILU = 1, MF_ACT_GELU_TANH = 2, MF_ACT_GELU = 3 } mf_activation;
 
 typedef struct {

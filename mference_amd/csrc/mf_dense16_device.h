@@ -13,12 +13,30 @@ __device__ __forceinline__ f32x4_t mfma16(const uint4& a, const uint4& b, const 
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// The activations on the hardware's exp2 and reciprocal (1 ulp each), from fp32 sums; the erf form on the library's erf.  The tanh form is
-// x / (1 + e^(-2u)), which is 0.5 x (1 + tanh u) without its cancellation.
+// z Phi(z) = z (1 + erf(z / sqrt 2)) / 2.  The tail H = erfc(|z| / sqrt 2) / 2 is e^(-z^2 / 2) t p(t), t = 1 / (1 + 0.35 |z|), p a least-maximum fit of degree 8 over
+// |z| <= 14 (2^-24.9 relative); Phi is H for negative arguments and 1 - H for the others, so that nothing cancels: 1 + erf in fp32 loses a twentieth of the result at -5
+// and all of it from -5.5 on.  2^-20.8 relative near 0, (z^2 + 19) 2^-23 far out.  777 rows 1280 -> 5120: 27.4 us, with 1 + the
+// library's erf 30.0, with its erfc 31.3.
+__device__ __forceinline__ float gelu(float z) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, __builtin_fabsf(z), 1.0f));
+  float p = -0.0291459281f;
+  p = __builtin_fmaf(p, t, 0.143971682f);
+  p = __builtin_fmaf(p, t, -0.255714238f);
+  p = __builtin_fmaf(p, t, 0.159174129f);
+  p = __builtin_fmaf(p, t, -0.0231098142f);
+  p = __builtin_fmaf(p, t, 0.105507992f);
+  p = __builtin_fmaf(p, t, 0.119832873f);
+  p = __builtin_fmaf(p, t, 0.139861867f);
+  p = __builtin_fmaf(p, t, 0.139621407f);
+  const float h = t * __builtin_amdgcn_exp2f(z * z * -0.72134752044f) * p;
+  return z * (z < 0.0f ? h : 1.0f - h);
+}
+
+// The activations on the hardware's exp2 and reciprocal (1 ulp each), from fp32 sums.  The tanh form is x / (1 + e^(-2u)), which is 0.5 x (1 + tanh u) without its cancellation.
 __device__ __forceinline__ float activate(float z, mf_activation act) {
   if (act == MF_ACT_SILU) return fast_silu(z);
   if (act == MF_ACT_GELU_TANH) return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.3022081986f * (z + 0.044715f * z * z * z)));
-  if (act == MF_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (act == MF_ACT_GELU) return gelu(z);
   return z;
 }
 
