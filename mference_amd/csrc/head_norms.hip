@@ -9,10 +9,12 @@ namespace mf {
 namespace {
 
 // Cosine and sine of a pair's angle at a row.  The number of turns is made and reduced to half a turn in fp64: 2^31 steps of a pair that turns once a step
-// leave 2^-22 of a turn.  A pair without an axis is not turned.
+// leave 2^-22 of a turn.  A pair without an axis is copied, since by cosine 1 and sine 0 an infinity in it would not stay alone: its sine is a NaN that no arithmetic makes.
+constexpr uint32_t kNoTurn = 0x7FEDCBA9u;
+__device__ __forceinline__ bool turns(const float2& cs) { return __float_as_uint(cs.y) != kNoTurn; }
 __device__ __forceinline__ float2 turn_of(const mf_head_norms_args& a, uint32_t pair, uint32_t row) {
   const uint32_t axis = a.axis_of_pair ? a.axis_of_pair[pair] : 0;
-  if (axis >= a.axes) return make_float2(1.0f, 0.0f);
+  if (axis >= a.axes) return make_float2(1.0f, __uint_as_float(kNoTurn));
   const double turns = a.positions[static_cast<size_t>(axis) * a.position_stride + row] * (static_cast<double>(a.inv_freq[pair]) * 0.15915494309189533577);
   float s, c;
   sincospif(2.0f * static_cast<float>(turns - __builtin_rint(turns)), &s, &c);
@@ -51,7 +53,7 @@ __device__ __forceinline__ void store_piece(uint16_t* p, const float (&y)[V]) {
 // of 32 + 8, 6.7 us, the loads and then the stores of one round.  The same bytes in heads of 72 (V = 4) 76 us, of 50 (V = 1) 110.
 template <int V>
 __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_args a, uint32_t log_lanes, uint32_t chunk, uint32_t chunks) {
-  __shared__ float2 turns[4][64 * V];
+  __shared__ float2 tables[4][64 * V];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint64_t task = static_cast<uint64_t>(blockIdx.x) * 4 + wave;
   if (task >= static_cast<uint64_t>(a.t) * chunks) return;  // (no barrier below)
@@ -78,13 +80,15 @@ __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_arg
   request(now, head);
   if (live && a.q.weight && a.q.heads) wq[0].load(a.q.weight + first), wq[1].load(a.q.weight + second);
   if (live && a.k.weight && a.k.heads) wk[0].load(a.k.weight + first), wk[1].load(a.k.weight + second);
-  float2* table = turns[wave];
+  float2* table = tables[wave];
   for (uint32_t p = lane; p < pairs; p += 64) table[p] = turn_of(a, p, row);
   issue_fence();  // (a wave's own LDS accesses keep their order)
   float c[V], s[V];
+  bool turn[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const float2 cs = rotates ? table[slot * V + e] : make_float2(1.0f, 0.0f);
+    turn[e] = rotates && turns(cs);
     c[e] = cs.x;
     s[e] = cs.y;
   }
@@ -111,20 +115,20 @@ __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_arg
     if (live && head < end) {
       uint16_t* out = (is_k ? a.k.out : a.q.out) + place(head, true);
       float y[2][V];
+      if (V > 1 && a.interleaved) {  // neighbours are a pair: of element i = h V + e pair i / 2 of the lane
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+        for (int p = 0; p < V; ++p) {
+          const float l = z[2 * p / V][2 * p % V], r = z[(2 * p + 1) / V][(2 * p + 1) % V];
+          y[2 * p / V][2 * p % V] = turn[p] ? l * c[p] - r * s[p] : l;
+          y[(2 * p + 1) / V][(2 * p + 1) % V] = turn[p] ? r * c[p] + l * s[p] : r;
+        }
+      } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          // (what is not rotated has cosine 1 and sine 0, but an infinity there would not stay alone)
-          float turned_to;
-          if (V > 1 && a.interleaved) {  // neighbours are a pair: of element i = h V + e pair i / 2 of the lane
-            const int i = h * V + e, j = i ^ 1, p = i / 2;
-            turned_to = i % 2 ? z[h][e] * c[p] + z[j / V][j % V] * s[p] : z[h][e] * c[p] - z[j / V][j % V] * s[p];
-          } else {
-            turned_to = h ? z[1][e] * c[e] + z[0][e] * s[e] : z[0][e] * c[e] - z[1][e] * s[e];
-          }
-          y[h][e] = rotates ? turned_to : z[h][e];
+          y[0][e] = turn[e] ? z[0][e] * c[e] - z[1][e] * s[e] : z[0][e];
+          y[1][e] = turn[e] ? z[1][e] * c[e] + z[0][e] * s[e] : z[1][e];
         }
+      }
       store_piece<V>(out + first, y[0]);
       store_piece<V>(out + second, y[1]);
     }
@@ -165,6 +169,10 @@ __global__ __launch_bounds__(256) void head_norms_any_kernel(const mf_head_norms
       const uint32_t i = a.interleaved ? 2 * p : p, j = a.interleaved ? 2 * p + 1 : p + pairs;
       out[i] = narrow_bf16(z[i] * cs.x - z[j] * cs.y);
       out[j] = narrow_bf16(z[j] * cs.x + z[i] * cs.y);
+      if (!turns(cs)) {  // (seldom: stored over the turned)
+        out[i] = narrow_bf16(z[i]);
+        out[j] = narrow_bf16(z[j]);
+      }
     }
     for (uint32_t e = rot + lane; e < a.head_dim; e += 64) out[e] = narrow_bf16(z[e]);
   }
