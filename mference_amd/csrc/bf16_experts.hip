@@ -175,9 +175,10 @@ __global__ __launch_bounds__(64 * kUpWaves) void experts_up_kernel(const Bf16Exp
       if (bias) gate += bf16_to_f(bias[j]), up += bf16_to_f(bias[f + j]);
       const float act = activate(gate, a.pool.activation) * up;
       const size_t to_at = static_cast<size_t>(list[base + column]) * f + j;
-      const uint16_t high = narrow_bf16(act);
+      // (nearer to 2^128 than to the last bf16: cut off, since the first term would be an infinity and the second cannot take that back)
+      const uint16_t near = narrow_bf16(act), high = __builtin_isfinite(act) && !__builtin_isfinite(bf16_to_f(near)) ? static_cast<uint16_t>(__float_as_uint(act) >> 16) : near;
       acts[to_at] = high;
-      acts[plane + to_at] = narrow_bf16(__builtin_isfinite(bf16_to_f(high)) ? act - bf16_to_f(high) : 0.0f);
+      acts[plane + to_at] = narrow_bf16(__builtin_isfinite(act) ? act - bf16_to_f(high) : 0.0f);
     }
   };
   if (XI == 2 && count - base > 8) rows_of(std::integral_constant<int, 2>{});
