@@ -1263,7 +1263,8 @@ mf_status mf_head_norms(mf_ctx* ctx, mf_stream stream, const mf_head_norms_args*
     if (!h->head_stride) h->head_stride = a.head_dim;
     if (!h->out_head_stride) h->out_head_stride = a.head_dim;
     const uint64_t row = static_cast<uint64_t>(h->heads) * h->head_stride, out_row = static_cast<uint64_t>(h->heads) * h->out_head_stride;
-    if ((!h->row_stride && row > ~0u) || (!h->out_row_stride && out_row > ~0u)) return MF_ERR_DIMENSION_MISMATCH;
+    // (one row has no row stride: its heads may lie anywhere, those of a long cache further apart than any row stride says)
+    if (a.t > 1 && ((!h->row_stride && row > ~0u) || (!h->out_row_stride && out_row > ~0u))) return MF_ERR_DIMENSION_MISMATCH;
     if (!h->row_stride) h->row_stride = static_cast<uint32_t>(row);
     if (!h->out_row_stride) h->out_row_stride = static_cast<uint32_t>(out_row);
     if (a.t == 0) continue;
