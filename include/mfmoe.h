@@ -815,7 +815,8 @@ typedef struct {
  * the reference's operators of this library.  Positions of several axes (time, height, width) turn the pairs that axis_of_pair gives
  * them.  The angle is reduced in fp64, so that far positions keep theirs; everything else is fp32.  head_dim 1 .. 1024, rotary_dim even,
  * 0 .. head_dim (0 without positions), axes 1 .. 8, heads 0 .. 65535, t 0 .. MF_MAX_ROWS.  What is written may share no memory with anything
- * else of the call but a head's own input in place (MF_ERR_INVALID_ARGUMENT).  Faster where head_dim and rotary_dim are multiples of 16
+ * else of the call but a head's own input in place (MF_ERR_INVALID_ARGUMENT); heads of the same strides are told apart
+ * element by element (a head's query beside its key), others by the columns or the ranges that they span.  Faster where head_dim and rotary_dim are multiples of 16
  * and all addresses and strides are of 16 bytes. */
 mf_status mf_head_norms(mf_ctx* ctx, mf_stream stream, const mf_head_norms_args* args);
 

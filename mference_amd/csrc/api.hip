@@ -1216,27 +1216,40 @@ mf_status mf_project(mf_ctx* ctx, mf_stream stream, const mf_project_args* args,
 
 namespace {
 
-// The bytes of t rows of heads as rows for rows_meet: rows of heads side by side, or heads of rows side by side.  False where rows or heads overlap.
+// t rows of heads: as they are, in bytes, and as rows for rows_meet (rows of heads side by side, or heads of rows side by side).
 struct HeadRows {
   Rows rows;
   uint64_t count;
+  uint64_t heads, row_stride, head_stride, width;
 };
+// false where rows or heads overlap
 bool head_rows(const void* p, uint64_t heads, uint64_t t, uint64_t row_stride, uint64_t head_stride, uint64_t dim, HeadRows* out) {
   const uint64_t across = (heads - 1) * head_stride + dim, along = (t - 1) * row_stride + dim;
   if ((heads == 1 || head_stride >= dim) && (t == 1 || row_stride >= across)) {
-    *out = {{p, 2 * (t == 1 ? std::max(row_stride, across) : row_stride), 2 * across}, t};
+    *out = {{p, 2 * (t == 1 ? std::max(row_stride, across) : row_stride), 2 * across}, t, heads, 2 * row_stride, 2 * head_stride, 2 * dim};
     return true;
   }
   if (row_stride >= dim && head_stride >= along) {
-    *out = {{p, 2 * head_stride, 2 * along}, heads};
+    *out = {{p, 2 * head_stride, 2 * along}, heads, heads, 2 * row_stride, 2 * head_stride, 2 * dim};
     return true;
   }
   return false;
 }
-bool heads_meet(const HeadRows& a, const HeadRows& b) {
+// Whether two sets of t rows of heads can share a byte.  Exact where their strides are the same (a head's query beside its key): two heads meet where they start less than a
+// head's width apart, and the rows that come nearest to that are found for every distance between two heads.
+bool heads_meet(const HeadRows& a, const HeadRows& b, uint64_t t) {
   const auto pa = reinterpret_cast<uintptr_t>(a.rows.p), pb = reinterpret_cast<uintptr_t>(b.rows.p);
   if (pa + (a.count - 1) * a.rows.stride + a.rows.width <= pb || pb + (b.count - 1) * b.rows.stride + b.rows.width <= pa) return false;
-  return rows_meet(a.rows, b.rows, std::max(a.count, b.count));
+  const bool same_rows = t == 1 || a.row_stride == b.row_stride, same_heads = a.heads == 1 || b.heads == 1 || a.head_stride == b.head_stride;
+  if (!same_rows || !same_heads) return rows_meet(a.rows, b.rows, std::max(a.count, b.count));
+  const auto head = static_cast<int64_t>(a.heads == 1 ? b.head_stride : a.head_stride), row = static_cast<int64_t>(a.row_stride), width = static_cast<int64_t>(a.width);
+  const auto most = static_cast<int64_t>(t - 1), delta = static_cast<int64_t>(pb - pa);
+  for (int64_t h = 1 - static_cast<int64_t>(a.heads); h < static_cast<int64_t>(b.heads); ++h) {
+    const int64_t apart = delta + h * head, rows = most ? std::min(std::max(-apart / row, -most), most) : 0;  // (towards zero: the nearest is this one or a neighbour)
+    for (int64_t i = std::max(rows - 1, -most); i <= std::min(rows + 1, most); ++i)
+      if (apart + i * row > -width && apart + i * row < width) return true;
+  }
+  return false;
 }
 
 }  // namespace
@@ -1281,8 +1294,8 @@ mf_status mf_head_norms(mf_ctx* ctx, mf_stream stream, const mf_head_norms_args*
   for (uint32_t i = 0; i < kinds; ++i) {
     if (rows_meet_any(out[i].rows, out[i].count, read)) return MF_ERR_INVALID_ARGUMENT;
     for (uint32_t j = 0; j < kinds; ++j) {
-      if (!(i == j && in_place[i]) && heads_meet(out[i], in[j])) return MF_ERR_INVALID_ARGUMENT;
-      if (i != j && heads_meet(out[i], out[j])) return MF_ERR_INVALID_ARGUMENT;
+      if (!(i == j && in_place[i]) && heads_meet(out[i], in[j], a.t)) return MF_ERR_INVALID_ARGUMENT;
+      if (i != j && heads_meet(out[i], out[j], a.t)) return MF_ERR_INVALID_ARGUMENT;
     }
   }
   const OnDevice on(ctx);

@@ -26,3 +26,26 @@ def test_one_row_of_a_long_cache(gpu):
         want, off = heads64(part, weight, positions.view(1, 1), freq, None, False, 1e-6, 0.0, 1.0)
         assert_near(got, want, off)
     assert torch.equal(whole[:, 4:], kept[:, 4:]) and all((v == 7).all() for v in around)
+
+
+@pytest.mark.parametrize("t", [1, 3, 130])
+@pytest.mark.parametrize("rows_first", [True, False])
+@pytest.mark.parametrize("dim, interleaved", [(128, False), (72, True), (50, False), (130, True)])
+def test_query_key_and_value_head_by_head(gpu, t, rows_first, dim, interleaved):
+    """queries and keys in place in a buffer that holds a head's query, key and value side by side, and queries to the place of the values"""
+    h = 4
+    whole = randn(generator(t + dim), *((t, h, 3, dim) if rows_first else (h, t, 3, dim))).bfloat16()
+    view = whole if rows_first else whole.transpose(0, 1)
+    kept = view.clone()
+    weights, freq = [randn(generator(k), dim).bfloat16() for k in range(2)], frequencies(dim // 2)
+    positions = torch.arange(t, dtype=torch.int32, device="cuda")
+    op = ops.HeadNorms(gpu, dim, freq, interleaved=interleaved, q_weight=weights[0], k_weight=weights[1])
+    want = [heads64(kept[:, :, i], weights[i], positions.view(1, -1), freq, None, interleaved, 1e-6, 0.0, 1.0) for i in range(2)]
+    op.encode(view[:, :, 0], view[:, :, 1], positions)
+    for i in range(2):
+        assert_near(view[:, :, i], *want[i])
+    assert torch.equal(view[:, :, 2], kept[:, :, 2])
+    view.copy_(kept)
+    op.encode(view[:, :, 0], positions=positions, q_out=view[:, :, 2])
+    assert_near(view[:, :, 2], *want[0])
+    assert torch.equal(view[:, :, :2], kept[:, :, :2])

@@ -2,13 +2,14 @@
 in for the context.  A call that passes every check reaches the HIP runtime, which has no device here (such calls are not made where there is
 one: no kernel may see these addresses)."""
 import ctypes as C
+import random
 
 import pytest
 import torch
 
 from mference_amd import _capi
 
-DIMENSION, LAUNCH = -2, -7
+INVALID, DIMENSION, LAUNCH = -1, -2, -7
 
 needs_no_device = pytest.mark.skipif(torch.cuda.device_count() > 0, reason="the accepted calls would be launched")
 
@@ -38,3 +39,46 @@ def test_one_row_of_a_long_cache(ctx):
     assert call(ctx, rows(0, 64, 0, far), None, 1, 128) == LAUNCH
     assert call(ctx, rows(0, 64, 0, far), None, 2, 128) == DIMENSION  # (of two rows it is one that no argument holds)
     assert call(ctx, rows(0, 64, 128, far), None, 2, 128) == LAUNCH
+
+
+@needs_no_device
+@pytest.mark.parametrize("t", [1, 2, 300])
+def test_queries_and_keys_head_by_head(ctx, t):
+    """a head's query, key and value side by side, in place and to another buffer of that kind; rows in front of heads and behind"""
+    h, dim = 5, 64
+    row, head = 3 * h * dim, 3 * dim
+    assert call(ctx, rows(0, h, row, head), rows(dim, h, row, head), t, dim) == LAUNCH
+    assert call(ctx, rows(2 * dim, h, row, head), rows(0, h, row, head), t, dim) == LAUNCH
+    assert call(ctx, rows(0, h, row, head, out=dim), None, t, dim) == LAUNCH
+    row, head = 3 * dim, 3 * dim * t
+    assert call(ctx, rows(0, h, row, head), rows(dim, h, row, head), t, dim) == LAUNCH
+
+
+def test_queries_and_keys_that_meet(ctx):
+    h, dim, t = 5, 64, 7
+    row, head = 3 * h * dim, 3 * dim
+    for shift in (1, dim - 1, head + dim - 1, head, row - dim + 1, row + 1, 2 * row + head - 1):
+        assert call(ctx, rows(0, h, row, head), rows(shift, h, row, head), t, dim) == INVALID, shift
+        assert call(ctx, rows(0, h, row, head, out=shift), None, t, dim) == INVALID, shift
+
+
+@needs_no_device
+def test_against_a_list_of_elements(ctx):
+    """two sets of the same strides at random places: refused exactly where they share an element"""
+    rng = random.Random(5)
+    seen = {INVALID: 0, LAUNCH: 0}
+    for _ in range(3000):
+        dim, t, hq, hk = rng.randint(1, 6), rng.randint(1, 5), rng.randint(1, 5), rng.randint(1, 5)
+        if rng.random() < 0.5:  # heads in rows
+            head = dim + rng.randint(0, 9)
+            row = (max(hq, hk) - 1) * head + dim + rng.randint(0, 9)
+        else:
+            row = dim + rng.randint(0, 9)
+            head = (t - 1) * row + dim + rng.randint(0, 9)
+        shift = rng.randint(0, 3 * (row + head))
+        a, b = (0, shift) if rng.random() < 0.5 else (shift, 0)
+        elements = lambda x, heads: {x + i * row + j * head + e for i in range(t) for j in range(heads) for e in range(dim)}
+        want = INVALID if elements(a, hq) & elements(b, hk) else LAUNCH
+        seen[want] += 1
+        assert call(ctx, rows(a, hq, row, head), rows(b, hk, row, head), t, dim) == want, (dim, t, hq, hk, row, head, a, b)
+    assert min(seen.values()) > 500
