@@ -796,12 +796,14 @@ typedef struct {
   uint32_t row_stride, head_stride, out_row_stride, out_head_stride; /* row strides 0: heads * head stride; head strides 0: head_dim */
 } mf_head_rows;
 
+#define MF_SAME_POSITIONS 0xFFFFFFFFu /* as position_stride: one row of positions is every axis's (text in a model of several axes) */
+
 typedef struct {
   mf_head_rows q, k;
   const int32_t* positions;     /* [axes, t], axis a of row i at a * position_stride + i; NULL: no rotation */
   const float* inv_freq;        /* [rotary_dim / 2]: the angle of a pair for each step of its position */
   const uint8_t* axis_of_pair;  /* [rotary_dim / 2], values 0 .. axes - 1 (others: the pair is not turned); NULL: axis 0 for all */
-  uint32_t t, head_dim, rotary_dim, axes, position_stride; /* position_stride 0: t */
+  uint32_t t, head_dim, rotary_dim, axes, position_stride; /* position_stride 0: t; MF_SAME_POSITIONS */
   int interleaved;              /* pair p is elements (2 p, 2 p + 1); else (p, p + rotary_dim / 2) */
   float eps, weight_bias;       /* weight_bias is added to both weights: 1 where a model stores them as differences from one */
   float rotation_scale;         /* times cosine and sine (scaled context windows); usually 1 */

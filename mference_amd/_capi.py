@@ -27,6 +27,7 @@ MAX_ADAPTER_TARGETS = 4    # MF_MAX_ADAPTER_TARGETS
 GATE_NONE, GATE_ROW, GATE_ELEMENT, GATE_CHANNEL = 0, 1, 2, 3
 ACT_NONE, ACT_SILU, ACT_GELU_TANH, ACT_GELU = 0, 1, 2, 3
 BF16_EXPERTS_ROWS = 64     # MF_BF16_EXPERTS_ROWS
+SAME_POSITIONS = 0xFFFFFFFF  # MF_SAME_POSITIONS
 
 STATUS_NAMES = {
     0: "MF_OK", -1: "MF_ERR_INVALID_ARGUMENT", -2: "MF_ERR_DIMENSION_MISMATCH",

@@ -1264,7 +1264,8 @@ mf_status mf_head_norms(mf_ctx* ctx, mf_stream stream, const mf_head_norms_args*
   if (a.positions) {
     if (a.axes == 0 || a.axes > 8) return MF_ERR_DIMENSION_MISMATCH;
     if (!a.position_stride) a.position_stride = a.t;
-    if (a.axes > 1 && a.position_stride < a.t) return MF_ERR_DIMENSION_MISMATCH;
+    if (a.position_stride == MF_SAME_POSITIONS) a.position_stride = 0;
+    else if (a.axes > 1 && a.position_stride < a.t) return MF_ERR_DIMENSION_MISMATCH;
     if (!aligned4(a.positions) || !aligned4(a.inv_freq)) return MF_ERR_INVALID_ARGUMENT;
   }
   HeadRows in[2], out[2];

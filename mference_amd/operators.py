@@ -20,7 +20,7 @@ import torch
 from . import _capi
 from ._capi import (ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU, BF16_EXPERTS_ROWS, BITS_2, BITS_4, BITS_8, BITS_TERNARY,
                     GATE_CHANNEL, GATE_ELEMENT, GATE_NONE, GATE_ROW, GROUP_SIZE, MAX_ADAPTER_RANK, MAX_ADAPTER_TARGETS, MAX_ADAPTERS, MAX_EXPERTS,
-                    MAX_ROWS, MAX_TOKENS, MAX_TOPK, ROUTER_FULL_SOFTMAX, ROUTER_TOPK_SOFTMAX, ExpertOffsets, MfError, check)
+                    MAX_ROWS, MAX_TOKENS, MAX_TOPK, ROUTER_FULL_SOFTMAX, ROUTER_TOPK_SOFTMAX, SAME_POSITIONS, ExpertOffsets, MfError, check)
 
 __all__ = [
     "MetalContext", "QuantizedTensor", "Quantization", "DequantInt4GEMV", "DequantInt4GEMVMultiX",
@@ -567,6 +567,15 @@ class HeadNorms:
             (q_weight, "q_weight", torch.bfloat16, head_dim), (k_weight, "k_weight", torch.bfloat16, head_dim),
             (inv_freq, "inv_freq", torch.float32, pairs), (axis_of_pair, "axis_of_pair", torch.uint8, pairs))]
         self._numbers = (eps, weight_bias, rotation_scale)
+        self._named = None if axis_of_pair is not None else 1
+
+    def _axes_named(self) -> int:
+        """how many axes the table names (numbers of 8 and more are none); read once, by the first call that gives the positions of one"""
+        if self._named is None:
+            if self.axis_of_pair.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise MfError(-1, "positions [t] beside a table of axes that no call has read yet, while a graph is captured: give [axes, t]")
+            self._named = 1 + max((axis for axis in self.axis_of_pair.tolist() if axis < 8), default=0)
+        return self._named
 
     @staticmethod
     def axes_of_sections(sections: Sequence[int], turns: bool = False, device="cuda") -> torch.Tensor:
@@ -600,7 +609,8 @@ class HeadNorms:
     def encode(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
                q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, stream=None) -> None:
         """q bf16 [t, heads, head_dim], k [t, kv heads, head_dim], views of a wider buffer or of any order of rows and heads among them;
-        in place without q_out / k_out.  positions int32 [t], or [axes, t]."""
+        in place without q_out / k_out.  positions int32 [axes, t], one row expanded over the axes where they share it; or [t] where no more
+        than one axis is named.  A pair whose axis is none of them is not turned."""
         ctx = self.context
         device = ctx.device.index
         if q.dim() != 3 or k is not None and k.dim() != 3:
@@ -631,10 +641,14 @@ class HeadNorms:
             axes = 1 if positions.dim() == 1 else positions.shape[0]
             if not 1 <= axes <= 8:
                 raise MfError(-2, f"{axes} axes")
+            if positions.dim() == 1 and self._axes_named() > 1:
+                raise MfError(-2, f"positions of one axis for a table of {self._axes_named()}: give [axes, t] (a row expanded over the axes where they share it)")
             if t > 1 and positions.stride(-1) != 1:
                 raise MfError(-1, "the positions of an axis must be contiguous")
             p_stride = positions.stride(0) if axes > 1 else t
-            if axes > 1 and not t <= p_stride <= _U32:
+            if axes > 1 and p_stride == 0:
+                p_stride = SAME_POSITIONS
+            elif axes > 1 and not t <= p_stride < SAME_POSITIONS:
                 raise MfError(-2, "the positions of the axes overlap, or are too far apart")
             at = _address(positions, "positions", torch.int32, device)
         if t == 0:

@@ -1,4 +1,4 @@
-"""Views of heads in mf_head_norms on the GPU, against the definition in 64 bits."""
+"""Views of heads and of positions in mf_head_norms on the GPU, against the definition in 64 bits."""
 import pytest
 import torch
 
@@ -49,3 +49,22 @@ def test_query_key_and_value_head_by_head(gpu, t, rows_first, dim, interleaved):
     op.encode(view[:, :, 0], positions=positions, q_out=view[:, :, 2])
     assert_near(view[:, :, 2], *want[0])
     assert torch.equal(view[:, :, :2], kept[:, :, :2])
+
+
+@pytest.mark.parametrize("t", [1, 40])
+@pytest.mark.parametrize("dim, interleaved", [(128, False), (72, True), (130, False)])
+def test_one_row_of_positions_for_all_axes(gpu, t, dim, interleaved):
+    """text in a model of three axes: a row of positions expanded over them turns as three equal rows do"""
+    pairs = dim // 2
+    whole, weight = randn(generator(t), t, 3, dim).bfloat16(), randn(generator(9), dim).bfloat16()
+    positions = torch.randint(0, 100000, (t,), generator=generator(3), device="cuda", dtype=torch.int32)
+    table = ops.HeadNorms.axes_of_sections((pairs - 2 * (pairs // 3), pairs // 3, pairs // 3), turns=True)
+    op = ops.HeadNorms(gpu, dim, frequencies(pairs), table, interleaved, q_weight=weight)
+    got, same = torch.empty_like(whole), torch.empty_like(whole)
+    op.encode(whole, positions=positions.expand(3, t), q_out=got)
+    op.encode(whole, positions=positions.expand(3, t).contiguous(), q_out=same)
+    assert torch.equal(got, same)
+    want, off = heads64(whole, weight, positions.expand(3, t), frequencies(pairs), table, interleaved, 1e-6, 0.0, 1.0)
+    assert_near(got, want, off)
+    with pytest.raises(ops.MfError):
+        op.encode(whole, positions=positions, q_out=got)
