@@ -815,7 +815,8 @@ typedef struct {
  *       positions[axis_of_pair[p], row] * inv_freq[p]
  * narrowed once.  RMSNorm.encodeBF16W (Kernels/Primitives/RMSNorm.swift:52-64) for heads, and the rotation behind it; no counterpart in
  * the reference's operators of this library.  Positions of several axes (time, height, width) turn the pairs that axis_of_pair gives
- * them.  The angle is reduced in fp64, so that far positions keep theirs; everything else is fp32.  head_dim 1 .. 1024, rotary_dim even,
+ * them.  A pair whose axis is none is copied.  The angle is reduced in fp64, so that far positions keep theirs; everything else is fp32,
+ * the squares of a head too: a head whose root mean square is 2^64 / sqrt(head_dim) or more overflows to a norm of 0.  head_dim 1 .. 1024, rotary_dim even,
  * 0 .. head_dim (0 without positions), axes 1 .. 8, heads 0 .. 65535, t 0 .. MF_MAX_ROWS.  What is written may share no memory with anything
  * else of the call but a head's own input in place (MF_ERR_INVALID_ARGUMENT); heads of the same strides are told apart
  * element by element (a head's query beside its key), others by the columns or the ranges that they span.  Faster where head_dim and rotary_dim are multiples of 16
@@ -839,8 +840,9 @@ typedef struct {
   mf_activation activation;
 } mf_bf16_expert_pool;
 
-/* The layer for a few tokens, in two launches (beyond eight tokens a third adds up the routes) that read each live expert once: for token i with experts idx[i, k] and weights w[i, k]
- * (from any of the routers above)
+/* The layer for a few tokens, in two launches (beyond eight tokens a third adds up the routes) that read live experts only, each once for
+ * every eight of its routes (beyond eight tokens: every sixteen; what is read again comes mostly from the caches): for token i with experts
+ * idx[i, k] and weights w[i, k] (from any of the routers above)
  *   y = narrow(residual + sum over k of w * (down_e a + down_bias_e) + sigmoid(shared_gate . x) * shared_down a_s)
  *   a = act(gate_e x + bias) * (up_e x + bias')
  * What mf_moe_decode_layer is for quantized experts (RealForwardRunner.swift:2811-3218), the routing given; no counterpart in the
