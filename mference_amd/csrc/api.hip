@@ -1240,8 +1240,9 @@ bool head_rows(const void* p, uint64_t heads, uint64_t t, uint64_t row_stride, u
 bool heads_meet(const HeadRows& a, const HeadRows& b, uint64_t t) {
   const auto pa = reinterpret_cast<uintptr_t>(a.rows.p), pb = reinterpret_cast<uintptr_t>(b.rows.p);
   if (pa + (a.count - 1) * a.rows.stride + a.rows.width <= pb || pb + (b.count - 1) * b.rows.stride + b.rows.width <= pa) return false;
+  if (!rows_meet(a.rows, b.rows, std::max(a.count, b.count))) return false;  // (column ranges of one buffer, the usual case, need no more)
   const bool same_rows = t == 1 || a.row_stride == b.row_stride, same_heads = a.heads == 1 || b.heads == 1 || a.head_stride == b.head_stride;
-  if (!same_rows || !same_heads) return rows_meet(a.rows, b.rows, std::max(a.count, b.count));
+  if (!same_rows || !same_heads) return true;
   const auto head = static_cast<int64_t>(a.heads == 1 ? b.head_stride : a.head_stride), row = static_cast<int64_t>(a.row_stride), width = static_cast<int64_t>(a.width);
   const auto most = static_cast<int64_t>(t - 1), delta = static_cast<int64_t>(pb - pa);
   for (int64_t h = 1 - static_cast<int64_t>(a.heads); h < static_cast<int64_t>(b.heads); ++h) {

@@ -636,20 +636,24 @@ class HeadNorms:
             raise MfError(-1, "positions and inv_freq come together")
         at = axes = p_stride = 0
         if positions is not None:
-            if positions.shape[-1] != t or positions.dim() not in (1, 2):
-                raise MfError(-2, f"positions {tuple(positions.shape)} for {t} rows")
-            axes = 1 if positions.dim() == 1 else positions.shape[0]
-            if not 1 <= axes <= 8:
-                raise MfError(-2, f"{axes} axes")
-            if positions.dim() == 1 and self._axes_named() > 1:
+            shape = positions.shape
+            if len(shape) not in (1, 2) or shape[-1] != t:
+                raise MfError(-2, f"positions {tuple(shape)} for {t} rows")
+            axes, p_stride = 1, t
+            if len(shape) == 2:
+                axes = shape[0]
+                if not 1 <= axes <= 8:
+                    raise MfError(-2, f"{axes} axes")
+                if axes > 1:
+                    p_stride = positions.stride(0)
+                    if p_stride == 0:
+                        p_stride = SAME_POSITIONS
+                    elif not t <= p_stride < SAME_POSITIONS:
+                        raise MfError(-2, "the positions of the axes overlap, or are too far apart")
+            elif self._axes_named() > 1:
                 raise MfError(-2, f"positions of one axis for a table of {self._axes_named()}: give [axes, t] (a row expanded over the axes where they share it)")
             if t > 1 and positions.stride(-1) != 1:
                 raise MfError(-1, "the positions of an axis must be contiguous")
-            p_stride = positions.stride(0) if axes > 1 else t
-            if axes > 1 and p_stride == 0:
-                p_stride = SAME_POSITIONS
-            elif axes > 1 and not t <= p_stride < SAME_POSITIONS:
-                raise MfError(-2, "the positions of the axes overlap, or are too far apart")
             at = _address(positions, "positions", torch.int32, device)
         if t == 0:
             return
