@@ -49,8 +49,8 @@ __device__ __forceinline__ void store_piece(uint16_t* p, const float (&y)[V]) {
 
 // A wave a row (or some of its heads, where there are few rows).  2^log_lanes lanes a head, each with V pairs: both elements of every pair in one lane, in two pieces of V that lie
 // together; what is not rotated is dealt out the same way.  The wave's lanes share the row's cosines and sines: each makes some, LDS hands them on while the first heads
-// are on their way.  The next heads are requested before this turn's are worked on.  What bounds it is memory: 8192 rows, 40 + 8 heads of 128, 201 MB in 39.4 us, 5.1 TB/s; at 777 rows
-// of 32 + 8, 6.7 us, the loads and then the stores of one round.  The same bytes in heads of 72 (V = 4) 76 us, of 50 (V = 1) 110.
+// are on their way.  The next heads are requested before this turn's are worked on.  What bounds it is memory: 8192 rows, 40 + 8 heads of 128, 201 MB in 38.1 us, 5.3 TB/s; at 777 rows
+// of 32 + 8, 6.5 us, the loads and then the stores of one round.  The same bytes in heads of 72 (V = 4) 75 us, of 50 (V = 1) 111.
 template <int V>
 __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_args a, uint32_t log_lanes, uint32_t chunk, uint32_t chunks) {
   __shared__ float2 tables[4][64 * V];
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_arg
 }
 
 // Heads that lanes cannot share out in equal pieces (an odd size, pairs of an odd number in a long head): a wave a head, the head in LDS.  The same bytes in heads
-// of 130: 223 us.
+// of 130: 222 us.
 __global__ __launch_bounds__(256) void head_norms_any_kernel(const mf_head_norms_args a) {
   __shared__ float rows[4][1024];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, heads = a.q.heads + a.k.heads;

@@ -108,9 +108,10 @@ constexpr int largest_part(int n, int most) {
 // of 64 values of n, a whole line of 128 bytes a row at a time, STAGES - 1 blocks ahead.  A block is two steps of the matrix cores; a wave reads a step's operands into
 // registers while the matrix cores work on the step before, so that a block costs one barrier and no wait for LDS.  The eight pieces of a row are turned by
 // the row's number, so that 16 lanes that read the same piece of 16 rows meet all banks.  A workgroup starts at a block of its own (`skew`), so that neighbours do not wait
-// for the same lines at once (3 %).  What bounds it: with many large tiles the matrix cores, 60 % of the units' time busy (4096 rows 5120 -> 17408, gated: 1208 us, 1.21 PFLOP/s; the
-// library's product without the gate 1200 to 1275); with one round of tiles the way to memory, 0.53 us a block of 128 x 192 where the matrix cores need 0.32 (777 rows 1280 -> 5120:
-// 22 us); with few, that and what stands in front of the first block and behind the last (200 rows 2816 -> 2113: 9.6).  Waves of four or fewer (kSpread) deal their reads and
+// for the same lines at once (3 %).  What bounds it is LDS, at 128 bytes a clock (119 measured): for a block of 128 x 192 the waves read 131 KB and the requests write 41, together
+// 0.56 us at 2.4 GHz; a block takes 0.53, the matrix cores need 0.32 of them (777 rows 1280 -> 5120, bias and gelu: 24.0 us, of which 10 stand in front of the first block and
+// behind the last and 3 are the bias and the gelu).  Of 256 x 256 LDS and the matrix cores need 0.85 us each of 1.5 (4096 rows 5120 -> 17408, gated: 1205 to 1225 us, 1.2 PFLOP/s; the library's
+// product without the gate 1194 to 1275).  200 rows 2816 -> 2113, tiles of 32 x 64: 9.6 us, 22 blocks one behind the other in either half of n, 0.27 each, and 4 around them.  Waves of four or fewer (kSpread) deal their reads and
 // requests out among the matrix instructions by hand; eight leave it to the scheduler's groups, as the order by hand would take registers that spill.
 template <int TM, int TN, int WM, int WN, int KG, int STAGES, bool GATED, bool ALIGNED>
 __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const TileArgs t) {
@@ -140,7 +141,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG) void project_tile_kernel(const T
   const uint16_t* src[kLoads];
   const uint32_t piece = lane_piece(lane), back = piece >= rest ? piece * 2 : 0;  // (elements; bytes)
   // Eight rows from a uniform base with one offset a lane for all of them, but where rows end among the eight: rows behind the last are that row again (their results are
-  // not stored).  Kept to so few registers because a spilled one, read back, would wait for every block that is on its way.
+  // not stored).  Kept to so few registers because a spilled one, read back, waits for every block that is on its way: 256 x 256 has 9 to 11 in scratch all the same, of which every
+  // second block reads six back right behind the next block's requests.
   const uint32_t x_edge = (min(a.t - i0, static_cast<uint32_t>(TM)) - 1) / 8 * 8, w_edge = (min(a.m - j0, kRows) - 1) / 8 * 8;
   constexpr bool kMixed = TM % (kLoads * 8) != 0;  // a wave may have rows of both
   const auto offset_of = [&](uint32_t most, uint32_t stride) { return (static_cast<At>(min(lane / 8, most)) * stride + piece) * 2; };  // (bytes)
