@@ -51,8 +51,9 @@ __device__ __forceinline__ void store_piece(uint16_t* p, const float (&y)[V]) {
 // together; what is not rotated is dealt out the same way.  The wave's lanes share the row's cosines and sines: each makes some, LDS hands them on while the first heads
 // are on their way.  The next heads are requested before this turn's are worked on.  What bounds it is memory: 8192 rows, 40 + 8 heads of 128, 201 MB in 38.1 us, 5.3 TB/s; at 777 rows
 // of 32 + 8, 6.5 us, the loads and then the stores of one round.  The same bytes in heads of 72 (V = 4) 75 us, of 50 (V = 1) 111.
+// Six waves a SIMD, 80 registers of a lane: with five, batches of 5120 to 6144 waves take a second round (6100 rows, 16 + 16 heads of 64: 13.6 us, 12.5 so).
 template <int V>
-__global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_args a, uint32_t log_lanes, uint32_t chunk, uint32_t chunks) {
+__global__ __launch_bounds__(256, 6) void head_norms_kernel(const mf_head_norms_args a, uint32_t log_lanes, uint32_t chunk, uint32_t chunks) {
   __shared__ float2 tables[4][64 * V];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint64_t task = static_cast<uint64_t>(blockIdx.x) * 4 + wave;
@@ -84,11 +85,11 @@ __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_arg
   for (uint32_t p = lane; p < pairs; p += 64) table[p] = turn_of(a, p, row);
   issue_fence();  // (a wave's own LDS accesses keep their order)
   float c[V], s[V];
-  bool turn[V];
+  uint32_t turn = 0;  // bit e: pair e of the lane has an axis
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const float2 cs = rotates ? table[slot * V + e] : make_float2(1.0f, 0.0f);
-    turn[e] = rotates && turns(cs);
+    turn |= rotates && turns(cs) ? 1u << e : 0u;
     c[e] = cs.x;
     s[e] = cs.y;
   }
@@ -119,14 +120,14 @@ __global__ __launch_bounds__(256) void head_norms_kernel(const mf_head_norms_arg
 #pragma unroll
         for (int p = 0; p < V; ++p) {
           const float l = z[2 * p / V][2 * p % V], r = z[(2 * p + 1) / V][(2 * p + 1) % V];
-          y[2 * p / V][2 * p % V] = turn[p] ? l * c[p] - r * s[p] : l;
-          y[(2 * p + 1) / V][(2 * p + 1) % V] = turn[p] ? r * c[p] + l * s[p] : r;
+          y[2 * p / V][2 * p % V] = (turn >> p & 1) ? l * c[p] - r * s[p] : l;
+          y[(2 * p + 1) / V][(2 * p + 1) % V] = (turn >> p & 1) ? r * c[p] + l * s[p] : r;
         }
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          y[0][e] = turn[e] ? z[0][e] * c[e] - z[1][e] * s[e] : z[0][e];
-          y[1][e] = turn[e] ? z[1][e] * c[e] + z[0][e] * s[e] : z[1][e];
+          y[0][e] = (turn >> e & 1) ? z[0][e] * c[e] - z[1][e] * s[e] : z[0][e];
+          y[1][e] = (turn >> e & 1) ? z[1][e] * c[e] + z[0][e] * s[e] : z[1][e];
         }
       }
       store_piece<V>(out + first, y[0]);
